@@ -1,0 +1,777 @@
+// KL(teacher || student) from a teacher that is known at k listed columns of each row, forward and
+// backward, for gfx950.
+//
+//   q_j           the teacher's probability of listed column j (softmax over the list, or exp(t - lse))
+//   row_loss      sum_j q_j (log q_j - log p_j)  [+ q_r (log q_r - log p_r), the unlisted columns as one]
+//   dstudent_j    (p_j sum(q) - q_j) scale;  unlisted, with the bucket: (p_j - q_r p_j / p_r) scale
+//
+// Bound by the student's row: 2 (+ 2) bytes per 16-bit logit against 12 bytes per listed column. One
+// workgroup per row: the list is turned into a small LDS table while the row is on its way into
+// registers, the row is folded into a running (maximum, sum) of its columns (of its UNLISTED columns
+// where the bucket is wanted: log p_r then never is the log of 1 - sum p, which loses every digit when
+// the student agrees with the list), and the gradient is written from the registers.
+//
+// Every unlisted column's gradient is one coefficient times exp2(z - m): the coefficient, the listed
+// columns and the loss are computed in 64 bits by the threads that hold the list (the loss is a small
+// difference of terms ten to a hundred times its size), the sweep over the row in fp32.
+#include "../../include/fm_hip_tokens.h"
+#include "fm_vocab.hip.h"
+
+using namespace fm;
+
+namespace {
+
+constexpr int kMaxList = 1024;
+constexpr int kSmallList = 128;
+constexpr uint16_t kEnd = 0xFFFFu;
+constexpr int kNoLead = 0x7fffffff;
+constexpr double kLn2d = 0.69314718055994530942;
+
+struct ListArgs {
+  const void* idx;
+  const void* teacher;
+  const float* teacher_lse;
+  int k;
+  bool idx64;
+  int teacher_dtype;
+  int probs;         // FM_TEACHER_PROBS
+  int tail;          // FM_TAIL_*
+  double inv_t;
+  float c;           // log2(e) / temperature, what the logits are multiplied by
+};
+
+__device__ __forceinline__ int64_t list_idx(const ListArgs& a, int64_t at) {
+  return a.idx64 ? static_cast<const int64_t*>(a.idx)[at] : (int64_t)static_cast<const int32_t*>(a.idx)[at];
+}
+__device__ __forceinline__ double list_value(const ListArgs& a, int64_t at) {
+  if (a.teacher_dtype == FM_F32) return (double)static_cast<const float*>(a.teacher)[at];
+  if (a.teacher_dtype == FM_BF16) return (double)Elem<bf16_t>::load1(static_cast<const bf16_t*>(a.teacher) + at);
+  return (double)Elem<f16_t>::load1(static_cast<const f16_t*>(a.teacher) + at);
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_max64(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const double w = __shfl_xor(v, o, 64);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+template <int NW, bool MAX>
+__device__ __forceinline__ double block_reduce64(double v, double* smem) {
+  v = MAX ? wave_max64(v) : wave_sum64(v);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) smem[wave] = v;
+  __syncthreads();
+  double r = smem[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) r = MAX ? (smem[i] > r ? smem[i] : r) : r + smem[i];
+  __syncthreads();
+  return r;
+}
+
+// Workgroup merge of per-thread running (maximum, sum): the maximum in fp32, the sums in 64 bits.
+struct Pair64 {
+  float m;
+  double s;
+};
+template <int NW>
+__device__ __forceinline__ Pair64 block_merge64(MaxSum v, double* smem, float* smemf) {
+  const float m = block_max<NW>(v.m, smemf);
+  return Pair64{m, block_reduce64<NW, false>((double)v.s * (double)fast_exp2(v.m - m), smem)};
+}
+
+// The list of one row in LDS. Distinct columns are found with an open-addressing table (a column's
+// first slot leads, the others hand their probability to it, added in slot order); the leaders hang
+// in per-thread chains: chain t holds the listed columns among the vectors that thread t sweeps, and
+// bit i of mask[t] says that there may be one in its i-th vector (bit 31: in the row's unaligned ends).
+template <int THREADS, int KCAP>
+struct ListShared {
+  static constexpr int kSlots = 2 * KCAP;
+  double q[KCAP];
+  double red[THREADS / 64];
+  float redf[THREADS / 64];
+  int hcol[kSlots];
+  int hlead[kSlots];
+  int col[KCAP];
+  float g[KCAP];
+  uint32_t mask[THREADS];
+  uint16_t nxt[KCAP];
+  uint16_t head[THREADS];
+  int redi[THREADS / 64];
+};
+
+// What a thread keeps of its slots (slot j * THREADS + tid) across the sweep.
+template <int SL>
+struct Mine {
+  int col[SL];       // -1: not the leader of a column
+  float x[SL];       // the student's logit there
+  double q[SL];
+};
+
+// place of a column in a table of SLOTS (a power of two): the high bits of a multiplicative hash, so
+// that columns a power of two apart spread too
+template <int SLOTS>
+__device__ __forceinline__ uint32_t hash_col(int col) {
+  return ((uint32_t)col * 2654435761u) >> (32 - __builtin_ctz(SLOTS));
+}
+
+template <typename T, int THREADS, int KCAP, int SL>
+__device__ __forceinline__ void list_load(const ListArgs& a, int64_t row, int64_t (&c)[SL], double (&t)[SL]) {
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    const int s = j * THREADS + (int)threadIdx.x;
+    c[j] = -1;
+    t[j] = 0.0;
+    if (s < a.k) {
+      c[j] = list_idx(a, row * a.k + s);
+      t[j] = list_value(a, row * a.k + s);
+    }
+  }
+}
+
+// Fills the LDS table and chains and returns the sum of q (NaN when a column is out of range);
+// *unique gets the number of distinct columns. All threads of the workgroup call it.
+template <typename T, int THREADS, int KCAP, int SL>
+__device__ __forceinline__ double list_build(const ListArgs& a, const T* rp, const RowSplit& sp, int64_t row, int v,
+                                             const int64_t (&c)[SL], const double (&t)[SL],
+                                             ListShared<THREADS, KCAP>& sh, Mine<SL>& mine, int* unique) {
+  constexpr int NW = THREADS / 64;
+  constexpr int EPV = Elem<T>::kVec;
+  constexpr int HS = ListShared<THREADS, KCAP>::kSlots;
+  const int tid = threadIdx.x;
+  for (int i = tid; i < HS; i += THREADS) { sh.hcol[i] = -1; sh.hlead[i] = kNoLead; }
+  sh.mask[tid] = 0u;
+  sh.head[tid] = kEnd;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    mine.col[j] = -1;
+    mine.x[j] = 0.f;
+    mine.q[j] = 0.0;
+    if (c[j] >= v) bad = true;
+    else if (c[j] >= 0) {
+      mine.col[j] = (int)c[j];
+      mine.x[j] = Elem<T>::load1(rp + c[j]);
+    }
+  }
+  // teacher probabilities of the used slots
+  if (a.probs == FM_TEACHER_PROBS) {
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mine.q[j] = t[j];
+  } else if (a.tail == FM_TAIL_RENORM) {
+    double mx = -__builtin_inf();
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mx = t[j] > mx ? t[j] : mx;
+    mx = block_reduce64<NW, true>(mx, sh.red);
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mine.q[j] = exp((t[j] - mx) * a.inv_t);
+  } else {
+    const double l = (double)a.teacher_lse[row];
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mine.q[j] = exp(t[j] * a.inv_t - l);
+  }
+  double sum = bad ? __builtin_nan("") : 0.0;
+#pragma unroll
+  for (int j = 0; j < SL; ++j) sum += mine.q[j];
+  sum = block_reduce64<NW, false>(sum, sh.red);      // its barriers also publish the cleared table
+  if (a.tail == FM_TAIL_RENORM) {
+    const double r = 1.0 / sum;
+#pragma unroll
+    for (int j = 0; j < SL; ++j) mine.q[j] *= r;
+    sum = sum * r;                                    // 1, or NaN
+  }
+  // distinct columns
+  int at[SL];
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    at[j] = -1;
+    if (mine.col[j] >= 0) {
+      const int s = j * THREADS + tid;
+      sh.q[s] = mine.q[j];
+      uint32_t h = hash_col<HS>(mine.col[j]);
+      for (;;) {       // at most KCAP of the 2 * KCAP places are taken, so this ends
+        const int was = atomicCAS(&sh.hcol[h], -1, mine.col[j]);
+        if (was == -1 || was == mine.col[j]) break;
+        h = (h + 1) % HS;
+      }
+      at[j] = (int)h;
+      atomicMin(&sh.hlead[h], s);
+    }
+  }
+  __syncthreads();
+  bool again[SL];
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    const int s = j * THREADS + tid;
+    again[j] = false;
+    if (s < KCAP) sh.col[s] = mine.col[j];       // -1 in an empty slot
+    if (at[j] >= 0) again[j] = sh.hlead[at[j]] != s;
+  }
+  __syncthreads();
+  // a leader with followers: mark the place (the key itself is no longer needed)
+#pragma unroll
+  for (int j = 0; j < SL; ++j) if (again[j]) { sh.hcol[at[j]] = -2; mine.col[j] = -1; mine.q[j] = 0.0; }
+  __syncthreads();
+  int lead = 0;
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    if (mine.col[j] < 0) continue;
+    const int s = j * THREADS + tid;
+    ++lead;
+    if (sh.hcol[at[j]] == -2) {
+      double q = mine.q[j];
+      for (int o = s + 1; o < a.k; ++o) {      // in slot order
+        const double more = sh.q[o];
+        if (sh.col[o] == mine.col[j]) q += more;
+      }
+      mine.q[j] = q;
+    }
+    // hang it into the chain of the thread that sweeps this column
+    const int col = mine.col[j];
+    int owner;
+    uint32_t bit;
+    if (col >= sp.head && col < sp.tail0) {
+      const int vec = (col - sp.head) / EPV;
+      owner = vec % THREADS;
+      bit = 1u << ((vec / THREADS) % 31);
+    } else {
+      const int e = col < sp.head ? col : sp.head + (col - sp.tail0);
+      owner = e % THREADS;
+      bit = 1u << 31;
+    }
+    atomicOr(&sh.mask[owner], bit);
+    // 16-bit exchange on the 32-bit word that holds the head
+    uint32_t* word = reinterpret_cast<uint32_t*>(&sh.head[owner & ~1]);
+    const int shift = (owner & 1) * 16;
+    uint32_t old = *word, seen;
+    do {
+      seen = old;
+      const uint32_t now = (seen & ~(0xFFFFu << shift)) | ((uint32_t)s << shift);
+      old = atomicCAS(word, seen, now);
+    } while (old != seen);
+    sh.nxt[s] = (uint16_t)(seen >> shift);
+  }
+  *unique = 0;
+  if (a.tail == FM_TAIL_BUCKET) {
+    lead = wave_sum_i(lead);
+    if ((tid & 63) == 0) sh.redi[tid >> 6] = lead;
+  }
+  __syncthreads();
+  if (a.tail == FM_TAIL_BUCKET) {
+    int u = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) u += sh.redi[i];
+    *unique = u;
+  }
+  return sum;
+}
+
+// value of the chain's entry for each element of the vector at col0: fn(element, slot)
+template <int EPV, int THREADS, int KCAP, typename F>
+__device__ __forceinline__ void walk(const ListShared<THREADS, KCAP>& sh, uint16_t head, int col0, F fn) {
+  for (uint32_t s = head; s != kEnd; s = sh.nxt[s]) {
+    const int d = sh.col[s] - col0;
+    if (d >= 0 && d < EPV) fn(d, (int)s);
+  }
+}
+
+// Gradient coefficients of a row and its loss (LOSS), from the merged pairs; the listed columns'
+// gradients go to sh.g. Returns the coefficient of an unlisted column: its gradient is
+// coef * exp2(x * c - rest.m).
+template <int THREADS, int KCAP, int SL, bool LOSS, bool GRAD>
+__device__ __forceinline__ float finish_row(const ListArgs& a, ListShared<THREADS, KCAP>& sh, const Mine<SL>& mine,
+                                            const Pair64& all, const Pair64& rest, double sum_q, int unique, int v,
+                                            double scale, float* loss_at) {
+  constexpr int NW = THREADS / 64;
+  const double lse2 = (double)all.m + log2(all.s);
+  double q_r = 0.0;
+  if (a.tail == FM_TAIL_BUCKET && unique < v) {
+    q_r = 1.0 - sum_q;
+    if (q_r < 0.0) q_r = 0.0;          // (a NaN stays)
+  }
+  const double total = sum_q + q_r;
+  double term = 0.0;
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    if (mine.col[j] < 0) continue;
+    const int s = j * THREADS + (int)threadIdx.x;
+    const double lp2 = (double)mine.x[j] * (double)a.c - lse2;
+    if (LOSS && !(mine.q[j] == 0.0)) term += mine.q[j] * (log(mine.q[j]) - lp2 * kLn2d);
+    if (GRAD) sh.g[s] = (float)((exp2(lp2) * total - mine.q[j]) * scale);
+  }
+  if (LOSS) {
+    term = block_reduce64<NW, false>(term, sh.red);
+    if (threadIdx.x == 0) {
+      if (!(q_r == 0.0)) term += q_r * (log(q_r) - ((double)rest.m + log2(rest.s) - lse2) * kLn2d);
+      if (sum_q != sum_q) term = sum_q;
+      *loss_at = (float)term;
+    }
+  }
+  if (!GRAD) return 0.f;
+  __syncthreads();                     // sh.g
+  double coef = total * exp2((double)rest.m - (double)all.m) / all.s;
+  if (!(q_r == 0.0)) coef -= q_r / rest.s;
+  // no unlisted column with any probability: their logits are -inf and their gradient 0
+  if (rest.s == 0.0 && q_r == 0.0) coef = 0.0;
+  return (float)(coef * scale);
+}
+
+// running (maximum, sum) of one vector; `skip` removes listed columns first
+template <typename T>
+__device__ __forceinline__ void fold(MaxSum& run, float (&x)[Elem<T>::kVec], float c) {
+  constexpr int EPV = Elem<T>::kVec;
+  float mx = x[0];
+#pragma unroll
+  for (int e = 1; e < EPV; ++e) mx = fmaxf(mx, x[e]);
+  const float cm = fmaxf(run.m, mx * c);
+  float acc = run.s * fast_exp2(run.m - cm);
+#pragma unroll
+  for (int e = 0; e < EPV; ++e) acc += fast_exp2(__builtin_fmaf(x[e], c, -cm));
+  run.m = cm;
+  run.s = acc;
+}
+
+// rows with a list among the first `n` (at least 1), read by every workgroup where n is small
+template <int THREADS>
+__device__ __forceinline__ float count_rows(const ListArgs& a, int64_t n, int* redi) {
+  int cnt = 0;
+  for (int64_t i = threadIdx.x; i < n; i += THREADS) cnt += list_idx(a, i * a.k) >= 0 ? 1 : 0;
+  cnt = wave_sum_i(cnt);
+  if ((threadIdx.x & 63) == 0) redi[threadIdx.x >> 6] = cnt;
+  __syncthreads();
+  int t = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) t += redi[i];
+  __syncthreads();
+  return t > 0 ? (float)t : 1.f;
+}
+
+// GRAD: loss and gradient, RI vectors a thread held in registers between the fold and the store,
+// what a row has beyond them read twice. !GRAD: loss and stats from one streaming read (RI vectors
+// a thread in flight).
+template <typename T, int THREADS, int KCAP, int RI, bool GRAD>
+__global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, ListArgs a, float* __restrict__ row_loss,
+                                                          float* __restrict__ stats, const float* __restrict__ n_valid,
+                                                          int count_n, T* dstudent, int v, bool vec_ok) {
+  constexpr int EPV = Elem<T>::kVec;
+  constexpr int NW = THREADS / 64;
+  constexpr int SL = (KCAP + THREADS - 1) / THREADS;
+  __shared__ ListShared<THREADS, KCAP> sh;
+  const int64_t row = blockIdx.x;
+  const T* rp = student + row * (int64_t)v;
+  T* gp = GRAD ? dstudent + row * (int64_t)v : nullptr;
+  const RowSplit sp = split_row<EPV>(row, v, vec_ok);
+  const int tid = threadIdx.x;
+  const int ne = edge_count(sp, v);
+  const bool bucket = a.tail == FM_TAIL_BUCKET;
+
+  if (list_idx(a, row * a.k) < 0) {     // no list: nothing is read, the gradient is zero
+    if (GRAD) {
+      const u32x4 zero = {0u, 0u, 0u, 0u};
+      for (int c = tid; c < sp.nvec; c += THREADS) store16_stream(gp + sp.head + (int64_t)c * EPV, zero);
+      for (int e = tid; e < ne; e += THREADS) Elem<T>::store1(gp + edge_col(sp, e), 0.f);
+    }
+    if (tid == 0) row_loss[row] = 0.f;
+    if (tid < 4 && stats != nullptr) stats[row * 4 + tid] = 0.f;
+    return;
+  }
+  // the list's loads go first: waiting for them then waits for nothing of the row
+  int64_t lc[SL];
+  double lt[SL];
+  list_load<T, THREADS, KCAP, SL>(a, row, lc, lt);
+  u32x4 raw[RI];
+  const int last = sp.nvec - 1;
+  if (sp.nvec > 0) {
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+      const int c = i * THREADS + tid;
+      raw[i] = load16_stream(rp + sp.head + (int64_t)(c < sp.nvec ? c : last) * EPV);
+    }
+  }
+  Mine<SL> mine;
+  int unique;
+  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, rp, sp, row, v, lc, lt, sh, mine, &unique);
+  const uint32_t mask = sh.mask[tid];
+  const uint16_t head = sh.head[tid];
+
+  MaxSum run{kNegBig, 0.f};
+  auto take = [&](u32x4& r, int c, int it) {
+    if (c >= sp.nvec) return;
+    float x[EPV];
+    Elem<T>::unpack(r, x);
+    if (bucket && ((mask >> (it % 31)) & 1u)) {
+      walk<EPV, THREADS, KCAP>(sh, head, sp.head + c * EPV, [&](int d, int) {
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) if (e == d) x[e] = -INFINITY;
+      });
+    }
+    fold<T>(run, x, a.c);
+  };
+  if (sp.nvec > 0) {
+#pragma unroll
+    for (int i = 0; i < RI; ++i) take(raw[i], i * THREADS + tid, i);
+    constexpr int UN = GRAD ? 2 : RI;
+    for (int c0 = RI * THREADS; c0 < sp.nvec; c0 += UN * THREADS) {
+      u32x4 more[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const T* at = rp + sp.head + (int64_t)clamp_col(c0 + u * THREADS + tid, sp.nvec) * EPV;
+        more[u] = GRAD ? load16(at) : load16_stream(at);
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        touch_whole(more[u]);
+        take(more[u], c0 + u * THREADS + tid, c0 / THREADS + u);
+      }
+    }
+  }
+  for (int e = tid; e < ne; e += THREADS) {
+    const int col = edge_col(sp, e);
+    float x = Elem<T>::load1(rp + col);
+    if (bucket && (mask >> 31)) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int) { x = -INFINITY; });
+    const float cm = fmaxf(run.m, x * a.c);
+    run.s = run.s * fast_exp2(run.m - cm) + fast_exp2(__builtin_fmaf(x, a.c, -cm));
+    run.m = cm;
+  }
+  const Pair64 rest = block_merge64<NW>(run, sh.red, sh.redf);
+  Pair64 all = rest;
+  if (bucket) {      // the listed columns join the unlisted ones
+    MaxSum w{rest.m, 0.f};
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (mine.col[j] >= 0) w.m = fmaxf(w.m, mine.x[j] * a.c);
+    all.m = block_max<NW>(w.m, sh.redf);
+    double s = tid == 0 ? rest.s * exp2((double)rest.m - (double)all.m) : 0.0;
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (mine.col[j] >= 0) s += exp2((double)mine.x[j] * (double)a.c - (double)all.m);
+    all.s = block_reduce64<NW, false>(s, sh.red);
+  }
+  double scale = a.inv_t;
+  if (GRAD) {
+    if (count_n > 0) scale /= (double)count_rows<THREADS>(a, count_n, sh.redi);
+    else if (n_valid != nullptr) scale /= (double)*n_valid;
+  }
+  const float coef = finish_row<THREADS, KCAP, SL, true, GRAD>(a, sh, mine, all, rest, sum_q, unique, v, scale,
+                                                               row_loss + row);
+  if (tid == 0 && stats != nullptr) {
+    stats[row * 4] = all.m;
+    stats[row * 4 + 1] = (float)all.s;
+    stats[row * 4 + 2] = rest.m;
+    stats[row * 4 + 3] = (float)rest.s;
+  }
+  if constexpr (GRAD) {
+    auto put = [&](u32x4& r, int c, int it) {
+      if (c >= sp.nvec) return;
+      float x[EPV], o[EPV];
+      Elem<T>::unpack(r, x);
+      const int col0 = sp.head + c * EPV;
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) o[e] = coef * fast_exp2(__builtin_fmaf(x[e], a.c, -rest.m));
+      if ((mask >> (it % 31)) & 1u) {
+        walk<EPV, THREADS, KCAP>(sh, head, col0, [&](int d, int s) {
+          const float g = sh.g[s];
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) if (e == d) o[e] = g;
+        });
+      }
+      store16_stream(gp + col0, Elem<T>::pack(o));
+    };
+    if (sp.nvec > 0) {
+#pragma unroll
+      for (int i = 0; i < RI; ++i) {
+        touch_whole(raw[i]);
+        put(raw[i], i * THREADS + tid, i);
+      }
+      for (int c0 = RI * THREADS; c0 < sp.nvec; c0 += 2 * THREADS) {
+        u32x4 more[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          more[u] = load16_stream(rp + sp.head + (int64_t)clamp_col(c0 + u * THREADS + tid, sp.nvec) * EPV);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          touch_whole(more[u]);
+          put(more[u], c0 + u * THREADS + tid, c0 / THREADS + u);
+        }
+      }
+    }
+    for (int e = tid; e < ne; e += THREADS) {
+      const int col = edge_col(sp, e);
+      float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), a.c, -rest.m));
+      if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { o = sh.g[s]; });
+      Elem<T>::store1(gp + col, o);
+    }
+  }
+}
+
+// The gradient from saved stats. chunks > 1: a workgroup takes one tile of THREADS * UN vectors of a
+// row (the row's unaligned ends go with its first tile); each tile builds the row's list again.
+template <typename T, int THREADS, int KCAP, int UN>
+__global__ __launch_bounds__(THREADS) void kl_topk_bwd_kernel(const T* student, ListArgs a,
+                                                              const float* __restrict__ stats,
+                                                              const float* __restrict__ n_valid,
+                                                              const float* __restrict__ grad_out, int grad_per_row,
+                                                              T* dstudent, int v, bool vec_ok, int chunks) {
+  constexpr int EPV = Elem<T>::kVec;
+  constexpr int SL = (KCAP + THREADS - 1) / THREADS;
+  __shared__ ListShared<THREADS, KCAP> sh;
+  const int64_t row = blockIdx.x / (unsigned)chunks;
+  const int chunk = (int)(blockIdx.x % (unsigned)chunks);
+  const T* rp = student + row * (int64_t)v;
+  T* gp = dstudent + row * (int64_t)v;
+  const RowSplit sp = split_row<EPV>(row, v, vec_ok);
+  const int tid = threadIdx.x;
+  const int ne = chunk == 0 ? edge_count(sp, v) : 0;
+  const int c_begin = chunk * THREADS * UN;
+  int c_end = chunks > 1 ? c_begin + THREADS * UN : sp.nvec;
+  if (c_end > sp.nvec) c_end = sp.nvec;
+
+  if (list_idx(a, row * a.k) < 0) {
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int c = c_begin + tid; c < c_end; c += THREADS) store16_stream(gp + sp.head + (int64_t)c * EPV, zero);
+    for (int e = tid; e < ne; e += THREADS) Elem<T>::store1(gp + edge_col(sp, e), 0.f);
+    return;
+  }
+  int64_t lc[SL];
+  double lt[SL];
+  list_load<T, THREADS, KCAP, SL>(a, row, lc, lt);
+  const Pair64 all{stats[row * 4], (double)stats[row * 4 + 1]}, rest{stats[row * 4 + 2], (double)stats[row * 4 + 3]};
+  double scale = a.inv_t;
+  if (grad_out != nullptr) scale *= (double)grad_out[grad_per_row ? row : 0];
+  if (n_valid != nullptr) scale /= (double)*n_valid;
+  Mine<SL> mine;
+  int unique;
+  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, rp, sp, row, v, lc, lt, sh, mine, &unique);
+  const uint32_t mask = sh.mask[tid];
+  const uint16_t head = sh.head[tid];
+  const float coef = finish_row<THREADS, KCAP, SL, false, true>(a, sh, mine, all, rest, sum_q, unique, v, scale, nullptr);
+  for (int c0 = c_begin; c0 < c_end; c0 += THREADS * UN) {
+    u32x4 raw[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      raw[u] = load16_stream(rp + sp.head + (int64_t)clamp_col(c0 + u * THREADS + tid, sp.nvec) * EPV);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int c = c0 + u * THREADS + tid;
+      touch_whole(raw[u]);
+      if (c < c_end) {
+        float x[EPV], o[EPV];
+        Elem<T>::unpack(raw[u], x);
+        const int col0 = sp.head + c * EPV;
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) o[e] = coef * fast_exp2(__builtin_fmaf(x[e], a.c, -rest.m));
+        if ((mask >> ((c / THREADS) % 31)) & 1u) {
+          walk<EPV, THREADS, KCAP>(sh, head, col0, [&](int d, int s) {
+            const float g = sh.g[s];
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) if (e == d) o[e] = g;
+          });
+        }
+        store16_stream(gp + col0, Elem<T>::pack(o));
+      }
+    }
+  }
+  for (int e = tid; e < ne; e += THREADS) {
+    const int col = edge_col(sp, e);
+    float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), a.c, -rest.m));
+    if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { o = sh.g[s]; });
+    Elem<T>::store1(gp + col, o);
+  }
+}
+
+// n_valid and (row_loss != nullptr) the reduced loss, one workgroup, fixed order, 64-bit sum
+__global__ __launch_bounds__(1024) void kl_topk_finalize_kernel(const float* __restrict__ row_loss, ListArgs a, int64_t n,
+                                                                int mean, float* __restrict__ loss,
+                                                                float* __restrict__ n_valid) {
+  __shared__ double sd[16];
+  __shared__ int si[16];
+  double s = 0.0;
+  int cnt = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    if (row_loss != nullptr) s += (double)row_loss[i];
+    cnt += list_idx(a, i * a.k) >= 0 ? 1 : 0;
+  }
+  s = wave_sum64(s);
+  cnt = wave_sum_i(cnt);
+  if ((threadIdx.x & 63) == 0) { sd[threadIdx.x >> 6] = s; si[threadIdx.x >> 6] = cnt; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = sd[0];
+    int c = si[0];
+    for (int i = 1; i < 16; ++i) { t += sd[i]; c += si[i]; }
+    const int nv = c > 0 ? c : 1;
+    *n_valid = (float)nv;
+    if (row_loss != nullptr) *loss = (float)(mean ? t / nv : t);
+  }
+}
+
+// up to this many rows every workgroup counts the listed rows itself; beyond, one launch counts
+constexpr int64_t kCountInKernel = 256;
+
+int check(const char* what, int64_t n, int64_t v, int k, int dtype, int index_bits, int teacher_dtype, int kind,
+          int tail, double temperature) {
+  FM_CHECK_ARG(n >= 0 && v > 0, "%s: bad shape n=%lld v=%lld", what, (long long)n, (long long)v);
+  FM_CHECK_ARG(k >= 1, "%s: k must be positive (got %d)", what, k);
+  FM_CHECK_ARG(dtype == FM_F32 || dtype == FM_F16 || dtype == FM_BF16, "%s: bad dtype %d", what, dtype);
+  FM_CHECK_ARG(teacher_dtype == FM_F32 || teacher_dtype == FM_F16 || teacher_dtype == FM_BF16,
+               "%s: bad teacher_dtype %d", what, teacher_dtype);
+  FM_CHECK_ARG(index_bits == 32 || index_bits == 64, "%s: index_bits must be 32 or 64 (got %d)", what, index_bits);
+  FM_CHECK_ARG(kind == FM_TEACHER_LOGITS || kind == FM_TEACHER_PROBS, "%s: bad teacher_kind %d", what, kind);
+  FM_CHECK_ARG(tail == FM_TAIL_RENORM || tail == FM_TAIL_DROP || tail == FM_TAIL_BUCKET, "%s: bad tail %d", what, tail);
+  FM_CHECK_ARG(temperature > 0.0 && temperature <= 3.0e38, "%s: temperature must be positive and finite", what);
+  if (n > 0x7fffffffLL || v > 0x7fffffffLL || k > kMaxList) {
+    fm_host::set_error("%s: n and v must be below 2^31 and k at most %d", what, kMaxList);
+    return FM_ERR_UNSUPPORTED;
+  }
+  return FM_OK;
+}
+
+ListArgs list_args(const void* idx, const void* teacher, const float* lse, int k, int index_bits, int teacher_dtype,
+                   int kind, int tail, double temperature) {
+  ListArgs a;
+  a.idx = idx; a.teacher = teacher; a.teacher_lse = lse; a.k = k; a.idx64 = index_bits == 64;
+  a.teacher_dtype = teacher_dtype; a.probs = kind; a.tail = tail; a.inv_t = 1.0 / temperature;
+  a.c = (float)(1.4426950408889634074 / temperature);
+  return a;
+}
+
+template <typename T, int KCAP>
+void launch_loss_grad(const void* student, const ListArgs& a, float* row_loss, float* stats, const float* n_valid,
+                      int count_n, void* dstudent, int64_t n, int v, bool vec_ok, hipStream_t st) {
+  const int64_t nvec = v / Elem<T>::kVec;
+#define GO(TH, RI)                                                                                           \
+  FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, true>), dim3((unsigned)n), dim3(TH), 0, st,                     \
+            static_cast<const T*>(student), a, row_loss, stats, n_valid, count_n, static_cast<T*>(dstudent), \
+            v, vec_ok)
+  if (nvec <= 256 * 2) GO(256, 2);
+  else if (nvec <= 256 * 8) GO(256, 8);
+  else if (nvec <= 512 * 8) GO(512, 8);
+  else if (nvec <= 1024 * 8) GO(1024, 8);
+  else GO(1024, 16);
+#undef GO
+}
+
+template <typename T, int KCAP>
+void launch_fwd(const void* student, const ListArgs& a, float* row_loss, float* stats, int64_t n, int v, bool vec_ok,
+                hipStream_t st) {
+  const int64_t nvec = v / Elem<T>::kVec;
+#define GO(TH, RI)                                                                                           \
+  FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, false>), dim3((unsigned)n), dim3(TH), 0, st,                    \
+            static_cast<const T*>(student), a, row_loss, stats, nullptr, 0, static_cast<T*>(nullptr), v, vec_ok)
+  if (nvec <= 256 * 8) GO(256, 4);
+  else GO(512, 4);
+#undef GO
+}
+
+template <typename T, int KCAP>
+void launch_bwd(const void* student, const ListArgs& a, const float* stats, const float* n_valid, const float* grad_out,
+                int per_row, void* dstudent, int64_t n, int v, bool vec_ok, hipStream_t st) {
+  const int64_t nvec = v / Elem<T>::kVec;
+#define GO(TH, UN)                                                                                            \
+  do {                                                                                                        \
+    int64_t chunks = (nvec + TH * UN - 1) / (TH * UN);                                                        \
+    if (chunks < 1 || n * chunks > 0x7fffffffLL) chunks = 1;                                                  \
+    FM_LAUNCH((kl_topk_bwd_kernel<T, TH, KCAP, UN>), dim3((unsigned)(n * chunks)), dim3(TH), 0, st,           \
+              static_cast<const T*>(student), a, stats, n_valid, grad_out, per_row, static_cast<T*>(dstudent), \
+              v, vec_ok, (int)chunks);                                                                        \
+  } while (0)
+  if (nvec <= 256 * 4) GO(256, 4);
+  else GO(1024, 4);
+#undef GO
+}
+
+#define FM_KLT_DISPATCH(dtype, k, FN, ...)                                          \
+  do {                                                                              \
+    const bool small__ = (k) <= kSmallList;                                         \
+    if ((dtype) == FM_F32) { if (small__) FN<float, kSmallList>(__VA_ARGS__); else FN<float, kMaxList>(__VA_ARGS__); }        \
+    else if ((dtype) == FM_BF16) { if (small__) FN<bf16_t, kSmallList>(__VA_ARGS__); else FN<bf16_t, kMaxList>(__VA_ARGS__); } \
+    else { if (small__) FN<f16_t, kSmallList>(__VA_ARGS__); else FN<f16_t, kMaxList>(__VA_ARGS__); }                          \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int fm_kl_topk_fwd(const void* student, const void* idx, const void* teacher, const float* teacher_lse,
+                   float* row_loss, float* stats, float* loss, float* n_valid, int64_t n, int64_t v, int k, int dtype,
+                   int index_bits, int teacher_dtype, int teacher_kind, int tail, double temperature, int reduction,
+                   fm_stream_t stream) {
+  const int rc = check("fm_kl_topk_fwd", n, v, k, dtype, index_bits, teacher_dtype, teacher_kind, tail, temperature);
+  if (rc != FM_OK) return rc;
+  FM_CHECK_ARG(reduction == FM_REDUCE_NONE || reduction == FM_REDUCE_SUM || reduction == FM_REDUCE_MEAN,
+               "fm_kl_topk_fwd: bad reduction %d", reduction);
+  FM_CHECK_ARG(reduction == FM_REDUCE_NONE || (loss && n_valid), "fm_kl_topk_fwd: NULL scalar output");
+  FM_CHECK_ARG(n == 0 || (student && idx && teacher && row_loss), "fm_kl_topk_fwd: NULL pointer");
+  FM_CHECK_ARG(n == 0 || teacher_lse || teacher_kind == FM_TEACHER_PROBS || tail == FM_TAIL_RENORM,
+               "fm_kl_topk_fwd: teacher logits need teacher_lse unless the list is renormalised");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const ListArgs a = list_args(idx, teacher, teacher_lse, k, index_bits, teacher_dtype, teacher_kind, tail, temperature);
+  if (n > 0) {
+    const bool vec_ok = fm_host::aligned16(student);
+    FM_KLT_DISPATCH(dtype, k, launch_fwd, student, a, row_loss, stats, n, (int)v, vec_ok, st);
+    FM_CHECK_LAUNCH("fm_kl_topk_fwd");
+  }
+  if (reduction != FM_REDUCE_NONE) {
+    hipLaunchKernelGGL(kl_topk_finalize_kernel, dim3(1), dim3(1024), 0, st, row_loss, a, n,
+                       reduction == FM_REDUCE_MEAN ? 1 : 0, loss, n_valid);
+    FM_CHECK_LAUNCH("fm_kl_topk_fwd(finalize)");
+  }
+  return FM_OK;
+}
+
+int fm_kl_topk_loss_grad(const void* student, const void* idx, const void* teacher, const float* teacher_lse,
+                         float* row_loss, float* stats, float* loss, float* n_valid, void* dstudent, int64_t n,
+                         int64_t v, int k, int dtype, int index_bits, int teacher_dtype, int teacher_kind, int tail,
+                         double temperature, int reduction, fm_stream_t stream) {
+  const int rc = check("fm_kl_topk_loss_grad", n, v, k, dtype, index_bits, teacher_dtype, teacher_kind, tail, temperature);
+  if (rc != FM_OK) return rc;
+  FM_CHECK_ARG(reduction == FM_REDUCE_SUM || reduction == FM_REDUCE_MEAN,
+               "fm_kl_topk_loss_grad: reduction must be sum or mean (got %d)", reduction);
+  FM_CHECK_ARG(loss && n_valid, "fm_kl_topk_loss_grad: NULL scalar output");
+  FM_CHECK_ARG(n == 0 || (student && idx && teacher && row_loss && dstudent), "fm_kl_topk_loss_grad: NULL pointer");
+  FM_CHECK_ARG(n == 0 || teacher_lse || teacher_kind == FM_TEACHER_PROBS || tail == FM_TAIL_RENORM,
+               "fm_kl_topk_loss_grad: teacher logits need teacher_lse unless the list is renormalised");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const ListArgs a = list_args(idx, teacher, teacher_lse, k, index_bits, teacher_dtype, teacher_kind, tail, temperature);
+  const bool mean = reduction == FM_REDUCE_MEAN;
+  if (n > 0) {
+    const bool count_here = mean && n <= kCountInKernel;
+    if (mean && !count_here) {
+      hipLaunchKernelGGL(kl_topk_finalize_kernel, dim3(1), dim3(1024), 0, st, nullptr, a, n, 0, loss, n_valid);
+      FM_CHECK_LAUNCH("fm_kl_topk_loss_grad(count)");
+    }
+    const bool vec_ok = fm_host::aligned16(student) && fm_host::aligned16(dstudent);
+    FM_KLT_DISPATCH(dtype, k, launch_loss_grad, student, a, row_loss, stats, mean ? n_valid : nullptr,
+                    count_here ? (int)n : 0, dstudent, n, (int)v, vec_ok, st);
+    FM_CHECK_LAUNCH("fm_kl_topk_loss_grad");
+  }
+  hipLaunchKernelGGL(kl_topk_finalize_kernel, dim3(1), dim3(1024), 0, st, row_loss, a, n, mean ? 1 : 0, loss, n_valid);
+  FM_CHECK_LAUNCH("fm_kl_topk_loss_grad(finalize)");
+  return FM_OK;
+}
+
+int fm_kl_topk_bwd(const void* student, const void* idx, const void* teacher, const float* teacher_lse,
+                   const float* stats, const float* n_valid, const float* grad_out, int grad_per_row, void* dstudent,
+                   int64_t n, int64_t v, int k, int dtype, int index_bits, int teacher_dtype, int teacher_kind,
+                   int tail, double temperature, fm_stream_t stream) {
+  const int rc = check("fm_kl_topk_bwd", n, v, k, dtype, index_bits, teacher_dtype, teacher_kind, tail, temperature);
+  if (rc != FM_OK) return rc;
+  if (n == 0) return FM_OK;
+  FM_CHECK_ARG(student && idx && teacher && stats && dstudent, "fm_kl_topk_bwd: NULL pointer");
+  FM_CHECK_ARG(student != dstudent, "fm_kl_topk_bwd: dstudent must not be the student buffer");
+  FM_CHECK_ARG(!grad_per_row || grad_out, "fm_kl_topk_bwd: a gradient per row needs grad_out");
+  FM_CHECK_ARG(teacher_lse || teacher_kind == FM_TEACHER_PROBS || tail == FM_TAIL_RENORM,
+               "fm_kl_topk_bwd: teacher logits need teacher_lse unless the list is renormalised");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const ListArgs a = list_args(idx, teacher, teacher_lse, k, index_bits, teacher_dtype, teacher_kind, tail, temperature);
+  const bool vec_ok = fm_host::aligned16(student) && fm_host::aligned16(dstudent);
+  FM_KLT_DISPATCH(dtype, k, launch_bwd, student, a, stats, n_valid, grad_out, grad_per_row, dstudent, n, (int)v, vec_ok, st);
+  FM_CHECK_LAUNCH("fm_kl_topk_bwd");
+  return FM_OK;
+}
+
+}  // extern "C"

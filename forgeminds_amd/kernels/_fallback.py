@@ -63,6 +63,49 @@ def kl_div_logits(student, teacher, reduction: str = "mean", temperature: float 
     return rows.sum() / max(rows.numel(), 1)
 
 
+def kl_div_topk(student, idx, teacher, teacher_lse=None, probs: bool = False, tail: str = "renorm",
+                reduction: str = "mean", temperature: float = 1.0):
+    """KL(teacher || student) from the teacher's values at the listed columns ``idx [..., k]``.
+
+    Rows whose first slot is negative are skipped, other negative slots are empty, a repeated
+    column counts once with the sum of its probabilities, a column past the row gives NaN.
+    """
+    s = _wide(student)
+    v = s.shape[-1]
+    logp = torch.log_softmax(s / temperature, dim=-1)
+    used = idx >= 0
+    col = idx.long().clamp(0, v - 1)
+    # the teacher's few values in the widest type at hand
+    t = torch.where(used, teacher.detach().double(), 0.0)
+    if not probs:
+        if tail == "renorm":
+            t = torch.where(used, t / temperature, -float("inf"))
+            t = torch.exp(t - torch.where(used[..., :1], t.amax(dim=-1, keepdim=True), 0.0))
+        else:
+            t = torch.where(used, torch.exp(t / temperature - teacher_lse.detach().double().unsqueeze(-1)), 0.0)
+    if tail == "renorm":
+        t = torch.where(used[..., :1], t / t.sum(dim=-1, keepdim=True), 0.0)
+    t = torch.where((idx >= v).any(dim=-1, keepdim=True), float("nan"), t)
+    q = torch.zeros_like(logp).scatter_add(-1, col, t.to(logp.dtype))
+    rows = torch.where(q == 0, 0.0, q * (torch.log(torch.where(q == 0, 1.0, q)) - logp)).sum(dim=-1)
+    if tail == "bucket":
+        listed = torch.zeros(logp.shape, dtype=torch.int32, device=logp.device).scatter_add(-1, col, used.int()) > 0
+        left = (1.0 - t.sum(dim=-1)).clamp(min=0).to(logp.dtype)
+        left = torch.where(listed.all(dim=-1) | (left == 0), 0.0, left)
+        some = left != 0
+        # rows without a bucket take a finite stand-in, so that no gradient meets an infinity
+        out = torch.where(some.unsqueeze(-1), logp.masked_fill(listed, -float("inf")), logp)
+        rows = rows + torch.where(some, left * (torch.log(torch.where(some, left, 1.0)) - torch.logsumexp(out, dim=-1)), 0.0)
+    live = used[..., 0]
+    rows = torch.where(live, rows, 0.0)
+    if reduction == "none":
+        return rows.float() if rows.dtype != torch.float64 else rows
+    total = rows.sum()
+    if reduction == "mean":
+        total = total / live.sum().clamp(min=1).to(total.dtype)
+    return total
+
+
 def cross_entropy(logits, labels, ignore_index: int = -100, reduction: str = "mean"):
     """fp32 loss of ``F.cross_entropy`` summed over valid rows (reference ``loss.py:63-70``).
 

@@ -1,4 +1,5 @@
-"""ctypes binding of ``libfmhip.so`` (the C ABI declared in ``include/fm_hip.h``).
+"""ctypes binding of ``libfmhip.so`` (the C ABI declared in ``include/fm_hip.h`` and, for the
+token-level entry points, ``include/fm_hip_tokens.h``).
 
 Nothing here computes: each wrapper checks shapes the kernels assume, resolves the current
 device and stream of the tensor, passes raw device pointers and raises ``RuntimeError`` with
@@ -28,6 +29,7 @@ _lib_err: "str | None" = None
 _lock = threading.Lock()
 
 _vp, _i64, _int, _f32, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
+_f64 = C.c_double
 
 # name -> (restype, argtypes); mirrors include/fm_hip.h one to one
 SIGNATURES = {
@@ -80,6 +82,13 @@ SIGNATURES = {
     "fm_route_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _vp]),
 }
 
+# the same for include/fm_hip_tokens.h
+TOKEN_SIGNATURES = {
+    "fm_kl_topk_fwd": (_int, [_vp] * 8 + [_i64, _i64] + [_int] * 6 + [_f64, _int, _vp]),
+    "fm_kl_topk_loss_grad": (_int, [_vp] * 9 + [_i64, _i64] + [_int] * 6 + [_f64, _int, _vp]),
+    "fm_kl_topk_bwd": (_int, [_vp] * 7 + [_int, _vp, _i64, _i64] + [_int] * 6 + [_f64, _vp]),
+}
+
 
 def _load():
     global _lib, _lib_err
@@ -92,7 +101,7 @@ def _load():
             return None
         try:
             lib = C.CDLL(LIB_PATH)
-            for name, (res, args) in SIGNATURES.items():
+            for name, (res, args) in {**SIGNATURES, **TOKEN_SIGNATURES}.items():
                 fn = getattr(lib, name)
                 fn.restype, fn.argtypes = res, args
         except (OSError, AttributeError) as exc:
@@ -447,6 +456,63 @@ def kl_bwd(s2, t2, lse_s, lse_t, grad_out, per_row: bool, grad_dtype, inv_temper
                                1 if per_row else 0, _ptr(g), n, v, dtype_code(s2.dtype),
                                dtype_code(grad_dtype), float(inv_temperature), float(scale),
                                _stream(s2)), "fm_kl_bwd")
+    return g
+
+
+# ------------------------------------------------------------------ KL from a teacher's list
+TAIL = {"renorm": 0, "drop": 1, "bucket": 2}
+
+
+def _list_args(idx2, teacher2, probs: bool, tail: str, temperature: float):
+    return (idx2.shape[1], 64 if idx2.dtype == torch.int64 else 32, dtype_code(teacher2.dtype), int(probs),
+            TAIL[tail], float(temperature))
+
+
+def kl_topk_fwd(s2, idx2, teacher2, lse_t, probs: bool, tail: str, temperature: float, reduction: str):
+    """-> (loss fp32 scalar or None, row_loss [n], stats [n, 4], n_valid fp32 scalar or None)."""
+    _dense(s2, idx2, teacher2, lse_t)
+    n, v = s2.shape
+    dev = s2.device
+    rows = torch.empty(n, device=dev, dtype=torch.float32)
+    stats = torch.empty(n, 4, device=dev, dtype=torch.float32)
+    scal = torch.empty(2, device=dev, dtype=torch.float32) if reduction != "none" else None
+    k, bits, tdt, kind, tl, temp = _list_args(idx2, teacher2, probs, tail, temperature)
+    loss, n_valid = (scal[0], scal[1]) if scal is not None else (None, None)
+    with _guard(dev):
+        _check(lib().fm_kl_topk_fwd(_ptr(s2), _ptr(idx2), _ptr(teacher2), _ptr(lse_t), _ptr(rows), _ptr(stats),
+                                    _ptr(loss), _ptr(n_valid), n, v, k, dtype_code(s2.dtype), bits, tdt, kind, tl,
+                                    temp, REDUCE[reduction], _stream(s2)), "fm_kl_topk_fwd")
+    return loss, rows, stats, n_valid
+
+
+def kl_topk_loss_grad(s2, idx2, teacher2, lse_t, probs: bool, tail: str, temperature: float, reduction: str,
+                      inplace: bool = False):
+    """-> (loss fp32 scalar, dstudent [n, v] for an upstream gradient of 1, row_loss [n]); the gradient
+    lands in ``s2`` itself when ``inplace``."""
+    _dense(s2, idx2, teacher2, lse_t)
+    n, v = s2.shape
+    dev = s2.device
+    buf = torch.empty(n + 2, device=dev, dtype=torch.float32)
+    g = s2 if inplace else torch.empty_like(s2)
+    k, bits, tdt, kind, tl, temp = _list_args(idx2, teacher2, probs, tail, temperature)
+    with _guard(dev):
+        _check(lib().fm_kl_topk_loss_grad(_ptr(s2), _ptr(idx2), _ptr(teacher2), _ptr(lse_t), buf.data_ptr() + 8,
+                                          None, buf.data_ptr(), buf.data_ptr() + 4, _ptr(g), n, v, k,
+                                          dtype_code(s2.dtype), bits, tdt, kind, tl, temp, REDUCE[reduction],
+                                          _stream(s2)), "fm_kl_topk_loss_grad")
+    return buf[0], g, buf[2:]
+
+
+def kl_topk_bwd(s2, idx2, teacher2, lse_t, stats, n_valid, grad_out, per_row: bool, probs: bool, tail: str,
+                temperature: float):
+    _dense(s2, idx2, teacher2, lse_t, stats, grad_out)
+    n, v = s2.shape
+    g = torch.empty_like(s2)
+    k, bits, tdt, kind, tl, temp = _list_args(idx2, teacher2, probs, tail, temperature)
+    with _guard(s2.device):
+        _check(lib().fm_kl_topk_bwd(_ptr(s2), _ptr(idx2), _ptr(teacher2), _ptr(lse_t), _ptr(stats), _ptr(n_valid),
+                                    _ptr(grad_out), 1 if per_row else 0, _ptr(g), n, v, k, dtype_code(s2.dtype),
+                                    bits, tdt, kind, tl, temp, _stream(s2)), "fm_kl_topk_bwd")
     return g
 
 

@@ -16,12 +16,13 @@ gradient is wrt the undivided student logits, with no T**2 factor.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _fallback as fb
 import typing
 
 from . import _hip, _ops
-from ._common import _note, fast_ok, tracing
+from ._common import _note, fast_ok, tracing, wants_grad
 
 _REDUCTIONS = ("mean", "sum", "none")
 
@@ -306,6 +307,152 @@ def kl_div_logits_topk(student: torch.Tensor, teacher: torch.Tensor, k: int,
                               index_dtype, bool(retain))
 
 
+# ------------------------------------------------------------------ from a teacher's list
+#: longest list a row may have on the kernel path
+MAX_LIST = 1024
+_TAILS = ("renorm", "drop", "bucket")
+
+
+def _list_rows(student, idx, teacher, teacher_lse, probs, tail):
+    """The dense two-dimensional views the kernels take (``teacher_lse`` only where it is read)."""
+    k = idx.shape[-1]
+    lse_t = None
+    if teacher_lse is not None and not probs and tail != "renorm":
+        lse_t = teacher_lse.detach().to(torch.float32).contiguous().view(-1)
+    return (student.contiguous().view(-1, student.shape[-1]), idx.contiguous().view(-1, k),
+            teacher.detach().contiguous().view(-1, k), lse_t)
+
+
+class _KLTopkFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, student, idx, teacher, teacher_lse, probs, tail, reduction, temperature, reuse, retain):
+        s2, i2, t2, lse_t = _list_rows(student, idx, teacher, teacher_lse, probs, tail)
+        ctx.meta = (student.shape, reduction, probs, tail, temperature)
+        ctx.spent = False
+        # as in _KLDivFn: the gradient is written in the forward, except where the upstream gradient
+        # has to come before the rounding (fp16) or is one per row
+        ctx.in_forward = reduction != "none" and student.dtype != torch.float16
+        if ctx.in_forward:
+            own = reuse and s2.data_ptr() == student.data_ptr()
+            loss, grad, _rows = _hip.kl_topk_loss_grad(s2.detach(), i2, t2, lse_t, probs, tail, temperature,
+                                                       reduction, own)
+            ctx.once = own or not retain
+            ctx.save_for_backward(*((grad,) if ctx.once else (grad, s2.detach(), i2, t2, lse_t)))
+            return loss
+        loss, rows, stats, n_valid = _hip.kl_topk_fwd(s2.detach(), i2, t2, lse_t, probs, tail, temperature, reduction)
+        ctx.save_for_backward(s2, i2, t2, lse_t, stats, n_valid if reduction == "mean" else None)
+        return rows.view(student.shape[:-1]) if reduction == "none" else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        shape, reduction, probs, tail, temperature = ctx.meta
+        nones = (None,) * 9
+        if ctx.in_forward:
+            grad = ctx.saved_tensors[0]
+            if ctx.spent:
+                if ctx.once:
+                    raise RuntimeError("kl_div_topk: the gradient buffer written in the forward was already "
+                                       "consumed by a backward pass; run the forward again, or pass retain=True "
+                                       "to keep the inputs for repeated backward passes")
+                _g, s2, i2, t2, lse_t = ctx.saved_tensors
+                _loss, grad, _rows = _hip.kl_topk_loss_grad(s2, i2, t2, lse_t, probs, tail, temperature, reduction)
+            ctx.spent = True
+            _hip.scale_inplace(grad, g.detach().to(torch.float32).contiguous())
+            return (grad.view(shape), *nones)
+        s2, i2, t2, lse_t, stats, n_valid = ctx.saved_tensors
+        g32 = g.detach().to(torch.float32).contiguous().view(-1)
+        grad = _hip.kl_topk_bwd(s2.detach(), i2, t2, lse_t, stats, n_valid, g32, reduction == "none", probs, tail,
+                                temperature)
+        return (grad.view(shape), *nones)
+
+
+def kl_div_topk(student: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
+                teacher_lse: "torch.Tensor | None" = None, probs: bool = False, tail: str = "renorm",
+                reduction: str = "mean", temperature: float = 1.0, reuse: bool = False,
+                retain: bool = False) -> torch.Tensor:
+    """``KL(teacher || student)`` from the teacher's values at ``k`` listed columns of each row.
+
+    For a stored or remote teacher: ``idx [..., k]`` (int32 or int64) are the columns, as
+    :func:`topk` or :func:`kl_div_logits_topk` return them, ``teacher [..., k]`` the values there,
+    ``student [..., V]`` the student's logits. Nothing like it exists in the reference, whose
+    distillation needs the teacher's whole row (``kernels/kl.py:194-238``).
+
+    * ``probs=False``: ``teacher`` holds logits, divided by ``temperature`` like the student's;
+      ``probs=True``: probabilities that are already at that temperature.
+    * ``tail="renorm"``: the teacher is its list, normalised to sum to one. ``"drop"``: the listed
+      probabilities as they are in the whole row, the rest ignored. ``"bucket"``: the same and
+      everything unlisted as one more outcome. The last two need ``teacher_lse [...]`` with logits:
+      the log-sum-exp of the teacher's whole row divided by ``temperature``.
+    * A negative entry of ``idx`` is an empty slot. A row whose first slot is empty is skipped (loss
+      and gradient 0): prompt tokens and padding. ``"mean"`` divides by the rows that are not skipped.
+    * A repeated column counts once, with the sum of its probabilities; a column ``>= V`` makes the
+      row's loss and gradient NaN.
+
+    Returns the fp32 loss (``"none"``: one per row). The teacher is a constant. ``temperature`` has
+    no ``T**2`` factor. ``reuse`` / ``retain`` as in :func:`kl_div_logits`.
+    """
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be mean|sum|none, got {reduction!r}")
+    if tail not in _TAILS:
+        raise ValueError(f"tail must be renorm|drop|bucket, got {tail!r}")
+    if not 0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if idx.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"idx must be int32 or int64, got {idx.dtype}")
+    if student.dim() < 1 or student.shape[-1] == 0 or not student.is_floating_point():
+        raise ValueError(f"student must be floating-point logits [..., V], got {tuple(student.shape)} {student.dtype}")
+    if (idx.shape != teacher.shape or idx.dim() != student.dim() or idx.shape[:-1] != student.shape[:-1]
+            or idx.shape[-1] == 0 or not teacher.is_floating_point()):
+        raise ValueError(f"kl_div_topk: student {tuple(student.shape)}, idx {tuple(idx.shape)}, teacher "
+                         f"{tuple(teacher.shape)} {teacher.dtype} disagree")
+    if not probs and tail != "renorm":
+        if teacher_lse is None:
+            raise ValueError(f"tail={tail!r} with teacher logits needs teacher_lse")
+        if teacher_lse.shape != student.shape[:-1]:
+            raise ValueError(f"teacher_lse must be {tuple(student.shape[:-1])}, got {tuple(teacher_lse.shape)}")
+    others = [idx, teacher] + ([teacher_lse] if teacher_lse is not None else [])
+    if any(t.device != student.device for t in others):
+        raise ValueError("kl_div_topk: student, idx, teacher and teacher_lse must be on one device")
+    temperature = float(temperature)
+    if student.numel() == 0 or idx.shape[-1] > MAX_LIST or tracing():
+        _note("kl_div_topk shape")
+        return fb.kl_div_topk(student, idx, teacher, teacher_lse, probs, tail, reduction, temperature)
+    if not _kernel_ok(student, teacher):
+        return fb.kl_div_topk(student, idx, teacher, teacher_lse, probs, tail, reduction, temperature)
+    if not wants_grad(student):
+        s2, i2, t2, lse_t = _list_rows(student, idx, teacher, teacher_lse, probs, tail)
+        loss, rows, _st, _nv = _hip.kl_topk_fwd(s2.detach(), i2, t2, lse_t, bool(probs), tail, temperature, reduction)
+        return rows.view(student.shape[:-1]) if reduction == "none" else loss
+    return _KLTopkFn.apply(student, idx, teacher, teacher_lse, bool(probs), tail, reduction, temperature,
+                           bool(reuse), bool(retain))
+
+
+def kl_distill_topk_loss(hs: torch.Tensor, w: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor, *,
+                         teacher_lse: "torch.Tensor | None" = None, probs: bool = False, tail: str = "renorm",
+                         temperature: float = 1.0, chunk: int = 4096) -> torch.Tensor:
+    """Mean :func:`kl_div_topk` of the student ``hs @ w.T`` over all rows that are not skipped,
+    ``chunk`` rows of logits at a time (:func:`kl_distill_loss` for a teacher that is a list)."""
+    if chunk < 1:
+        raise ValueError(f"chunk must be positive, got {chunk}")
+    rows = hs.reshape(-1, hs.shape[-1])
+    i2, t2 = idx.reshape(-1, idx.shape[-1]), teacher.reshape(-1, teacher.shape[-1])
+    lse = None if teacher_lse is None else teacher_lse.reshape(-1)
+    n = rows.shape[0]
+    if i2.shape[0] != n or t2.shape[0] != n or (lse is not None and lse.shape[0] != n):
+        raise ValueError(f"student has {n} rows, idx {i2.shape[0]}, teacher {t2.shape[0]}")
+    if n == 0:
+        return rows.new_zeros((), dtype=torch.float32)
+    w_t = w.t()
+    pieces = []
+    for lo in range(0, n, chunk):
+        part = slice(lo, lo + chunk)
+        # the block's logits are a temporary of this call: the gradient may overwrite them
+        pieces.append(kl_div_topk(rows[part] @ w_t, i2[part], t2[part], teacher_lse=None if lse is None else lse[part],
+                                  probs=probs, tail=tail, reduction="sum", temperature=temperature, reuse=True))
+    return torch.stack(pieces).sum() / (i2[:, 0] >= 0).sum().clamp(min=1)
+
+
 def _distill_piece(rows_s: torch.Tensor, rows_t: torch.Tensor, w_t: torch.Tensor, teacher_head) -> torch.Tensor:
     """Summed KL of one block of rows. The student logits of the block are a temporary of this
     call, so the kernel may write their gradient over them (``reuse=True``)."""
@@ -343,4 +490,5 @@ def kl_distill_loss(hs: torch.Tensor, ht: torch.Tensor, w: torch.Tensor, teacher
 kl_div = kl_div_logits
 distill_kl = kl_distill_loss
 
-__all__ = ["kl_div_logits", "kl_div_logits_topk", "kl_div", "kl_distill_loss", "distill_kl"]
+__all__ = ["kl_div_logits", "kl_div_logits_topk", "kl_div_topk", "kl_div", "kl_distill_loss", "kl_distill_topk_loss",
+           "distill_kl"]
