@@ -6,6 +6,8 @@
     loss = fm.kernels.cross_entropy(logits, labels)      # fp32, mean over valid rows
     loss = fm.kernels.kl_div_logits(student, teacher)    # KL(teacher || student)
     v, i = fm.kernels.topk(x, 64)                        # canonical, deterministic order
+    tok, logp = fm.kernels.sample_tokens(x, u, top_p=0.9)        # from given uniform numbers
+    loss = fm.kernels.kl_div_topk(student, i, v)         # from a teacher's listed columns
     r = fm.kernels.moe_route(router_logits, k=2)         # idx, weights, counts, slot, order
     xs = fm.kernels.moe_gather(x, r.order, 2, r.slot)    # tokens grouped by expert
     out = fm.kernels.moe_combine(ys, r.weights, r.slot, r.order)   # weighted return to tokens
@@ -33,6 +35,7 @@ from .layernorm import add_layer_norm, layer_norm
 from .norm import add_rms_norm, rms_norm
 from .rope import qk_norm_rope
 from .route import Routing, moe_route
+from .sample import sample_tokens
 from .softmax import softmax
 from .swiglu import swiglu, swiglu_split
 from .topk import topk
@@ -42,7 +45,7 @@ __all__ = [
     "rms_norm", "add_rms_norm", "qk_norm_rope", "swiglu", "swiglu_split",
     "layer_norm", "add_layer_norm", "kl_div_logits", "kl_div_logits_topk", "kl_div_topk", "kl_div", "kl_distill_loss",
     "kl_distill_topk_loss", "distill_kl",
-    "newton_schulz", "topk", "softmax", "cross_entropy", "moe_route", "Routing",
+    "newton_schulz", "topk", "softmax", "sample_tokens", "cross_entropy", "moe_route", "Routing",
     "moe_gather", "moe_combine",
     "enable", "patch", "revert", "available", "use_custom_ops",
 ]

@@ -156,3 +156,37 @@ def topk_canonical(x, k: int):
     second = torch.sort(composite, dim=-1, descending=True, stable=True).indices
     idx = torch.gather(order, -1, second)[..., :k]
     return torch.gather(x, -1, idx), idx
+
+
+def sample_tokens(x, u, temp, top_k, top_p, min_p):
+    """Token and log-probability per row of ``x [n, v]``; the settings are ``[n, 1]`` tensors.
+
+    64-bit weights and sums, like the kernel: a border between two tokens must not move.
+    """
+    n, v = x.shape
+    if x.numel() == 0:
+        return x.new_zeros(n, dtype=torch.int64), x.new_zeros(n, dtype=torch.float32)
+    temp, top_p, min_p = temp.double(), top_p.double(), min_p.double().clamp(max=1.0)
+    order = torch.sort(x.double(), dim=-1, descending=True, stable=True)
+    m = order.values[:, :1]
+    fine = torch.isfinite(m) & ~torch.isnan(x).any(dim=-1, keepdim=True) & (temp >= 0) & (temp < float("inf"))
+    greedy = temp == 0
+    safe_m = torch.where(fine, m, 0.0)
+    gap = torch.where(fine, order.values - safe_m, 0.0)
+    e = torch.exp(gap / torch.where(greedy | ~fine, 1.0, temp))
+    rank = torch.arange(v, device=x.device)[None, :]
+    keep = (top_k <= 0) | (top_k >= v) | (rank < top_k)
+    w = torch.where(keep, e, 0.0)
+    run = torch.cumsum(w, -1)
+    keep = keep & (~(top_p < 1) | (rank == 0) | ((run - w) < top_p * run[:, -1:]))
+    keep = keep & (~(min_p > 0) | (e >= min_p))
+    keep = torch.where(greedy, rank == 0, keep)
+    mass = torch.zeros_like(w).scatter_(1, order.indices, torch.where(keep, e, 0.0))
+    run = torch.cumsum(mass, -1)
+    total = run[:, -1:]
+    u = torch.where(u > 0, u, 0.0).clamp(max=1.0 - 2.0 ** -24).double().unsqueeze(-1)
+    token = torch.minimum((run <= u * total).sum(-1, keepdim=True),
+                          torch.where(mass > 0, rank, 0).max(-1, keepdim=True).values)
+    logprob = torch.log(mass.gather(1, token) / total)
+    return (torch.where(fine, token, -1).squeeze(-1),
+            torch.where(fine, logprob, float("nan")).squeeze(-1).float())

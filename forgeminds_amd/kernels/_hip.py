@@ -87,6 +87,7 @@ TOKEN_SIGNATURES = {
     "fm_kl_topk_fwd": (_int, [_vp] * 8 + [_i64, _i64] + [_int] * 6 + [_f64, _int, _vp]),
     "fm_kl_topk_loss_grad": (_int, [_vp] * 9 + [_i64, _i64] + [_int] * 6 + [_f64, _int, _vp]),
     "fm_kl_topk_bwd": (_int, [_vp] * 7 + [_int, _vp, _i64, _i64] + [_int] * 6 + [_f64, _vp]),
+    "fm_sample": (_int, [_vp] * 6 + [_f32, _int, _f32, _f32, _vp, _vp, _i64, _i64, _int, _vp]),
 }
 
 
@@ -548,6 +549,22 @@ def softmax_bwd(y2, dy2):
         _check(lib().fm_softmax_bwd(_ptr(y2), _ptr(dy2), _ptr(dx), n, v, dtype_code(y2.dtype),
                                     _stream(y2)), "fm_softmax_bwd")
     return dx
+
+
+def sample(logits2, u, temperature, top_k, top_p, min_p):
+    """-> (token int64 [n], logprob fp32 [n]); each setting is a number or a tensor [n] (fp32; top_k int32)."""
+    settings = (temperature, top_k, top_p, min_p)
+    per_row = [t if torch.is_tensor(t) else None for t in settings]
+    whole = [0 if torch.is_tensor(t) else t for t in settings]
+    _dense(logits2, u, *per_row)
+    n, v = logits2.shape
+    token = torch.empty(n, device=logits2.device, dtype=torch.int64)
+    logprob = torch.empty(n, device=logits2.device, dtype=torch.float32)
+    with _guard(logits2.device):
+        _check(lib().fm_sample(_ptr(logits2), _ptr(u), *(_ptr(t) for t in per_row), float(whole[0]), int(whole[1]),
+                               float(whole[2]), float(whole[3]), _ptr(token), _ptr(logprob), n, v,
+                               dtype_code(logits2.dtype), _stream(logits2)), "fm_sample")
+    return token, logprob
 
 
 _ROUTE_WS: dict = {}     # (rows, experts, k) -> workspace bytes, until a tuning parameter changes

@@ -60,6 +60,27 @@ int fm_kl_topk_bwd(const void* student, const void* idx, const void* teacher, co
                    void* dstudent, int64_t n, int64_t v, int k, int dtype, int index_bits, int teacher_dtype,
                    int teacher_kind, int tail, double temperature, fm_stream_t stream);
 
+/* ------------------------------------------------------------------ sampling
+ * One token per row of logits [n, v] from one uniform number per row. With T the temperature,
+ * m the row's maximum and e_j = exp((x_j - m) / T), and the order "value descending, index ascending":
+ *   top_k   > 0 (and below v): only the first top_k of the order stay;
+ *   top_p   < 1: rank r stays iff the mass before it is below top_p times the mass top_k left
+ *           (rank 0 always stays);
+ *   min_p   > 0: only e_j >= min_p stay (values above 1 count as 1);
+ *   token   = the first column (ascending) whose running sum of the e that stay exceeds u times their
+ *           sum; logprob = log(e_token / sum).
+ * T == 0 takes the first maximum (logprob 0), whatever the filters. A row that has no distribution --
+ * it holds a NaN or +inf or nothing but -inf, or T is negative, infinite or NaN -- gets token -1 and
+ * logprob NaN. u counts as at most the largest fp32 below 1 and at least 0 (NaN: 0). top_p or min_p
+ * NaN: off. Logits of -inf are never taken.
+ * u: fp32 [n]. temperature, top_p, min_p: fp32 [n] or NULL for the number behind them for every row;
+ * top_k: int32 [n] or NULL likewise. token: int64 [n]; logprob: fp32 [n] or NULL. logits may have any
+ * alignment of their type. Weights and sums are held in 64 bits. v <= 2^20. */
+int fm_sample(const void* logits, const float* u, const float* temperature, const int32_t* top_k,
+              const float* top_p, const float* min_p, float temperature0, int top_k0, float top_p0,
+              float min_p0, int64_t* token, float* logprob, int64_t n, int64_t v, int dtype,
+              fm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -77,3 +77,39 @@ def kl_topk(student, idx, teacher, lse=None, probs=False, tail="renorm", tempera
             size[i, out] += left * share
     return (torch.from_numpy(loss), torch.from_numpy(grad / temperature), torch.from_numpy(size / temperature),
             torch.from_numpy(valid))
+
+
+def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One row: (token, logprob, margin). ``margin`` is how far, relative to the mass, the nearest
+    decision (the cut of top-p, the border of the token) is from falling otherwise."""
+    x = np.asarray(x, np.float64)
+    if np.isnan(x).any() or not np.isfinite(x.max()) or not 0 <= temperature < math.inf:
+        return -1, math.nan, 1.0
+    if temperature == 0:
+        return int(np.argmax(x)), 0.0, 1.0
+    with np.errstate(over="ignore"):
+        e = np.exp((x - x.max()) / temperature)
+    order = sorted(range(x.size), key=lambda j: (-x[j], j)) if x.size < 5000 else list(np.argsort(-x, kind="stable"))
+    margin = 1.0
+    if 0 < top_k < x.size:
+        order = order[:top_k]
+    if top_p < 1:
+        total = math.fsum(e[order])
+        goal = top_p * total
+        before, kept = 0.0, []
+        run = np.concatenate([[0.0], np.cumsum(e[order])])
+        kept = [j for r, j in enumerate(order) if r == 0 or run[r] < goal]
+        if top_p > 0:
+            margin = min(margin, float(np.abs(run[1:-1] - goal).min()) / total if len(order) > 1 else 1.0)
+        order = kept
+    if min_p > 0:
+        order = [j for j in order if e[j] >= min(min_p, 1.0)]
+    order = np.array(sorted(order))
+    run = np.cumsum(e[order])
+    u = min(max(float(u), 0.0), 1 - 2.0 ** -24) if u == u else 0.0
+    r = u * run[-1]
+    at = int(np.searchsorted(run, r, side="right"))
+    if u > 0 and order.size > 1:
+        margin = min(margin, float(np.abs(run[:-1] - r).min()) / run[-1])
+    at = min(at, int(np.nonzero(e[order])[0][-1]))
+    return int(order[at]), math.log(e[order[at]] / run[-1]), margin
