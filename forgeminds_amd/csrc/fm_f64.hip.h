@@ -1,0 +1,91 @@
+// 64-bit helpers of the token-level kernels: reductions by DPP, 2^t and log2 with few live registers.
+// 64-bit vector operations run at the rate of 32-bit ones on this part, so what a result's exactness
+// hangs on is simply computed in 64 bits.
+#pragma once
+
+#include "fm_vocab.hip.h"
+
+namespace fm {
+
+constexpr double kLn2d = 0.69314718055994530942;
+constexpr double kLog2ed = 1.4426950408889634074;
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double readlane64(double v, int l) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, l);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), l);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+struct Sum64 { __device__ static __forceinline__ double f(double a, double b) { return a + b; } };
+struct Max64 { __device__ static __forceinline__ double f(double a, double b) { return b > a ? b : a; } };
+
+// over aligned groups of G lanes (4, 8, 16 or 64), the result in every lane, fixed order
+template <int G, typename Op>
+__device__ __forceinline__ double group_reduce64(double v) {
+  v = Op::f(v, dpp64<kDppXor1>(v));
+  v = Op::f(v, dpp64<kDppXor2>(v));
+  if constexpr (G >= 8) v = Op::f(v, dpp64<kDppHalfMirror>(v));
+  if constexpr (G >= 16) v = Op::f(v, dpp64<kDppMirror>(v));
+  if constexpr (G == 64)
+    v = Op::f(Op::f(readlane64(v, 0), readlane64(v, 16)), Op::f(readlane64(v, 32), readlane64(v, 48)));
+  return v;
+}
+__device__ __forceinline__ double wave_sum64(double v) { return group_reduce64<64, Sum64>(v); }
+
+// across the NW waves of a workgroup; the waves' results are combined by lanes rather than by every
+// thread reading all of them (32 registers beside a held row)
+template <int NW, typename Op>
+__device__ __forceinline__ double block_reduce64(double v, double* smem) {
+  v = group_reduce64<64, Op>(v);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) smem[wave] = v;
+  __syncthreads();
+  v = group_reduce64<NW, Op>(smem[lane & (NW - 1)]);
+  __syncthreads();
+  return v;
+}
+template <int NW>
+__device__ __forceinline__ float block_max32(float v, float* smem) {
+  v = wave_max(v);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) smem[wave] = v;
+  __syncthreads();
+  v = group_reduce<NW, OpMax>(smem[lane & (NW - 1)]);
+  __syncthreads();
+  return v;
+}
+
+// 2^t: degree-8 polynomial through the Chebyshev nodes of [-1/2, 1/2] (relative error 1.1e-12) and an
+// exact scaling. Below 2^-1100 the result is zero; NaN stays.
+__device__ __forceinline__ double exp2_64(double t) {
+  t = t < -1100.0 ? -1100.0 : t;
+  const double n = __builtin_rint(t);
+  const double f = t - n;
+  double r = 1.3255224878668817e-06;
+  r = __builtin_fma(r, f, 1.5310079402249296e-05);
+  r = __builtin_fma(r, f, 0.00015403455852453838);
+  r = __builtin_fma(r, f, 0.0013333450568000645);
+  r = __builtin_fma(r, f, 0.009618129159402558);
+  r = __builtin_fma(r, f, 0.05550410941205933);
+  r = __builtin_fma(r, f, 0.2402265069581299);
+  r = __builtin_fma(r, f, 0.6931471805459335);
+  r = __builtin_fma(r, f, 1.0);
+  return __builtin_amdgcn_ldexp(r, (int)n);
+}
+// the fp32 logarithm of the mantissa, corrected by the first two terms of log(1 + r) for what is left
+__device__ __forceinline__ double log2_64(double x) {
+  const double m = __builtin_amdgcn_frexp_mant(x);
+  const double y = (double)fast_log2((float)m);
+  const double r = __builtin_fma(m, exp2_64(-y), -1.0);
+  const double l = (double)__builtin_amdgcn_frexp_exp(x) + y + r * __builtin_fma(r, -0.5, 1.0) * kLog2ed;
+  return x == 0.0 ? -__builtin_inf() : l;
+}
+
+}  // namespace fm

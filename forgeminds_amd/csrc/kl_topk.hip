@@ -15,7 +15,7 @@
 // columns and the loss are computed in 64 bits by the threads that hold the list (the loss is a small
 // difference of terms ten to a hundred times its size), the sweep over the row in fp32.
 #include "../../include/fm_hip_tokens.h"
-#include "fm_vocab.hip.h"
+#include "fm_f64.hip.h"
 
 using namespace fm;
 
@@ -25,7 +25,6 @@ constexpr int kMaxList = 1024;
 constexpr int kSmallList = 128;
 constexpr uint16_t kEnd = 0xFFFFu;
 constexpr int kNoLead = 0x7fffffff;
-constexpr double kLn2d = 0.69314718055994530942;
 
 struct ListArgs {
   const void* idx;
@@ -43,36 +42,69 @@ struct ListArgs {
 __device__ __forceinline__ int64_t list_idx(const ListArgs& a, int64_t at) {
   return a.idx64 ? static_cast<const int64_t*>(a.idx)[at] : (int64_t)static_cast<const int32_t*>(a.idx)[at];
 }
-__device__ __forceinline__ double list_value(const ListArgs& a, int64_t at) {
-  if (a.teacher_dtype == FM_F32) return (double)static_cast<const float*>(a.teacher)[at];
-  if (a.teacher_dtype == FM_BF16) return (double)Elem<bf16_t>::load1(static_cast<const bf16_t*>(a.teacher) + at);
-  return (double)Elem<f16_t>::load1(static_cast<const f16_t*>(a.teacher) + at);
+// A slot's column and teacher value as loaded. The loads name no branch, whatever the two types, and
+// nothing is converted yet: the wait for them comes where they are used, behind the row's own loads.
+struct SlotBits {
+  uint32_t lo, hi;
+  uint16_t t0, t1;
+};
+__device__ __forceinline__ SlotBits slot_load(const ListArgs& a, int64_t at) {
+  SlotBits b;
+  const char* i = static_cast<const char*>(a.idx) + at * (a.idx64 ? 8 : 4);
+  b.lo = *reinterpret_cast<const uint32_t*>(i);
+  b.hi = *reinterpret_cast<const uint32_t*>(i + (a.idx64 ? 4 : 0));
+  const char* t = static_cast<const char*>(a.teacher) + at * (a.teacher_dtype == FM_F32 ? 4 : 2);
+  b.t0 = *reinterpret_cast<const uint16_t*>(t);
+  b.t1 = *reinterpret_cast<const uint16_t*>(t + (a.teacher_dtype == FM_F32 ? 2 : 0));
+  return b;
+}
+__device__ __forceinline__ int64_t slot_col(const ListArgs& a, const SlotBits& b) {
+  const uint32_t hi = a.idx64 ? b.hi : (uint32_t)((int32_t)b.lo >> 31);
+  return (int64_t)(((uint64_t)hi << 32) | b.lo);
+}
+__device__ __forceinline__ float slot_value(const ListArgs& a, const SlotBits& b) {
+  const uint32_t word = ((uint32_t)b.t1 << 16) | (a.teacher_dtype == FM_F32 ? b.t0 : 0);
+  const float half = (float)__builtin_bit_cast(_Float16, b.t0);
+  return a.teacher_dtype == FM_F16 ? half : u2f(word);
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+// element d of a packed vector: its value, and the vector with the element's bits replaced
+template <typename T>
+__device__ __forceinline__ uint32_t word_at(const u32x4& r, int w) {
+  const uint32_t a = w & 1 ? r.y : r.x, b = w & 1 ? r.w : r.z;
+  return w & 2 ? b : a;
 }
-__device__ __forceinline__ double wave_max64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const double w = __shfl_xor(v, o, 64);
-    v = w > v ? w : v;
+template <typename T>
+__device__ __forceinline__ float get_elem(const u32x4& r, int d) {
+  if constexpr (sizeof(T) == 4) {
+    return u2f(word_at<T>(r, d));
+  } else {
+    const uint32_t w = word_at<T>(r, d >> 1);
+    T t;
+    t.bits = (uint16_t)(d & 1 ? w >> 16 : w);
+    return Elem<T>::load1(&t);
   }
-  return v;
 }
-template <int NW, bool MAX>
-__device__ __forceinline__ double block_reduce64(double v, double* smem) {
-  v = MAX ? wave_max64(v) : wave_sum64(v);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (lane == 0) smem[wave] = v;
-  __syncthreads();
-  double r = smem[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) r = MAX ? (smem[i] > r ? smem[i] : r) : r + smem[i];
-  __syncthreads();
-  return r;
+template <typename T>
+__device__ __forceinline__ void set_elem(u32x4& r, int d, uint32_t bits) {
+  uint32_t w = bits;
+  int at = d;
+  if constexpr (sizeof(T) == 2) {
+    at = d >> 1;
+    const uint32_t old = word_at<T>(r, at);
+    w = d & 1 ? (old & 0xffffu) | (bits << 16) : (old & 0xffff0000u) | bits;
+  }
+  r.x = at == 0 ? w : r.x;
+  r.y = at == 1 ? w : r.y;
+  r.z = at == 2 ? w : r.z;
+  r.w = at == 3 ? w : r.w;
+}
+// the bits of a value as stored in T (for the half types in the low 16)
+template <typename T>
+__device__ __forceinline__ uint32_t bits_of(float f) {
+  if constexpr (std::is_same<T, float>::value) return f2u(f);
+  else if constexpr (std::is_same<T, bf16_t>::value) return pack_bf16(f, 0.f) & 0xffffu;
+  else return pack_f16(f, 0.f) & 0xffffu;
 }
 
 // Workgroup merge of per-thread running (maximum, sum): the maximum in fp32, the sums in 64 bits.
@@ -82,8 +114,8 @@ struct Pair64 {
 };
 template <int NW>
 __device__ __forceinline__ Pair64 block_merge64(MaxSum v, double* smem, float* smemf) {
-  const float m = block_max<NW>(v.m, smemf);
-  return Pair64{m, block_reduce64<NW, false>((double)v.s * (double)fast_exp2(v.m - m), smem)};
+  const float m = block_max32<NW>(v.m, smemf);
+  return Pair64{m, block_reduce64<NW, Sum64>((double)v.s * (double)fast_exp2(v.m - m), smem)};
 }
 
 // The list of one row in LDS. Distinct columns are found with an open-addressing table (a column's
@@ -99,7 +131,8 @@ struct ListShared {
   int hcol[kSlots];
   int hlead[kSlots];
   int col[KCAP];
-  float g[KCAP];
+  float x[KCAP];
+  uint32_t g[KCAP];
   uint32_t mask[THREADS];
   uint16_t nxt[KCAP];
   uint16_t head[THREADS];
@@ -110,7 +143,6 @@ struct ListShared {
 template <int SL>
 struct Mine {
   int col[SL];       // -1: not the leader of a column
-  float x[SL];       // the student's logit there
   double q[SL];
 };
 
@@ -121,25 +153,20 @@ __device__ __forceinline__ uint32_t hash_col(int col) {
   return ((uint32_t)col * 2654435761u) >> (32 - __builtin_ctz(SLOTS));
 }
 
-template <typename T, int THREADS, int KCAP, int SL>
-__device__ __forceinline__ void list_load(const ListArgs& a, int64_t row, int64_t (&c)[SL], double (&t)[SL]) {
+template <int THREADS, int SL>
+__device__ __forceinline__ void list_load(const ListArgs& a, int64_t row, SlotBits (&bits)[SL]) {
 #pragma unroll
   for (int j = 0; j < SL; ++j) {
     const int s = j * THREADS + (int)threadIdx.x;
-    c[j] = -1;
-    t[j] = 0.0;
-    if (s < a.k) {
-      c[j] = list_idx(a, row * a.k + s);
-      t[j] = list_value(a, row * a.k + s);
-    }
+    bits[j] = slot_load(a, row * a.k + (s < a.k ? s : 0));
   }
 }
 
 // Fills the LDS table and chains and returns the sum of q (NaN when a column is out of range);
 // *unique gets the number of distinct columns. All threads of the workgroup call it.
 template <typename T, int THREADS, int KCAP, int SL>
-__device__ __forceinline__ double list_build(const ListArgs& a, const T* rp, const RowSplit& sp, int64_t row, int v,
-                                             const int64_t (&c)[SL], const double (&t)[SL],
+__device__ __forceinline__ double list_build(const ListArgs& a, const RowSplit& sp, int64_t row, int v,
+                                             const SlotBits (&bits)[SL], float lse_t,
                                              ListShared<THREADS, KCAP>& sh, Mine<SL>& mine, int* unique) {
   constexpr int NW = THREADS / 64;
   constexpr int EPV = Elem<T>::kVec;
@@ -149,37 +176,38 @@ __device__ __forceinline__ double list_build(const ListArgs& a, const T* rp, con
   sh.mask[tid] = 0u;
   sh.head[tid] = kEnd;
   bool bad = false;
+  float t[SL];
+  bool used[SL];
 #pragma unroll
   for (int j = 0; j < SL; ++j) {
-    mine.col[j] = -1;
-    mine.x[j] = 0.f;
+    const int64_t c = j * THREADS + tid < a.k ? slot_col(a, bits[j]) : -1;
+    t[j] = slot_value(a, bits[j]);
+    used[j] = c >= 0;
+    bad |= c >= v;
+    mine.col[j] = c >= v ? -1 : (int)c;
+    if (c < 0) mine.col[j] = -1;
     mine.q[j] = 0.0;
-    if (c[j] >= v) bad = true;
-    else if (c[j] >= 0) {
-      mine.col[j] = (int)c[j];
-      mine.x[j] = Elem<T>::load1(rp + c[j]);
-    }
   }
   // teacher probabilities of the used slots
   if (a.probs == FM_TEACHER_PROBS) {
 #pragma unroll
-    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mine.q[j] = t[j];
+    for (int j = 0; j < SL; ++j) if (used[j]) mine.q[j] = (double)t[j];
   } else if (a.tail == FM_TAIL_RENORM) {
     double mx = -__builtin_inf();
 #pragma unroll
-    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mx = t[j] > mx ? t[j] : mx;
-    mx = block_reduce64<NW, true>(mx, sh.red);
+    for (int j = 0; j < SL; ++j) if (used[j]) mx = (double)t[j] > mx ? (double)t[j] : mx;
+    mx = block_reduce64<NW, Max64>(mx, sh.red);
 #pragma unroll
-    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mine.q[j] = exp((t[j] - mx) * a.inv_t);
+    for (int j = 0; j < SL; ++j) if (used[j]) mine.q[j] = exp2_64(((double)t[j] - mx) * (a.inv_t * kLog2ed));
   } else {
-    const double l = (double)a.teacher_lse[row];
+    const double l = (double)lse_t;
 #pragma unroll
-    for (int j = 0; j < SL; ++j) if (c[j] >= 0) mine.q[j] = exp(t[j] * a.inv_t - l);
+    for (int j = 0; j < SL; ++j) if (used[j]) mine.q[j] = exp2_64(((double)t[j] * a.inv_t - l) * kLog2ed);
   }
   double sum = bad ? __builtin_nan("") : 0.0;
 #pragma unroll
   for (int j = 0; j < SL; ++j) sum += mine.q[j];
-  sum = block_reduce64<NW, false>(sum, sh.red);      // its barriers also publish the cleared table
+  sum = block_reduce64<NW, Sum64>(sum, sh.red);      // its barriers also publish the cleared table
   if (a.tail == FM_TAIL_RENORM) {
     const double r = 1.0 / sum;
 #pragma unroll
@@ -265,31 +293,31 @@ __device__ __forceinline__ double list_build(const ListArgs& a, const T* rp, con
   __syncthreads();
   if (a.tail == FM_TAIL_BUCKET) {
     int u = 0;
-#pragma unroll
     for (int i = 0; i < NW; ++i) u += sh.redi[i];
     *unique = u;
   }
   return sum;
 }
 
-// value of the chain's entry for each element of the vector at col0: fn(element, slot)
+// the chain's entries in the EPV columns from col0: fn(element, slot)
 template <int EPV, int THREADS, int KCAP, typename F>
 __device__ __forceinline__ void walk(const ListShared<THREADS, KCAP>& sh, uint16_t head, int col0, F fn) {
+#pragma unroll 1
   for (uint32_t s = head; s != kEnd; s = sh.nxt[s]) {
     const int d = sh.col[s] - col0;
-    if (d >= 0 && d < EPV) fn(d, (int)s);
+    if ((unsigned)d < (unsigned)EPV) fn(d, (int)s);
   }
 }
 
 // Gradient coefficients of a row and its loss (LOSS), from the merged pairs; the listed columns'
 // gradients go to sh.g. Returns the coefficient of an unlisted column: its gradient is
 // coef * exp2(x * c - rest.m).
-template <int THREADS, int KCAP, int SL, bool LOSS, bool GRAD>
+template <typename T, int THREADS, int KCAP, int SL, bool LOSS, bool GRAD>
 __device__ __forceinline__ float finish_row(const ListArgs& a, ListShared<THREADS, KCAP>& sh, const Mine<SL>& mine,
                                             const Pair64& all, const Pair64& rest, double sum_q, int unique, int v,
                                             double scale, float* loss_at) {
   constexpr int NW = THREADS / 64;
-  const double lse2 = (double)all.m + log2(all.s);
+  const double lse2 = (double)all.m + log2_64(all.s);
   double q_r = 0.0;
   if (a.tail == FM_TAIL_BUCKET && unique < v) {
     q_r = 1.0 - sum_q;
@@ -301,35 +329,38 @@ __device__ __forceinline__ float finish_row(const ListArgs& a, ListShared<THREAD
   for (int j = 0; j < SL; ++j) {
     if (mine.col[j] < 0) continue;
     const int s = j * THREADS + (int)threadIdx.x;
-    const double lp2 = (double)mine.x[j] * (double)a.c - lse2;
-    if (LOSS && !(mine.q[j] == 0.0)) term += mine.q[j] * (log(mine.q[j]) - lp2 * kLn2d);
-    if (GRAD) sh.g[s] = (float)((exp2(lp2) * total - mine.q[j]) * scale);
+    const double lp2 = (double)sh.x[s] * (double)a.c - lse2;
+    if (LOSS && !(mine.q[j] == 0.0)) term += mine.q[j] * (log2_64(mine.q[j]) - lp2);
+    if (GRAD) sh.g[s] = bits_of<T>((float)((exp2_64(lp2) * total - mine.q[j]) * scale));
   }
   if (LOSS) {
-    term = block_reduce64<NW, false>(term, sh.red);
+    term = block_reduce64<NW, Sum64>(term, sh.red);
     if (threadIdx.x == 0) {
-      if (!(q_r == 0.0)) term += q_r * (log(q_r) - ((double)rest.m + log2(rest.s) - lse2) * kLn2d);
+      term *= kLn2d;
+      if (!(q_r == 0.0)) term += q_r * (log2_64(q_r) - ((double)rest.m + log2_64(rest.s) - lse2)) * kLn2d;
       if (sum_q != sum_q) term = sum_q;
       *loss_at = (float)term;
     }
   }
   if (!GRAD) return 0.f;
   __syncthreads();                     // sh.g
-  double coef = total * exp2((double)rest.m - (double)all.m) / all.s;
+  double coef = total * exp2_64((double)rest.m - (double)all.m) / all.s;
   if (!(q_r == 0.0)) coef -= q_r / rest.s;
   // no unlisted column with any probability: their logits are -inf and their gradient 0
   if (rest.s == 0.0 && q_r == 0.0) coef = 0.0;
   return (float)(coef * scale);
 }
 
-// running (maximum, sum) of one vector; `skip` removes listed columns first
+// one vector into the running (maximum, sum); a NaN reaches both
 template <typename T>
-__device__ __forceinline__ void fold(MaxSum& run, float (&x)[Elem<T>::kVec], float c) {
+__device__ __forceinline__ void fold(MaxSum& run, const u32x4& r, float c) {
   constexpr int EPV = Elem<T>::kVec;
+  float x[EPV];
+  Elem<T>::unpack(r, x);
   float mx = x[0];
 #pragma unroll
-  for (int e = 1; e < EPV; ++e) mx = fmaxf(mx, x[e]);
-  const float cm = fmaxf(run.m, mx * c);
+  for (int e = 1; e < EPV; ++e) mx = __builtin_elementwise_maximum(mx, x[e]);
+  const float cm = __builtin_elementwise_maximum(run.m, mx * c);
   float acc = run.s * fast_exp2(run.m - cm);
 #pragma unroll
   for (int e = 0; e < EPV; ++e) acc += fast_exp2(__builtin_fmaf(x[e], c, -cm));
@@ -352,13 +383,37 @@ __device__ __forceinline__ float count_rows(const ListArgs& a, int64_t n, int* r
   return t > 0 ? (float)t : 1.f;
 }
 
+template <typename T>
+__device__ __forceinline__ void store_bits(T* p, uint32_t bits) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(p) = bits;
+  else *reinterpret_cast<uint16_t*>(p) = (uint16_t)bits;
+}
+
+// the gradient of vector c (its first column col0), packed
+template <typename T, int THREADS, int KCAP>
+__device__ __forceinline__ u32x4 grad_of(const u32x4& r, float scale, float m, float coef,
+                                         const ListShared<THREADS, KCAP>& sh, uint32_t mask, uint16_t head, int c,
+                                         int col0) {
+  constexpr int EPV = Elem<T>::kVec;
+  float x[EPV];
+  Elem<T>::unpack(r, x);
+#pragma unroll
+  for (int e = 0; e < EPV; ++e) x[e] = coef * fast_exp2(__builtin_fmaf(x[e], scale, -m));
+  u32x4 o = Elem<T>::pack(x);
+  if ((mask >> ((c / THREADS) % 31)) & 1u)
+    walk<EPV, THREADS, KCAP>(sh, head, col0, [&](int d, int s) { set_elem<T>(o, d, sh.g[s]); });
+  return o;
+}
+
 // GRAD: loss and gradient, RI vectors a thread held in registers between the fold and the store,
 // what a row has beyond them read twice. !GRAD: loss and stats from one streaming read (RI vectors
-// a thread in flight).
-template <typename T, int THREADS, int KCAP, int RI, bool GRAD>
+// a thread in flight). VEC: the buffers are 16-byte aligned and every row holds a whole vector, so the
+// row's loads stand behind no branch -- behind one, the first wait of the list's loads would be a wait
+// for all of them ([4096,128256] bf16, loss and gradient: 552 us). !VEC: one element at a time.
+template <typename T, int THREADS, int KCAP, int RI, bool GRAD, bool VEC>
 __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, ListArgs a, float* __restrict__ row_loss,
                                                           float* __restrict__ stats, const float* __restrict__ n_valid,
-                                                          int count_n, T* dstudent, int v, bool vec_ok) {
+                                                          int count_n, T* dstudent, int v) {
   constexpr int EPV = Elem<T>::kVec;
   constexpr int NW = THREADS / 64;
   constexpr int SL = (KCAP + THREADS - 1) / THREADS;
@@ -366,7 +421,7 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   const int64_t row = blockIdx.x;
   const T* rp = student + row * (int64_t)v;
   T* gp = GRAD ? dstudent + row * (int64_t)v : nullptr;
-  const RowSplit sp = split_row<EPV>(row, v, vec_ok);
+  const RowSplit sp = split_row<EPV>(row, v, VEC);
   const int tid = threadIdx.x;
   const int ne = edge_count(sp, v);
   const bool bucket = a.tail == FM_TAIL_BUCKET;
@@ -382,60 +437,62 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     return;
   }
   // the list's loads go first: waiting for them then waits for nothing of the row
-  int64_t lc[SL];
-  double lt[SL];
-  list_load<T, THREADS, KCAP, SL>(a, row, lc, lt);
+  SlotBits bits[SL];
+  list_load<THREADS, SL>(a, row, bits);
+  const float lse_t = *(a.teacher_lse != nullptr ? a.teacher_lse + row : static_cast<const float*>(a.idx));
+  const T* vp = rp + sp.head;              // 16-byte aligned where there are vectors
+  auto at = [&](int c) { return reinterpret_cast<const T*>(reinterpret_cast<const char*>(vp) + (uint32_t)c * 16u); };
   u32x4 raw[RI];
-  const int last = sp.nvec - 1;
-  if (sp.nvec > 0) {
+  if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < RI; ++i) {
-      const int c = i * THREADS + tid;
-      raw[i] = load16_stream(rp + sp.head + (int64_t)(c < sp.nvec ? c : last) * EPV);
-    }
+    for (int i = 0; i < RI; ++i) raw[i] = load16_stream(at(clamp_col(i * THREADS + tid, sp.nvec)));
   }
   Mine<SL> mine;
   int unique;
-  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, rp, sp, row, v, lc, lt, sh, mine, &unique);
+  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, sp, row, v, bits, lse_t, sh, mine, &unique);
   const uint32_t mask = sh.mask[tid];
   const uint16_t head = sh.head[tid];
 
+  // The sweep leaves the listed logits in sh.x and, for the bucket, folds the other columns only.
   MaxSum run{kNegBig, 0.f};
-  auto take = [&](u32x4& r, int c, int it) {
+  auto take = [&](u32x4 r, int c) {
     if (c >= sp.nvec) return;
-    float x[EPV];
-    Elem<T>::unpack(r, x);
-    if (bucket && ((mask >> (it % 31)) & 1u)) {
-      walk<EPV, THREADS, KCAP>(sh, head, sp.head + c * EPV, [&](int d, int) {
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) if (e == d) x[e] = -INFINITY;
+    if ((mask >> ((c / THREADS) % 31)) & 1u) {
+      walk<EPV, THREADS, KCAP>(sh, head, sp.head + c * EPV, [&](int d, int s) {
+        sh.x[s] = get_elem<T>(r, d);
+        if (bucket) set_elem<T>(r, d, bits_of<T>(-INFINITY));
       });
     }
-    fold<T>(run, x, a.c);
+    fold<T>(run, r, a.c);
   };
-  if (sp.nvec > 0) {
+  if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < RI; ++i) take(raw[i], i * THREADS + tid, i);
+    for (int i = 0; i < RI; ++i) take(raw[i], i * THREADS + tid);
     constexpr int UN = GRAD ? 2 : RI;
     for (int c0 = RI * THREADS; c0 < sp.nvec; c0 += UN * THREADS) {
       u32x4 more[UN];
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
-        const T* at = rp + sp.head + (int64_t)clamp_col(c0 + u * THREADS + tid, sp.nvec) * EPV;
-        more[u] = GRAD ? load16(at) : load16_stream(at);
+        const T* from = at(clamp_col(c0 + u * THREADS + tid, sp.nvec));
+        more[u] = GRAD ? load16(from) : load16_stream(from);
       }
 #pragma unroll
       for (int u = 0; u < UN; ++u) {
         touch_whole(more[u]);
-        take(more[u], c0 + u * THREADS + tid, c0 / THREADS + u);
+        take(more[u], c0 + u * THREADS + tid);
       }
     }
   }
   for (int e = tid; e < ne; e += THREADS) {
     const int col = edge_col(sp, e);
     float x = Elem<T>::load1(rp + col);
-    if (bucket && (mask >> 31)) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int) { x = -INFINITY; });
-    const float cm = fmaxf(run.m, x * a.c);
+    if (mask >> 31) {
+      walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) {
+        sh.x[s] = x;
+        if (bucket) x = -INFINITY;
+      });
+    }
+    const float cm = __builtin_elementwise_maximum(run.m, x * a.c);
     run.s = run.s * fast_exp2(run.m - cm) + fast_exp2(__builtin_fmaf(x, a.c, -cm));
     run.m = cm;
   }
@@ -444,19 +501,21 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   if (bucket) {      // the listed columns join the unlisted ones
     MaxSum w{rest.m, 0.f};
 #pragma unroll
-    for (int j = 0; j < SL; ++j) if (mine.col[j] >= 0) w.m = fmaxf(w.m, mine.x[j] * a.c);
-    all.m = block_max<NW>(w.m, sh.redf);
-    double s = tid == 0 ? rest.s * exp2((double)rest.m - (double)all.m) : 0.0;
+    for (int j = 0; j < SL; ++j)
+      if (mine.col[j] >= 0) w.m = __builtin_elementwise_maximum(w.m, sh.x[j * THREADS + tid] * a.c);
+    all.m = block_max32<NW>(w.m, sh.redf);
+    double s = tid == 0 ? rest.s * exp2_64((double)rest.m - (double)all.m) : 0.0;
 #pragma unroll
-    for (int j = 0; j < SL; ++j) if (mine.col[j] >= 0) s += exp2((double)mine.x[j] * (double)a.c - (double)all.m);
-    all.s = block_reduce64<NW, false>(s, sh.red);
+    for (int j = 0; j < SL; ++j)
+      if (mine.col[j] >= 0) s += exp2_64((double)sh.x[j * THREADS + tid] * (double)a.c - (double)all.m);
+    all.s = block_reduce64<NW, Sum64>(s, sh.red);
   }
   double scale = a.inv_t;
   if (GRAD) {
     if (count_n > 0) scale /= (double)count_rows<THREADS>(a, count_n, sh.redi);
     else if (n_valid != nullptr) scale /= (double)*n_valid;
   }
-  const float coef = finish_row<THREADS, KCAP, SL, true, GRAD>(a, sh, mine, all, rest, sum_q, unique, v, scale,
+  const float coef = finish_row<T, THREADS, KCAP, SL, true, GRAD>(a, sh, mine, all, rest, sum_q, unique, v, scale,
                                                                row_loss + row);
   if (tid == 0 && stats != nullptr) {
     stats[row * 4] = all.m;
@@ -465,45 +524,35 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     stats[row * 4 + 3] = (float)rest.s;
   }
   if constexpr (GRAD) {
-    auto put = [&](u32x4& r, int c, int it) {
+    T* vg = gp + sp.head;
+    auto put = [&](const u32x4& r, int c) {
       if (c >= sp.nvec) return;
-      float x[EPV], o[EPV];
-      Elem<T>::unpack(r, x);
-      const int col0 = sp.head + c * EPV;
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) o[e] = coef * fast_exp2(__builtin_fmaf(x[e], a.c, -rest.m));
-      if ((mask >> (it % 31)) & 1u) {
-        walk<EPV, THREADS, KCAP>(sh, head, col0, [&](int d, int s) {
-          const float g = sh.g[s];
-#pragma unroll
-          for (int e = 0; e < EPV; ++e) if (e == d) o[e] = g;
-        });
-      }
-      store16_stream(gp + col0, Elem<T>::pack(o));
+      store16_stream(reinterpret_cast<T*>(reinterpret_cast<char*>(vg) + (uint32_t)c * 16u),
+                     grad_of<T, THREADS, KCAP>(r, a.c, rest.m, coef, sh, mask, head, c, sp.head + c * EPV));
     };
-    if (sp.nvec > 0) {
+    if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < RI; ++i) {
         touch_whole(raw[i]);
-        put(raw[i], i * THREADS + tid, i);
+        put(raw[i], i * THREADS + tid);
       }
       for (int c0 = RI * THREADS; c0 < sp.nvec; c0 += 2 * THREADS) {
         u32x4 more[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          more[u] = load16_stream(rp + sp.head + (int64_t)clamp_col(c0 + u * THREADS + tid, sp.nvec) * EPV);
+        for (int u = 0; u < 2; ++u) more[u] = load16_stream(at(clamp_col(c0 + u * THREADS + tid, sp.nvec)));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           touch_whole(more[u]);
-          put(more[u], c0 + u * THREADS + tid, c0 / THREADS + u);
+          put(more[u], c0 + u * THREADS + tid);
         }
       }
     }
     for (int e = tid; e < ne; e += THREADS) {
       const int col = edge_col(sp, e);
       float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), a.c, -rest.m));
-      if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { o = sh.g[s]; });
-      Elem<T>::store1(gp + col, o);
+      uint32_t one = bits_of<T>(o);
+      if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { one = sh.g[s]; });
+      store_bits(gp + col, one);
     }
   }
 }
@@ -536,19 +585,22 @@ __global__ __launch_bounds__(THREADS) void kl_topk_bwd_kernel(const T* student, 
     for (int e = tid; e < ne; e += THREADS) Elem<T>::store1(gp + edge_col(sp, e), 0.f);
     return;
   }
-  int64_t lc[SL];
-  double lt[SL];
-  list_load<T, THREADS, KCAP, SL>(a, row, lc, lt);
+  SlotBits bits[SL];
+  list_load<THREADS, SL>(a, row, bits);
+  const float lse_t = *(a.teacher_lse != nullptr ? a.teacher_lse + row : static_cast<const float*>(a.idx));
   const Pair64 all{stats[row * 4], (double)stats[row * 4 + 1]}, rest{stats[row * 4 + 2], (double)stats[row * 4 + 3]};
   double scale = a.inv_t;
   if (grad_out != nullptr) scale *= (double)grad_out[grad_per_row ? row : 0];
   if (n_valid != nullptr) scale /= (double)*n_valid;
   Mine<SL> mine;
   int unique;
-  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, rp, sp, row, v, lc, lt, sh, mine, &unique);
+  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, sp, row, v, bits, lse_t, sh, mine, &unique);
+#pragma unroll
+  for (int j = 0; j < SL; ++j)
+    if (mine.col[j] >= 0) sh.x[j * THREADS + tid] = Elem<T>::load1(rp + mine.col[j]);
   const uint32_t mask = sh.mask[tid];
   const uint16_t head = sh.head[tid];
-  const float coef = finish_row<THREADS, KCAP, SL, false, true>(a, sh, mine, all, rest, sum_q, unique, v, scale, nullptr);
+  const float coef = finish_row<T, THREADS, KCAP, SL, false, true>(a, sh, mine, all, rest, sum_q, unique, v, scale, nullptr);
   for (int c0 = c_begin; c0 < c_end; c0 += THREADS * UN) {
     u32x4 raw[UN];
 #pragma unroll
@@ -558,54 +610,65 @@ __global__ __launch_bounds__(THREADS) void kl_topk_bwd_kernel(const T* student, 
     for (int u = 0; u < UN; ++u) {
       const int c = c0 + u * THREADS + tid;
       touch_whole(raw[u]);
-      if (c < c_end) {
-        float x[EPV], o[EPV];
-        Elem<T>::unpack(raw[u], x);
-        const int col0 = sp.head + c * EPV;
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) o[e] = coef * fast_exp2(__builtin_fmaf(x[e], a.c, -rest.m));
-        if ((mask >> ((c / THREADS) % 31)) & 1u) {
-          walk<EPV, THREADS, KCAP>(sh, head, col0, [&](int d, int s) {
-            const float g = sh.g[s];
-#pragma unroll
-            for (int e = 0; e < EPV; ++e) if (e == d) o[e] = g;
-          });
-        }
-        store16_stream(gp + col0, Elem<T>::pack(o));
-      }
+      if (c < c_end)
+        store16_stream(gp + sp.head + (int64_t)c * EPV,
+                       grad_of<T, THREADS, KCAP>(raw[u], a.c, rest.m, coef, sh, mask, head, c, sp.head + c * EPV));
     }
   }
   for (int e = tid; e < ne; e += THREADS) {
     const int col = edge_col(sp, e);
     float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), a.c, -rest.m));
-    if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { o = sh.g[s]; });
-    Elem<T>::store1(gp + col, o);
+    uint32_t one = bits_of<T>(o);
+    if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { one = sh.g[s]; });
+    store_bits(gp + col, one);
   }
 }
 
-// n_valid and (row_loss != nullptr) the reduced loss, one workgroup, fixed order, 64-bit sum
-__global__ __launch_bounds__(1024) void kl_topk_finalize_kernel(const float* __restrict__ row_loss, ListArgs a, int64_t n,
-                                                                int mean, float* __restrict__ loss,
-                                                                float* __restrict__ n_valid) {
+// *n_valid = rows with a list (COUNT); *loss = sum of row_loss [/ n_valid] (LOSS). One workgroup, eight
+// rows' loads of a thread in flight, 64-bit sum in a fixed order.
+template <bool COUNT, bool LOSS>
+__global__ __launch_bounds__(1024) void kl_topk_reduce_kernel(const float* __restrict__ row_loss, ListArgs a, int64_t n,
+                                                              int mean, float* __restrict__ loss,
+                                                              float* __restrict__ n_valid) {
   __shared__ double sd[16];
   __shared__ int si[16];
   double s = 0.0;
   int cnt = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    if (row_loss != nullptr) s += (double)row_loss[i];
-    cnt += list_idx(a, i * a.k) >= 0 ? 1 : 0;
+  for (int64_t i = threadIdx.x; i < n; i += 8 * 1024) {
+    float r[8];
+    int used[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t at = i + u * 1024 < n ? i + u * 1024 : i;
+      if (LOSS) r[u] = row_loss[at];
+      // the sign of slot 0
+      if (COUNT) used[u] = static_cast<const int32_t*>(a.idx)[at * a.k * (a.idx64 ? 2 : 1) + (a.idx64 ? 1 : 0)];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (i + u * 1024 < n) {
+        if (LOSS) s += (double)r[u];
+        if (COUNT) cnt += used[u] >= 0 ? 1 : 0;
+      }
+    }
   }
-  s = wave_sum64(s);
-  cnt = wave_sum_i(cnt);
-  if ((threadIdx.x & 63) == 0) { sd[threadIdx.x >> 6] = s; si[threadIdx.x >> 6] = cnt; }
-  __syncthreads();
+  if (LOSS) s = block_reduce64<16, Sum64>(s, sd);
+  if (COUNT) {
+    cnt = wave_sum_i(cnt);
+    if ((threadIdx.x & 63) == 0) si[threadIdx.x >> 6] = cnt;
+    __syncthreads();
+  }
   if (threadIdx.x == 0) {
-    double t = sd[0];
-    int c = si[0];
-    for (int i = 1; i < 16; ++i) { t += sd[i]; c += si[i]; }
-    const int nv = c > 0 ? c : 1;
-    *n_valid = (float)nv;
-    if (row_loss != nullptr) *loss = (float)(mean ? t / nv : t);
+    float nv = 1.f;
+    if (COUNT) {
+      int c = 0;
+      for (int i = 0; i < 16; ++i) c += si[i];
+      nv = c > 0 ? (float)c : 1.f;
+      *n_valid = nv;
+    } else if (mean) {
+      nv = *n_valid;
+    }
+    if (LOSS) *loss = (float)(mean ? s / (double)nv : s);
   }
 }
 
@@ -643,15 +706,15 @@ template <typename T, int KCAP>
 void launch_loss_grad(const void* student, const ListArgs& a, float* row_loss, float* stats, const float* n_valid,
                       int count_n, void* dstudent, int64_t n, int v, bool vec_ok, hipStream_t st) {
   const int64_t nvec = v / Elem<T>::kVec;
-#define GO(TH, RI)                                                                                           \
-  FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, true>), dim3((unsigned)n), dim3(TH), 0, st,                     \
-            static_cast<const T*>(student), a, row_loss, stats, n_valid, count_n, static_cast<T*>(dstudent), \
-            v, vec_ok)
-  if (nvec <= 256 * 2) GO(256, 2);
-  else if (nvec <= 256 * 8) GO(256, 8);
-  else if (nvec <= 512 * 8) GO(512, 8);
-  else if (nvec <= 1024 * 8) GO(1024, 8);
-  else GO(1024, 16);
+#define GO(TH, RI, VEC)                                                                                      \
+  FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, true, VEC>), dim3((unsigned)n), dim3(TH), 0, st,                \
+            static_cast<const T*>(student), a, row_loss, stats, n_valid, count_n, static_cast<T*>(dstudent), v)
+  if (!vec_ok || v < 2 * Elem<T>::kVec) GO(256, 2, false);
+  else if (nvec <= 256 * 2) GO(256, 2, true);
+  else if (nvec <= 256 * 8) GO(256, 8, true);
+  else if (nvec <= 512 * 8) GO(512, 8, true);
+  else if (nvec <= 1024 * 8) GO(1024, 8, true);
+  else GO(1024, 16, true);
 #undef GO
 }
 
@@ -659,11 +722,12 @@ template <typename T, int KCAP>
 void launch_fwd(const void* student, const ListArgs& a, float* row_loss, float* stats, int64_t n, int v, bool vec_ok,
                 hipStream_t st) {
   const int64_t nvec = v / Elem<T>::kVec;
-#define GO(TH, RI)                                                                                           \
-  FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, false>), dim3((unsigned)n), dim3(TH), 0, st,                    \
-            static_cast<const T*>(student), a, row_loss, stats, nullptr, 0, static_cast<T*>(nullptr), v, vec_ok)
-  if (nvec <= 256 * 8) GO(256, 4);
-  else GO(512, 4);
+#define GO(TH, RI, VEC)                                                                                      \
+  FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, false, VEC>), dim3((unsigned)n), dim3(TH), 0, st,               \
+            static_cast<const T*>(student), a, row_loss, stats, nullptr, 0, static_cast<T*>(nullptr), v)
+  if (!vec_ok || v < 2 * Elem<T>::kVec) GO(256, 4, false);
+  else if (nvec <= 256 * 8) GO(256, 4, true);
+  else GO(512, 4, true);
 #undef GO
 }
 
@@ -716,7 +780,7 @@ int fm_kl_topk_fwd(const void* student, const void* idx, const void* teacher, co
     FM_CHECK_LAUNCH("fm_kl_topk_fwd");
   }
   if (reduction != FM_REDUCE_NONE) {
-    hipLaunchKernelGGL(kl_topk_finalize_kernel, dim3(1), dim3(1024), 0, st, row_loss, a, n,
+    hipLaunchKernelGGL((kl_topk_reduce_kernel<true, true>), dim3(1), dim3(1024), 0, st, row_loss, a, n,
                        reduction == FM_REDUCE_MEAN ? 1 : 0, loss, n_valid);
     FM_CHECK_LAUNCH("fm_kl_topk_fwd(finalize)");
   }
@@ -741,7 +805,8 @@ int fm_kl_topk_loss_grad(const void* student, const void* idx, const void* teach
   if (n > 0) {
     const bool count_here = mean && n <= kCountInKernel;
     if (mean && !count_here) {
-      hipLaunchKernelGGL(kl_topk_finalize_kernel, dim3(1), dim3(1024), 0, st, nullptr, a, n, 0, loss, n_valid);
+      hipLaunchKernelGGL((kl_topk_reduce_kernel<true, false>), dim3(1), dim3(1024), 0, st, nullptr, a, n, 0, loss,
+                         n_valid);
       FM_CHECK_LAUNCH("fm_kl_topk_loss_grad(count)");
     }
     const bool vec_ok = fm_host::aligned16(student) && fm_host::aligned16(dstudent);
@@ -749,7 +814,11 @@ int fm_kl_topk_loss_grad(const void* student, const void* idx, const void* teach
                     count_here ? (int)n : 0, dstudent, n, (int)v, vec_ok, st);
     FM_CHECK_LAUNCH("fm_kl_topk_loss_grad");
   }
-  hipLaunchKernelGGL(kl_topk_finalize_kernel, dim3(1), dim3(1024), 0, st, row_loss, a, n, mean ? 1 : 0, loss, n_valid);
+  if (mean && n > kCountInKernel)      // n_valid is there
+    hipLaunchKernelGGL((kl_topk_reduce_kernel<false, true>), dim3(1), dim3(1024), 0, st, row_loss, a, n, 1, loss, n_valid);
+  else
+    hipLaunchKernelGGL((kl_topk_reduce_kernel<true, true>), dim3(1), dim3(1024), 0, st, row_loss, a, n, mean ? 1 : 0, loss,
+                       n_valid);
   FM_CHECK_LAUNCH("fm_kl_topk_loss_grad(finalize)");
   return FM_OK;
 }

@@ -20,6 +20,7 @@
 //      take a radix search over the bits of the value
 //   3  kept mass of each 64-vector segment in index order, the segment that holds u, the token in it
 #include "../../include/fm_hip_tokens.h"
+#include "fm_f64.hip.h"
 #include "fm_topk.hip.h"
 
 using namespace fm;
@@ -45,11 +46,6 @@ struct SampleArgs {
   int v;
 };
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
 __device__ __forceinline__ double wave_incl64(double v) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -121,40 +117,12 @@ struct SampleShared {
   double mass;
 };
 
-// exp((x - m) / T) = 2^((x - m) c). Degree-8 polynomial through the Chebyshev nodes of [-1/2, 1/2]
-// (relative error 1.1e-12) and an exact scaling: seventeen 64-bit operations, which run at the rate of
-// 32-bit ones here. The maximum's weight is exactly 1, so that rows of few distinct values split
-// evenly. The floor on the exponent turns -inf into a weight of zero.
+// exp((x - m) / T) = 2^((x - m) c), to 1.1e-12. The maximum's weight is exactly 1, so that rows of few
+// distinct values split evenly; that of -inf is zero.
 struct Weight {
   double m, c;
-  __device__ __forceinline__ double operator()(float x) const {
-    const double t = fmax(((double)x - m) * c, -1100.0);
-    const double n = __builtin_rint(t);
-    const double f = t - n;
-    double r = 1.3255224878668817e-06;
-    r = __builtin_fma(r, f, 1.5310079402249296e-05);
-    r = __builtin_fma(r, f, 0.00015403455852453838);
-    r = __builtin_fma(r, f, 0.0013333450568000645);
-    r = __builtin_fma(r, f, 0.009618129159402558);
-    r = __builtin_fma(r, f, 0.05550410941205933);
-    r = __builtin_fma(r, f, 0.2402265069581299);
-    r = __builtin_fma(r, f, 0.6931471805459335);
-    r = __builtin_fma(r, f, 1.0);
-    return __builtin_amdgcn_ldexp(r, (int)n);
-  }
+  __device__ __forceinline__ double operator()(float x) const { return exp2_64(((double)x - m) * c); }
 };
-
-template <int THREADS>
-__device__ __forceinline__ double block_sum64(double v, double* smem) {
-  v = wave_sum64(v);
-  if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double s = smem[0];
-#pragma unroll
-  for (int i = 1; i < THREADS / 64; ++i) s += smem[i];
-  __syncthreads();
-  return s;
-}
 
 // First of `n` non-negative entries (in LDS, in order) whose running sum reaches `target`
 // (strict: exceeds it); *before is the sum ahead of it. n when there is none. All threads call it.
@@ -376,7 +344,7 @@ __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x
   segment_sums<T, THREADS, 1>(rv, nseg, equal, sh);
   double mine = 0.0;
   for (int i = threadIdx.x; i < nseg; i += THREADS) mine += sh.seg[i];
-  const double all = block_sum64<THREADS>(mine, sh.red);
+  const double all = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
   if (c >= all) return 0x7fffffff;
   double w;
   return pick<T, THREADS>(rv, nseg, c - 0.5, equal, sh, &w);
@@ -505,7 +473,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
           if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], fixed(w));
         }
       });
-      total = block_sum64<THREADS>(total, sh.red);
+      total = block_reduce64<THREADS / 64, Sum64>(total, sh.red);
       target = (double)p * total * unit;
     }
     __syncthreads();
@@ -546,7 +514,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
           if (use_k) {
             double mine = 0.0;
             for (int i = tid; i < k; i += THREADS) mine += weight(value(i));
-            goal = (double)p * block_sum64<THREADS>(mine, sh.red);
+            goal = (double)p * block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
           } else {
             goal = (double)p * total;
             base = ahead / unit;
@@ -572,7 +540,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         if (use_p) {      // the mass of those k
           double mine = 0.0;
           each_element<T, THREADS>(rv, [&](float x, int) { if (x > cut.x) mine += weight(x); });
-          total = block_sum64<THREADS>(mine, sh.red) + ties * weight(cut.x);
+          total = block_reduce64<THREADS / 64, Sum64>(mine, sh.red) + ties * weight(cut.x);
         }
       }
       if (use_p) {
@@ -612,7 +580,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   segment_sums<T, THREADS, UN>(rv, nseg, kept_weight, sh);
   double mine = 0.0;
   for (int i = tid; i < nseg; i += THREADS) mine += sh.seg[i];
-  const double kept = block_sum64<THREADS>(mine, sh.red);
+  const double kept = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
   double w;
   const int col = pick<T, THREADS>(rv, nseg, u * kept, kept_weight, sh, &w);
   if (tid == 0) {
