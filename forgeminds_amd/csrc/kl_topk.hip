@@ -58,6 +58,9 @@ __device__ __forceinline__ SlotBits slot_load(const ListArgs& a, int64_t at) {
   b.t1 = *reinterpret_cast<const uint16_t*>(t + (a.teacher_dtype == FM_F32 ? 2 : 0));
   return b;
 }
+__device__ __forceinline__ int slot_sign(const ListArgs& a, int64_t at) {
+  return static_cast<const int32_t*>(a.idx)[a.idx64 ? at * 2 + 1 : at];
+}
 __device__ __forceinline__ int64_t slot_col(const ListArgs& a, const SlotBits& b) {
   const uint32_t hi = a.idx64 ? b.hi : (uint32_t)((int32_t)b.lo >> 31);
   return (int64_t)(((uint64_t)hi << 32) | b.lo);
@@ -107,15 +110,49 @@ __device__ __forceinline__ uint32_t bits_of(float f) {
   else return pack_f16(f, 0.f) & 0xffffu;
 }
 
-// Workgroup merge of per-thread running (maximum, sum): the maximum in fp32, the sums in 64 bits.
+// A running (maximum, sum) whose sum is held in 64 bits.
 struct Pair64 {
   float m;
   double s;
 };
 template <int NW>
-__device__ __forceinline__ Pair64 block_merge64(MaxSum v, double* smem, float* smemf) {
-  const float m = block_max32<NW>(v.m, smemf);
-  return Pair64{m, block_reduce64<NW, Sum64>((double)v.s * (double)fast_exp2(v.m - m), smem)};
+struct MergeShared {
+  double s[2][NW];
+  float m[2][NW];
+};
+// Workgroup merge of two running pairs per thread, the unlisted columns' and the listed ones': one
+// barrier, the sums in 64 bits, fixed order. `all` is both together.
+template <int NW>
+__device__ __forceinline__ void merge_pairs(const MaxSum& rest_, const MaxSum& listed_, bool with_listed,
+                                            MergeShared<NW>& sh, Pair64* rest, Pair64* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float rm = wave_max(rest_.m);
+  const double rs = wave_sum64((double)rest_.s * (double)fast_exp2(rest_.m - rm));
+  if (lane == 0) { sh.m[0][wave] = rm; sh.s[0][wave] = rs; }
+  if (with_listed) {
+    const float lm = wave_max(listed_.m);
+    const double ls = wave_sum64((double)listed_.s * (double)fast_exp2(listed_.m - lm));
+    if (lane == 0) { sh.m[1][wave] = lm; sh.s[1][wave] = ls; }
+  }
+  __syncthreads();
+  const int w = lane & (NW - 1);
+  const float mr = sh.m[0][w];
+  rest->m = group_reduce<NW, OpMax>(mr);
+  rest->s = group_reduce64<NW, Sum64>(sh.s[0][w] * (double)fast_exp2(mr - rest->m));
+  *all = *rest;
+  if (with_listed) {
+    const float ml = sh.m[1][w];
+    const float lm = group_reduce<NW, OpMax>(ml);
+    all->m = fmaxf(rest->m, lm);
+    const double ls = group_reduce64<NW, Sum64>(sh.s[1][w] * (double)fast_exp2(ml - all->m));
+    all->s = rest->s * (double)fast_exp2(rest->m - all->m) + ls;
+  }
+}
+// one element into a running pair
+__device__ __forceinline__ void fold1(MaxSum& run, float x, float c) {
+  const float cm = __builtin_elementwise_maximum(run.m, x * c);
+  run.s = run.s * fast_exp2(run.m - cm) + fast_exp2(__builtin_fmaf(x, c, -cm));
+  run.m = cm;
 }
 
 // The list of one row in LDS. Distinct columns are found with an open-addressing table (a column's
@@ -127,7 +164,7 @@ struct ListShared {
   static constexpr int kSlots = 2 * KCAP;
   double q[KCAP];
   double red[THREADS / 64];
-  float redf[THREADS / 64];
+  MergeShared<THREADS / 64> merge;
   int hcol[kSlots];
   int hlead[kSlots];
   int col[KCAP];
@@ -137,6 +174,7 @@ struct ListShared {
   uint16_t nxt[KCAP];
   uint16_t head[THREADS];
   int redi[THREADS / 64];
+  int count[THREADS / 64];
 };
 
 // What a thread keeps of its slots (slot j * THREADS + tid) across the sweep.
@@ -309,46 +347,57 @@ __device__ __forceinline__ void walk(const ListShared<THREADS, KCAP>& sh, uint16
   }
 }
 
-// Gradient coefficients of a row and its loss (LOSS), from the merged pairs; the listed columns'
-// gradients go to sh.g. Returns the coefficient of an unlisted column: its gradient is
-// coef * exp2(x * c - rest.m).
-template <typename T, int THREADS, int KCAP, int SL, bool LOSS, bool GRAD>
-__device__ __forceinline__ float finish_row(const ListArgs& a, ListShared<THREADS, KCAP>& sh, const Mine<SL>& mine,
-                                            const Pair64& all, const Pair64& rest, double sum_q, int unique, int v,
-                                            double scale, float* loss_at) {
-  constexpr int NW = THREADS / 64;
-  const double lse2 = (double)all.m + log2_64(all.s);
-  double q_r = 0.0;
+// What the merged pairs and the list make of a row.
+struct RowTerms {
+  double lse2;       // base-2 log-sum-exp of the whole row
+  double q_r;        // probability of the bucket
+  double total;      // sum of q and the bucket
+};
+__device__ __forceinline__ RowTerms row_terms(const ListArgs& a, const Pair64& all, double sum_q, int unique, int v) {
+  RowTerms t;
+  t.lse2 = (double)all.m + log2_64(all.s);
+  t.q_r = 0.0;
   if (a.tail == FM_TAIL_BUCKET && unique < v) {
-    q_r = 1.0 - sum_q;
-    if (q_r < 0.0) q_r = 0.0;          // (a NaN stays)
+    t.q_r = 1.0 - sum_q;
+    if (t.q_r < 0.0) t.q_r = 0.0;          // (a NaN stays)
   }
-  const double total = sum_q + q_r;
-  double term = 0.0;
+  t.total = sum_q + t.q_r;
+  return t;
+}
+// The listed columns' gradients into sh.g, as stored bits (a barrier ends it); returns the coefficient
+// of an unlisted column, whose gradient is coef * exp2(x * c - rest.m).
+template <typename T, int THREADS, int KCAP, int SL>
+__device__ __forceinline__ float row_gradient(const ListArgs& a, ListShared<THREADS, KCAP>& sh, const Mine<SL>& mine,
+                                              const Pair64& all, const Pair64& rest, const RowTerms& t, double scale) {
 #pragma unroll
   for (int j = 0; j < SL; ++j) {
     if (mine.col[j] < 0) continue;
     const int s = j * THREADS + (int)threadIdx.x;
-    const double lp2 = (double)sh.x[s] * (double)a.c - lse2;
-    if (LOSS && !(mine.q[j] == 0.0)) term += mine.q[j] * (log2_64(mine.q[j]) - lp2);
-    if (GRAD) sh.g[s] = bits_of<T>((float)((exp2_64(lp2) * total - mine.q[j]) * scale));
+    const double lp2 = (double)sh.x[s] * (double)a.c - t.lse2;
+    sh.g[s] = bits_of<T>((float)((exp2_64(lp2) * t.total - mine.q[j]) * scale));
   }
-  if (LOSS) {
-    term = block_reduce64<NW, Sum64>(term, sh.red);
-    if (threadIdx.x == 0) {
-      term *= kLn2d;
-      if (!(q_r == 0.0)) term += q_r * (log2_64(q_r) - ((double)rest.m + log2_64(rest.s) - lse2)) * kLn2d;
-      if (sum_q != sum_q) term = sum_q;
-      *loss_at = (float)term;
-    }
-  }
-  if (!GRAD) return 0.f;
-  __syncthreads();                     // sh.g
-  double coef = total * exp2_64((double)rest.m - (double)all.m) / all.s;
-  if (!(q_r == 0.0)) coef -= q_r / rest.s;
+  __syncthreads();
+  double coef = t.total * exp2_64((double)rest.m - (double)all.m) / all.s;
+  if (!(t.q_r == 0.0)) coef -= t.q_r / rest.s;
   // no unlisted column with any probability: their logits are -inf and their gradient 0
-  if (rest.s == 0.0 && q_r == 0.0) coef = 0.0;
+  if (rest.s == 0.0 && t.q_r == 0.0) coef = 0.0;
   return (float)(coef * scale);
+}
+template <int THREADS, int KCAP, int SL>
+__device__ __forceinline__ void row_loss_of(const ListArgs& a, ListShared<THREADS, KCAP>& sh, const Mine<SL>& mine,
+                                            const Pair64& rest, const RowTerms& t, double sum_q, float* loss_at) {
+  double term = 0.0;
+#pragma unroll
+  for (int j = 0; j < SL; ++j) {
+    if (mine.col[j] < 0 || mine.q[j] == 0.0) continue;
+    const double lp2 = (double)sh.x[j * THREADS + (int)threadIdx.x] * (double)a.c - t.lse2;
+    term += mine.q[j] * (log2_64(mine.q[j]) - lp2);
+  }
+  term = block_reduce64<THREADS / 64, Sum64>(term, sh.red);
+  if (threadIdx.x == 0) {
+    if (!(t.q_r == 0.0)) term += t.q_r * (log2_64(t.q_r) - ((double)rest.m + log2_64(rest.s) - t.lse2));
+    *loss_at = (float)(sum_q != sum_q ? sum_q : term * kLn2d);
+  }
 }
 
 // one vector into the running (maximum, sum); a NaN reaches both
@@ -366,21 +415,6 @@ __device__ __forceinline__ void fold(MaxSum& run, const u32x4& r, float c) {
   for (int e = 0; e < EPV; ++e) acc += fast_exp2(__builtin_fmaf(x[e], c, -cm));
   run.m = cm;
   run.s = acc;
-}
-
-// rows with a list among the first `n` (at least 1), read by every workgroup where n is small
-template <int THREADS>
-__device__ __forceinline__ float count_rows(const ListArgs& a, int64_t n, int* redi) {
-  int cnt = 0;
-  for (int64_t i = threadIdx.x; i < n; i += THREADS) cnt += list_idx(a, i * a.k) >= 0 ? 1 : 0;
-  cnt = wave_sum_i(cnt);
-  if ((threadIdx.x & 63) == 0) redi[threadIdx.x >> 6] = cnt;
-  __syncthreads();
-  int t = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / 64; ++i) t += redi[i];
-  __syncthreads();
-  return t > 0 ? (float)t : 1.f;
 }
 
 template <typename T>
@@ -439,6 +473,9 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   // the list's loads go first: waiting for them then waits for nothing of the row
   SlotBits bits[SL];
   list_load<THREADS, SL>(a, row, bits);
+  // where the rows are few, every workgroup counts those with a list itself
+  const int first = GRAD ? slot_sign(a, (int64_t)(tid < count_n ? tid : 0) * a.k) : 0;
+  const float nv = *(GRAD && n_valid != nullptr ? n_valid : static_cast<const float*>(a.idx));
   const float lse_t = *(a.teacher_lse != nullptr ? a.teacher_lse + row : static_cast<const float*>(a.idx));
   const T* vp = rp + sp.head;              // 16-byte aligned where there are vectors
   auto at = [&](int c) { return reinterpret_cast<const T*>(reinterpret_cast<const char*>(vp) + (uint32_t)c * 16u); };
@@ -453,14 +490,23 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   const uint32_t mask = sh.mask[tid];
   const uint16_t head = sh.head[tid];
 
-  // The sweep leaves the listed logits in sh.x and, for the bucket, folds the other columns only.
-  MaxSum run{kNegBig, 0.f};
+  if (GRAD && count_n > 0) {
+    const int c = __builtin_popcountll(__ballot(tid < count_n && first >= 0));
+    if ((tid & 63) == 0) sh.count[tid >> 6] = c;
+  }
+
+  // The sweep leaves the listed logits in sh.x and, for the bucket, folds the two kinds of columns apart.
+  MaxSum run{kNegBig, 0.f}, listed{kNegBig, 0.f};
   auto take = [&](u32x4 r, int c) {
     if (c >= sp.nvec) return;
     if ((mask >> ((c / THREADS) % 31)) & 1u) {
       walk<EPV, THREADS, KCAP>(sh, head, sp.head + c * EPV, [&](int d, int s) {
-        sh.x[s] = get_elem<T>(r, d);
-        if (bucket) set_elem<T>(r, d, bits_of<T>(-INFINITY));
+        const float x = get_elem<T>(r, d);
+        sh.x[s] = x;
+        if (bucket) {
+          fold1(listed, x, a.c);
+          set_elem<T>(r, d, bits_of<T>(-INFINITY));
+        }
       });
     }
     fold<T>(run, r, a.c);
@@ -489,34 +535,17 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     if (mask >> 31) {
       walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) {
         sh.x[s] = x;
-        if (bucket) x = -INFINITY;
+        if (bucket) {
+          fold1(listed, x, a.c);
+          x = -INFINITY;
+        }
       });
     }
-    const float cm = __builtin_elementwise_maximum(run.m, x * a.c);
-    run.s = run.s * fast_exp2(run.m - cm) + fast_exp2(__builtin_fmaf(x, a.c, -cm));
-    run.m = cm;
+    fold1(run, x, a.c);
   }
-  const Pair64 rest = block_merge64<NW>(run, sh.red, sh.redf);
-  Pair64 all = rest;
-  if (bucket) {      // the listed columns join the unlisted ones
-    MaxSum w{rest.m, 0.f};
-#pragma unroll
-    for (int j = 0; j < SL; ++j)
-      if (mine.col[j] >= 0) w.m = __builtin_elementwise_maximum(w.m, sh.x[j * THREADS + tid] * a.c);
-    all.m = block_max32<NW>(w.m, sh.redf);
-    double s = tid == 0 ? rest.s * exp2_64((double)rest.m - (double)all.m) : 0.0;
-#pragma unroll
-    for (int j = 0; j < SL; ++j)
-      if (mine.col[j] >= 0) s += exp2_64((double)sh.x[j * THREADS + tid] * (double)a.c - (double)all.m);
-    all.s = block_reduce64<NW, Sum64>(s, sh.red);
-  }
-  double scale = a.inv_t;
-  if (GRAD) {
-    if (count_n > 0) scale /= (double)count_rows<THREADS>(a, count_n, sh.redi);
-    else if (n_valid != nullptr) scale /= (double)*n_valid;
-  }
-  const float coef = finish_row<T, THREADS, KCAP, SL, true, GRAD>(a, sh, mine, all, rest, sum_q, unique, v, scale,
-                                                               row_loss + row);
+  Pair64 rest, all;
+  merge_pairs<NW>(run, listed, bucket, sh.merge, &rest, &all);      // its barrier also publishes sh.x
+  const RowTerms terms = row_terms(a, all, sum_q, unique, v);
   if (tid == 0 && stats != nullptr) {
     stats[row * 4] = all.m;
     stats[row * 4 + 1] = (float)all.s;
@@ -524,6 +553,15 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     stats[row * 4 + 3] = (float)rest.s;
   }
   if constexpr (GRAD) {
+    double scale = a.inv_t;
+    if (count_n > 0) {
+      int rows = 0;
+      for (int i = 0; i < NW; ++i) rows += sh.count[i];
+      scale /= (double)(rows > 0 ? rows : 1);
+    } else if (n_valid != nullptr) {
+      scale /= (double)nv;
+    }
+    const float coef = row_gradient<T, THREADS, KCAP, SL>(a, sh, mine, all, rest, terms, scale);
     T* vg = gp + sp.head;
     auto put = [&](const u32x4& r, int c) {
       if (c >= sp.nvec) return;
@@ -555,6 +593,8 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
       store_bits(gp + col, one);
     }
   }
+  // last: the reduction runs while the stores drain
+  row_loss_of<THREADS, KCAP, SL>(a, sh, mine, rest, terms, sum_q, row_loss + row);
 }
 
 // The gradient from saved stats. chunks > 1: a workgroup takes one tile of THREADS * UN vectors of a
@@ -600,7 +640,7 @@ __global__ __launch_bounds__(THREADS) void kl_topk_bwd_kernel(const T* student, 
     if (mine.col[j] >= 0) sh.x[j * THREADS + tid] = Elem<T>::load1(rp + mine.col[j]);
   const uint32_t mask = sh.mask[tid];
   const uint16_t head = sh.head[tid];
-  const float coef = finish_row<T, THREADS, KCAP, SL, false, true>(a, sh, mine, all, rest, sum_q, unique, v, scale, nullptr);
+  const float coef = row_gradient<T, THREADS, KCAP, SL>(a, sh, mine, all, rest, row_terms(a, all, sum_q, unique, v), scale);
   for (int c0 = c_begin; c0 < c_end; c0 += THREADS * UN) {
     u32x4 raw[UN];
 #pragma unroll
@@ -642,7 +682,7 @@ __global__ __launch_bounds__(1024) void kl_topk_reduce_kernel(const float* __res
       const int64_t at = i + u * 1024 < n ? i + u * 1024 : i;
       if (LOSS) r[u] = row_loss[at];
       // the sign of slot 0
-      if (COUNT) used[u] = static_cast<const int32_t*>(a.idx)[at * a.k * (a.idx64 ? 2 : 1) + (a.idx64 ? 1 : 0)];
+      if (COUNT) used[u] = slot_sign(a, at * a.k);
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
