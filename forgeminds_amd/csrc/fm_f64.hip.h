@@ -26,11 +26,11 @@ __device__ __forceinline__ double readlane64(double v, int l) {
 struct Sum64 { __device__ static __forceinline__ double f(double a, double b) { return a + b; } };
 struct Max64 { __device__ static __forceinline__ double f(double a, double b) { return b > a ? b : a; } };
 
-// over aligned groups of G lanes (4, 8, 16 or 64), the result in every lane, fixed order
+// over aligned groups of G lanes (1, 2, 4, 8, 16 or 64), the result in every lane, fixed order
 template <int G, typename Op>
 __device__ __forceinline__ double group_reduce64(double v) {
-  v = Op::f(v, dpp64<kDppXor1>(v));
-  v = Op::f(v, dpp64<kDppXor2>(v));
+  if constexpr (G >= 2) v = Op::f(v, dpp64<kDppXor1>(v));
+  if constexpr (G >= 4) v = Op::f(v, dpp64<kDppXor2>(v));
   if constexpr (G >= 8) v = Op::f(v, dpp64<kDppHalfMirror>(v));
   if constexpr (G >= 16) v = Op::f(v, dpp64<kDppMirror>(v));
   if constexpr (G == 64)
@@ -51,17 +51,6 @@ __device__ __forceinline__ double block_reduce64(double v, double* smem) {
   __syncthreads();
   return v;
 }
-template <int NW>
-__device__ __forceinline__ float block_max32(float v, float* smem) {
-  v = wave_max(v);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (lane == 0) smem[wave] = v;
-  __syncthreads();
-  v = group_reduce<NW, OpMax>(smem[lane & (NW - 1)]);
-  __syncthreads();
-  return v;
-}
-
 // 2^t: degree-8 polynomial through the Chebyshev nodes of [-1/2, 1/2] (relative error 1.1e-12) and an
 // exact scaling. Below 2^-1100 the result is zero; NaN stays.
 __device__ __forceinline__ double exp2_64(double t) {

@@ -24,7 +24,6 @@ namespace {
 constexpr int kMaxList = 1024;
 constexpr int kSmallList = 128;
 constexpr uint16_t kEnd = 0xFFFFu;
-constexpr int kNoLead = 0x7fffffff;
 
 struct ListArgs {
   const void* idx;
@@ -155,26 +154,29 @@ __device__ __forceinline__ void fold1(MaxSum& run, float x, float c) {
   run.m = cm;
 }
 
-// The list of one row in LDS. Distinct columns are found with an open-addressing table (a column's
-// first slot leads, the others hand their probability to it, added in slot order); the leaders hang
-// in per-thread chains: chain t holds the listed columns among the vectors that thread t sweeps, and
-// bit i of mask[t] says that there may be one in its i-th vector (bit 31: in the row's unaligned ends).
+// The list of one row in LDS: per-thread chains. Chain t holds the listed columns among the vectors that
+// thread t sweeps, and bit i % 31 of mask[t] says that there may be one in its i-th vector (bit 31: in
+// the row's unaligned ends). A column that occurs twice is found where its chain is walked first; its
+// first slot then leads and takes over what the others have, added in slot order.
 template <int THREADS, int KCAP>
 struct ListShared {
-  static constexpr int kSlots = 2 * KCAP;
-  double q[KCAP];
+  union {
+    double q[KCAP];      // while slots are merged
+    struct {
+      float x[KCAP];     // the student's logit there
+      uint32_t g[KCAP];  // the gradient there, as stored bits
+    };
+  };
   double red[THREADS / 64];
   MergeShared<THREADS / 64> merge;
-  int hcol[kSlots];
-  int hlead[kSlots];
-  int col[KCAP];
-  float x[KCAP];
-  uint32_t g[KCAP];
+  int col[KCAP];         // -1: empty, or merged into another slot
   uint32_t mask[THREADS];
   uint16_t nxt[KCAP];
   uint16_t head[THREADS];
   int redi[THREADS / 64];
   int count[THREADS / 64];
+  float top[THREADS / 64];
+  int twice;
 };
 
 // What a thread keeps of its slots (slot j * THREADS + tid) across the sweep.
@@ -183,13 +185,6 @@ struct Mine {
   int col[SL];       // -1: not the leader of a column
   double q[SL];
 };
-
-// place of a column in a table of SLOTS (a power of two): the high bits of a multiplicative hash, so
-// that columns a power of two apart spread too
-template <int SLOTS>
-__device__ __forceinline__ uint32_t hash_col(int col) {
-  return ((uint32_t)col * 2654435761u) >> (32 - __builtin_ctz(SLOTS));
-}
 
 template <int THREADS, int SL>
 __device__ __forceinline__ void list_load(const ListArgs& a, int64_t row, SlotBits (&bits)[SL]) {
@@ -200,140 +195,158 @@ __device__ __forceinline__ void list_load(const ListArgs& a, int64_t row, SlotBi
   }
 }
 
-// Fills the LDS table and chains and returns the sum of q (NaN when a column is out of range);
-// *unique gets the number of distinct columns. All threads of the workgroup call it.
-template <typename T, int THREADS, int KCAP, int SL>
-__device__ __forceinline__ double list_build(const ListArgs& a, const RowSplit& sp, int64_t row, int v,
-                                             const SlotBits (&bits)[SL], float lse_t,
-                                             ListShared<THREADS, KCAP>& sh, Mine<SL>& mine, int* unique) {
+// The first two listed columns of a thread's chain among its vectors 0 .. RI-1, in registers (vector,
+// element, slot), and the mask of the vectors that hold more of them. A wave meets a listed column in a
+// quarter to most of its vectors; from registers it costs a dozen operations there instead of a walk of
+// dependent LDS reads ([8192,32000] bf16, lists of 64: 235 us with the walk, 228 without).
+constexpr uint32_t kNone = 0xFFFFFFFFu;
+struct Near {
+  uint32_t e0, e1;     // vector | element << 8 | slot << 16
+  uint32_t more;       // as mask, of what is not e0 or e1
+};
+// `twice`: set when two entries of the chain name one column (the walk then ends)
+template <typename T, int THREADS, int KCAP, int RI>
+__device__ __forceinline__ Near near_of(const ListShared<THREADS, KCAP>& sh, const RowSplit& sp, uint16_t head, bool* twice) {
+  constexpr int EPV = Elem<T>::kVec;
+  Near n{kNone, kNone, 0u};
+#pragma unroll 1
+  for (uint32_t s = head; s != kEnd; s = sh.nxt[s]) {
+    const int col = sh.col[s];
+    if (col < 0) continue;
+    bool same = false;
+#pragma unroll 1
+    for (uint32_t o = sh.nxt[s]; o != kEnd && !same; o = sh.nxt[o]) same = sh.col[o] == col;
+    if (same) { *twice = true; break; }
+    if (col < sp.head || col >= sp.tail0) { n.more |= 1u << 31; continue; }
+    const uint32_t vec = (uint32_t)(col - sp.head) / EPV, d = (uint32_t)(col - sp.head) % EPV, i = vec / THREADS;
+    const uint32_t e = i | d << 8 | s << 16;
+    if (i < (uint32_t)RI && n.e0 == kNone) n.e0 = e;
+    else if (i < (uint32_t)RI && n.e1 == kNone) n.e1 = e;
+    else n.more |= 1u << (i % 31);
+  }
+  return n;
+}
+
+// Fills the chains and returns the sum of q (NaN when a column is out of range); *unique gets the number
+// of distinct columns. Three barriers; columns that occur twice cost three more. Only columns among the
+// vectors [c_begin, c_end) and, with `ends`, the row's unaligned ends are hung into chains. All threads
+// of the workgroup call it.
+template <typename T, int THREADS, int KCAP, int SL, int RI>
+__device__ __forceinline__ double list_build(const ListArgs& a, const RowSplit& sp, int v, const SlotBits (&bits)[SL],
+                                             float lse_t, int c_begin, int c_end, bool ends,
+                                             ListShared<THREADS, KCAP>& sh, Mine<SL>& mine, Near* near, int* unique) {
   constexpr int NW = THREADS / 64;
   constexpr int EPV = Elem<T>::kVec;
-  constexpr int HS = ListShared<THREADS, KCAP>::kSlots;
-  const int tid = threadIdx.x;
-  for (int i = tid; i < HS; i += THREADS) { sh.hcol[i] = -1; sh.hlead[i] = kNoLead; }
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool renorm = a.tail == FM_TAIL_RENORM, logits = a.probs == FM_TEACHER_LOGITS;
   sh.mask[tid] = 0u;
   sh.head[tid] = kEnd;
+  if (tid == 0) sh.twice = 0;
   bool bad = false;
   float t[SL];
   bool used[SL];
+  float mx = -INFINITY;
+  int places = 0;
 #pragma unroll
   for (int j = 0; j < SL; ++j) {
-    const int64_t c = j * THREADS + tid < a.k ? slot_col(a, bits[j]) : -1;
+    const int s = j * THREADS + tid;
+    const int64_t c = s < a.k ? slot_col(a, bits[j]) : -1;
     t[j] = slot_value(a, bits[j]);
     used[j] = c >= 0;
     bad |= c >= v;
-    mine.col[j] = c >= v ? -1 : (int)c;
-    if (c < 0) mine.col[j] = -1;
-    mine.q[j] = 0.0;
+    mine.col[j] = c >= 0 && c < v ? (int)c : -1;
+    if (s < KCAP) sh.col[s] = mine.col[j];
+    if (used[j]) mx = fmaxf(mx, t[j]);
+    places += mine.col[j] >= 0 ? 1 : 0;
   }
-  // teacher probabilities of the used slots
-  if (a.probs == FM_TEACHER_PROBS) {
-#pragma unroll
-    for (int j = 0; j < SL; ++j) if (used[j]) mine.q[j] = (double)t[j];
-  } else if (a.tail == FM_TAIL_RENORM) {
-    double mx = -__builtin_inf();
-#pragma unroll
-    for (int j = 0; j < SL; ++j) if (used[j]) mx = (double)t[j] > mx ? (double)t[j] : mx;
-    mx = block_reduce64<NW, Max64>(mx, sh.red);
-#pragma unroll
-    for (int j = 0; j < SL; ++j) if (used[j]) mine.q[j] = exp2_64(((double)t[j] - mx) * (a.inv_t * kLog2ed));
-  } else {
-    const double l = (double)lse_t;
-#pragma unroll
-    for (int j = 0; j < SL; ++j) if (used[j]) mine.q[j] = exp2_64(((double)t[j] * a.inv_t - l) * kLog2ed);
+  if (renorm && logits) {
+    mx = wave_max(mx);
+    if (lane == 0) sh.top[wave] = mx;
   }
+  __syncthreads();
+  // teacher probabilities, and the slots into the chains of the threads that sweep their columns
+  const double shift = !logits ? 0.0
+                       : renorm ? (double)group_reduce<NW, OpMax>(sh.top[lane & (NW - 1)]) * a.inv_t : (double)lse_t;
   double sum = bad ? __builtin_nan("") : 0.0;
 #pragma unroll
-  for (int j = 0; j < SL; ++j) sum += mine.q[j];
-  sum = block_reduce64<NW, Sum64>(sum, sh.red);      // its barriers also publish the cleared table
-  if (a.tail == FM_TAIL_RENORM) {
-    const double r = 1.0 / sum;
-#pragma unroll
-    for (int j = 0; j < SL; ++j) mine.q[j] *= r;
-    sum = sum * r;                                    // 1, or NaN
-  }
-  // distinct columns
-  int at[SL];
-#pragma unroll
   for (int j = 0; j < SL; ++j) {
-    at[j] = -1;
-    if (mine.col[j] >= 0) {
-      const int s = j * THREADS + tid;
-      sh.q[s] = mine.q[j];
-      uint32_t h = hash_col<HS>(mine.col[j]);
-      for (;;) {       // at most KCAP of the 2 * KCAP places are taken, so this ends
-        const int was = atomicCAS(&sh.hcol[h], -1, mine.col[j]);
-        if (was == -1 || was == mine.col[j]) break;
-        h = (h + 1) % HS;
-      }
-      at[j] = (int)h;
-      atomicMin(&sh.hlead[h], s);
-    }
-  }
-  __syncthreads();
-  bool again[SL];
-#pragma unroll
-  for (int j = 0; j < SL; ++j) {
-    const int s = j * THREADS + tid;
-    again[j] = false;
-    if (s < KCAP) sh.col[s] = mine.col[j];       // -1 in an empty slot
-    if (at[j] >= 0) again[j] = sh.hlead[at[j]] != s;
-  }
-  __syncthreads();
-  // a leader with followers: mark the place (the key itself is no longer needed)
-#pragma unroll
-  for (int j = 0; j < SL; ++j) if (again[j]) { sh.hcol[at[j]] = -2; mine.col[j] = -1; mine.q[j] = 0.0; }
-  __syncthreads();
-  int lead = 0;
-#pragma unroll
-  for (int j = 0; j < SL; ++j) {
-    if (mine.col[j] < 0) continue;
-    const int s = j * THREADS + tid;
-    ++lead;
-    if (sh.hcol[at[j]] == -2) {
-      double q = mine.q[j];
-      for (int o = s + 1; o < a.k; ++o) {      // in slot order
-        const double more = sh.q[o];
-        if (sh.col[o] == mine.col[j]) q += more;
-      }
-      mine.q[j] = q;
-    }
-    // hang it into the chain of the thread that sweeps this column
-    const int col = mine.col[j];
+    const int s = j * THREADS + tid, col = mine.col[j];
+    mine.q[j] = 0.0;
+    if (used[j]) mine.q[j] = logits ? exp2_64(((double)t[j] * a.inv_t - shift) * kLog2ed) : (double)t[j];
+    sum += mine.q[j];
+    if (col < 0) continue;
     int owner;
     uint32_t bit;
     if (col >= sp.head && col < sp.tail0) {
       const int vec = (col - sp.head) / EPV;
+      if (vec < c_begin || vec >= c_end) continue;
       owner = vec % THREADS;
       bit = 1u << ((vec / THREADS) % 31);
     } else {
-      const int e = col < sp.head ? col : sp.head + (col - sp.tail0);
-      owner = e % THREADS;
+      if (!ends) continue;
+      owner = (col < sp.head ? col : sp.head + (col - sp.tail0)) % THREADS;
       bit = 1u << 31;
     }
     atomicOr(&sh.mask[owner], bit);
     // 16-bit exchange on the 32-bit word that holds the head
     uint32_t* word = reinterpret_cast<uint32_t*>(&sh.head[owner & ~1]);
-    const int shift = (owner & 1) * 16;
+    const int shift16 = (owner & 1) * 16;
     uint32_t old = *word, seen;
     do {
       seen = old;
-      const uint32_t now = (seen & ~(0xFFFFu << shift)) | ((uint32_t)s << shift);
+      const uint32_t now = (seen & ~(0xFFFFu << shift16)) | ((uint32_t)s << shift16);
       old = atomicCAS(word, seen, now);
     } while (old != seen);
-    sh.nxt[s] = (uint16_t)(seen >> shift);
+    sh.nxt[s] = (uint16_t)(seen >> shift16);
   }
-  *unique = 0;
-  if (a.tail == FM_TAIL_BUCKET) {
-    lead = wave_sum_i(lead);
-    if ((tid & 63) == 0) sh.redi[tid >> 6] = lead;
+  sum = wave_sum64(sum);
+  places = wave_sum_i(places);
+  if (lane == 0) { sh.red[wave] = sum; sh.redi[wave] = places; }
+  __syncthreads();
+  bool twice = false;
+  *near = near_of<T, THREADS, KCAP, RI>(sh, sp, sh.head[tid], &twice);
+  if (twice) sh.twice = 1;
+  sum = group_reduce64<NW, Sum64>(sh.red[lane & (NW - 1)]);
+  int u = 0;
+  for (int i = 0; i < NW; ++i) u += sh.redi[i];
+  if (renorm) {
+    const double r = 1.0 / sum;
+#pragma unroll
+    for (int j = 0; j < SL; ++j) mine.q[j] *= r;
+    sum = sum * r;                                    // 1, or NaN
   }
   __syncthreads();
-  if (a.tail == FM_TAIL_BUCKET) {
-    int u = 0;
-    for (int i = 0; i < NW; ++i) u += sh.redi[i];
-    *unique = u;
+  if (sh.twice) {
+    int lost = 0;
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (j * THREADS + tid < KCAP) sh.q[j * THREADS + tid] = mine.q[j];
+    __syncthreads();
+    bool follows[SL];
+#pragma unroll
+    for (int j = 0; j < SL; ++j) {
+      const int s = j * THREADS + tid;
+      follows[j] = false;
+      if (mine.col[j] < 0) continue;
+      double q = 0.0;
+      for (int o = 0; o < a.k; ++o) {      // in slot order, whichever slot leads
+        const double more = sh.q[o];
+        const bool same = sh.col[o] == mine.col[j];
+        if (same) q += more;
+        follows[j] |= same && o < s;
+      }
+      mine.q[j] = q;
+      if (follows[j]) ++lost;
+    }
+    lost = wave_sum_i(lost);
+    if (lane == 0) sh.count[wave] = lost;
+    __syncthreads();
+    for (int i = 0; i < NW; ++i) u -= sh.count[i];
+#pragma unroll
+    for (int j = 0; j < SL; ++j) if (follows[j]) { sh.col[j * THREADS + tid] = -1; mine.col[j] = -1; mine.q[j] = 0.0; }
+    __syncthreads();
+    *near = near_of<T, THREADS, KCAP, RI>(sh, sp, sh.head[tid], &twice);
   }
+  *unique = u;
   return sum;
 }
 
@@ -443,7 +456,8 @@ __device__ __forceinline__ u32x4 grad_of(const u32x4& r, float scale, float m, f
 // what a row has beyond them read twice. !GRAD: loss and stats from one streaming read (RI vectors
 // a thread in flight). VEC: the buffers are 16-byte aligned and every row holds a whole vector, so the
 // row's loads stand behind no branch -- behind one, the first wait of the list's loads would be a wait
-// for all of them ([4096,128256] bf16, loss and gradient: 552 us). !VEC: one element at a time.
+// for all of them ([4096,128256] bf16, loss and gradient, one workgroup a row and compute unit: 552 us
+// behind one, 479 without). !VEC: one element at a time.
 template <typename T, int THREADS, int KCAP, int RI, bool GRAD, bool VEC>
 __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, ListArgs a, float* __restrict__ row_loss,
                                                           float* __restrict__ stats, const float* __restrict__ n_valid,
@@ -486,8 +500,10 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   }
   Mine<SL> mine;
   int unique;
-  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, sp, row, v, bits, lse_t, sh, mine, &unique);
-  const uint32_t mask = sh.mask[tid];
+  Near near;
+  const double sum_q = list_build<T, THREADS, KCAP, SL, VEC ? RI : 0>(a, sp, v, bits, lse_t, 0, sp.nvec, true, sh, mine,
+                                                                      &near, &unique);
+  uint32_t mask = sh.mask[tid];
   const uint16_t head = sh.head[tid];
 
   if (GRAD && count_n > 0) {
@@ -497,23 +513,33 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
 
   // The sweep leaves the listed logits in sh.x and, for the bucket, folds the two kinds of columns apart.
   MaxSum run{kNegBig, 0.f}, listed{kNegBig, 0.f};
-  auto take = [&](u32x4 r, int c) {
+  auto meet = [&](u32x4& r, int d, int s) {
+    const float x = get_elem<T>(r, d);
+    sh.x[s] = x;
+    if (bucket) {
+      fold1(listed, x, a.c);
+      set_elem<T>(r, d, bits_of<T>(-INFINITY));
+    }
+  };
+  auto take = [&](u32x4 r, int c) {       // what the registers of near_of do not cover
     if (c >= sp.nvec) return;
-    if ((mask >> ((c / THREADS) % 31)) & 1u) {
+    if ((near.more >> ((c / THREADS) % 31)) & 1u) {
       walk<EPV, THREADS, KCAP>(sh, head, sp.head + c * EPV, [&](int d, int s) {
-        const float x = get_elem<T>(r, d);
-        sh.x[s] = x;
-        if (bucket) {
-          fold1(listed, x, a.c);
-          set_elem<T>(r, d, bits_of<T>(-INFINITY));
-        }
+        if (s != (int)(near.e0 >> 16) && s != (int)(near.e1 >> 16)) meet(r, d, s);
       });
     }
     fold<T>(run, r, a.c);
   };
   if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < RI; ++i) take(raw[i], i * THREADS + tid);
+    for (int i = 0; i < RI; ++i) {
+      u32x4 r = raw[i];
+      if ((mask >> (i % 31)) & 1u) {
+        if ((near.e0 & 255u) == (uint32_t)i) meet(r, (near.e0 >> 8) & 15u, (int)(near.e0 >> 16));
+        if ((near.e1 & 255u) == (uint32_t)i) meet(r, (near.e1 >> 8) & 15u, (int)(near.e1 >> 16));
+      }
+      take(r, i * THREADS + tid);
+    }
     constexpr int UN = GRAD ? 2 : RI;
     for (int c0 = RI * THREADS; c0 < sp.nvec; c0 += UN * THREADS) {
       u32x4 more[UN];
@@ -562,6 +588,10 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
       scale /= (double)nv;
     }
     const float coef = row_gradient<T, THREADS, KCAP, SL>(a, sh, mine, all, rest, terms, scale);
+    const uint32_t g0 = near.e0 != kNone ? sh.g[near.e0 >> 16] : 0u, g1 = near.e1 != kNone ? sh.g[near.e1 >> 16] : 0u;
+    // taken afresh: the comparisons of the sweep are not worth keeping in scalar registers until here
+    int me = tid;
+    asm volatile("" : "+v"(near.e0), "+v"(near.e1), "+v"(near.more), "+v"(mask), "+v"(me));
     T* vg = gp + sp.head;
     auto put = [&](const u32x4& r, int c) {
       if (c >= sp.nvec) return;
@@ -572,7 +602,14 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
 #pragma unroll
       for (int i = 0; i < RI; ++i) {
         touch_whole(raw[i]);
-        put(raw[i], i * THREADS + tid);
+        const int c = i * THREADS + me;
+        if (c >= sp.nvec) continue;
+        u32x4 o = grad_of<T, THREADS, KCAP>(raw[i], a.c, rest.m, coef, sh, near.more, head, c, sp.head + c * EPV);
+        if ((mask >> (i % 31)) & 1u) {
+          if ((near.e0 & 255u) == (uint32_t)i) set_elem<T>(o, (near.e0 >> 8) & 15u, g0);
+          if ((near.e1 & 255u) == (uint32_t)i) set_elem<T>(o, (near.e1 >> 8) & 15u, g1);
+        }
+        store16_stream(reinterpret_cast<T*>(reinterpret_cast<char*>(vg) + (uint32_t)c * 16u), o);
       }
       for (int c0 = RI * THREADS; c0 < sp.nvec; c0 += 2 * THREADS) {
         u32x4 more[2];
@@ -634,7 +671,9 @@ __global__ __launch_bounds__(THREADS) void kl_topk_bwd_kernel(const T* student, 
   if (n_valid != nullptr) scale /= (double)*n_valid;
   Mine<SL> mine;
   int unique;
-  const double sum_q = list_build<T, THREADS, KCAP, SL>(a, sp, row, v, bits, lse_t, sh, mine, &unique);
+  Near near;
+  const double sum_q = list_build<T, THREADS, KCAP, SL, 0>(a, sp, v, bits, lse_t, c_begin, c_end, chunk == 0, sh, mine,
+                                                           &near, &unique);
 #pragma unroll
   for (int j = 0; j < SL; ++j)
     if (mine.col[j] >= 0) sh.x[j * THREADS + tid] = Elem<T>::load1(rp + mine.col[j]);
@@ -749,12 +788,21 @@ void launch_loss_grad(const void* student, const ListArgs& a, float* row_loss, f
 #define GO(TH, RI, VEC)                                                                                      \
   FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, true, VEC>), dim3((unsigned)n), dim3(TH), 0, st,                \
             static_cast<const T*>(student), a, row_loss, stats, n_valid, count_n, static_cast<T*>(dstudent), v)
+  // Smallest workgroups that hold a row in 16 vectors a thread: several rows a compute unit, in different
+  // phases. Wide rows do better with half of the row held by each of two workgroups a unit and the rest
+  // read again from the caches than with one workgroup that holds all of it ([4185,128256] bf16: 433
+  // against 520 us; [2684,200000]: 455 against 458; fp32 [2092,128256]: 508 against 430, so not beyond
+  // 20480 vectors), unless there is no second row for the unit ([16,128256]: 27 us against 29).
+  // A long list (KCAP 1024) wants more threads than a short row does.
+  const bool few = n <= fm_host::num_cus();
   if (!vec_ok || v < 2 * Elem<T>::kVec) GO(256, 2, false);
-  else if (nvec <= 256 * 2) GO(256, 2, true);
-  else if (nvec <= 256 * 8) GO(256, 8, true);
-  else if (nvec <= 512 * 8) GO(512, 8, true);
-  else if (nvec <= 1024 * 8) GO(1024, 8, true);
-  else GO(1024, 16, true);
+  else if (nvec > (few ? 8192 : 20480)) GO(1024, 16, true);
+  else if (nvec > 4096 || (few && nvec > 2048)) GO(512, 16, true);
+  else if (nvec > 2048) GO(256, 16, true);
+  else if constexpr (KCAP > kSmallList) GO(256, 8, true);
+  else if (nvec > 1024) GO(128, 16, true);
+  else if (nvec > 512) GO(128, 8, true);
+  else GO(64, 8, true);
 #undef GO
 }
 
@@ -765,9 +813,16 @@ void launch_fwd(const void* student, const ListArgs& a, float* row_loss, float* 
 #define GO(TH, RI, VEC)                                                                                      \
   FM_LAUNCH((kl_topk_kernel<T, TH, KCAP, RI, false, VEC>), dim3((unsigned)n), dim3(TH), 0, st,               \
             static_cast<const T*>(student), a, row_loss, stats, nullptr, 0, static_cast<T*>(nullptr), v)
+  // one streaming read: rows in small workgroups, more threads where few rows have to fill the device
+  const bool few = n <= fm_host::num_cus();
   if (!vec_ok || v < 2 * Elem<T>::kVec) GO(256, 4, false);
-  else if (nvec <= 256 * 8) GO(256, 4, true);
-  else GO(512, 4, true);
+  else if (few && nvec > 8192) GO(1024, 4, true);
+  else if (nvec > 8192) GO(512, 4, true);
+  else if (few && nvec > 2048) GO(512, 8, true);
+  else if (nvec > 2048) GO(256, 8, true);
+  else if constexpr (KCAP > kSmallList) GO(256, 4, true);
+  else if (nvec > 256) GO(128, 8, true);
+  else GO(64, 4, true);
 #undef GO
 }
 
@@ -783,8 +838,11 @@ void launch_bwd(const void* student, const ListArgs& a, const float* stats, cons
               static_cast<const T*>(student), a, stats, n_valid, grad_out, per_row, static_cast<T*>(dstudent), \
               v, vec_ok, (int)chunks);                                                                        \
   } while (0)
-  if (nvec <= 256 * 4) GO(256, 4);
-  else GO(1024, 4);
+  if (nvec > 2048 && KCAP > kSmallList) GO(512, 8);
+  else if (nvec > 1024) GO(256, 8);
+  else if constexpr (KCAP > kSmallList) GO(256, 4);
+  else if (nvec > 256) GO(128, 4);
+  else GO(64, 4);
 #undef GO
 }
 
