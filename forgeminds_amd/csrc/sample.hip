@@ -13,12 +13,16 @@
 //
 // One workgroup per row, which reads it once from memory and again from the caches:
 //   1  maximum of the row (NaN propagates)
-//   2  where top-k or top-p cut: a histogram over 2048 equal steps of the logit below the maximum --
-//      counts for top-k, masses (64-bit fixed point: integer adds give the same sum in any order) for
-//      top-p -- names the step that holds the cut; that step's few elements are sorted. Rows where the
-//      step holds more than a list's worth (long runs of equal values, a cut far below the maximum)
-//      take a radix search over the bits of the value
-//   3  kept mass of each 64-vector segment in index order, the segment that holds u, the token in it
+//   2  candidates: the elements from the maximum down to a bound at or below the cut, into a list in LDS.
+//      top-k: the waves' thread maxima vouch for k elements above the bound. min-p: its own bound. top-p
+//      alone: a histogram of the row's masses (64-bit fixed point: integer adds give the same sum in any
+//      order) over 2048 equal steps of the logit names the step that holds the cut
+//   3  the exact cut: histograms of the list narrow it to one step, whose elements are put in order
+//   4  token: masses of the segments in index order, the segment that holds u, the token in it -- from the
+//      list, or over the row again where the list is too long (flat rows) or nothing cuts
+// Weights are computed for the candidates only, unless the mass of the whole row is asked for. Steps with
+// more elements than the ordering takes (runs of equal values) and cuts far below the maximum are searched
+// by the bits of the value, over the row.
 #include "../../include/fm_hip_tokens.h"
 #include "fm_f64.hip.h"
 #include "fm_topk.hip.h"
@@ -28,8 +32,7 @@ using namespace fm;
 namespace {
 
 constexpr int kBins = 2048;
-constexpr int kList = 1024;          // candidates that are sorted
-constexpr int kMaxSegs = 4096;       // segments of 64 vectors
+constexpr int kStep = 1024;          // candidates of one step (or one segment)
 constexpr int64_t kMaxCols = 1 << 20;
 
 struct SampleArgs {
@@ -77,18 +80,24 @@ struct RowView {
   __device__ __forceinline__ bool whole(int c) const { return c >= w0 && c < w1; }
   __device__ __forceinline__ int clamp(int c) const { return c < w0 ? w0 : (c < w1 ? c : w1 - 1); }
   __device__ __forceinline__ int col0(int c) const { return c * EPV - lead; }
+  __device__ __forceinline__ float load_one(int col) const {
+    return Elem<T>::load1(base + lead + col);
+  }
   __device__ __forceinline__ u32x4 partial(int c) const {
     float f[EPV];
 #pragma unroll
     for (int e = 0; e < EPV; ++e) {
       const int col = col0(c) + e;
-      f[e] = (col >= 0 && col < v) ? Elem<T>::load1(base + (int64_t)c * EPV + e) : -INFINITY;
+      f[e] = (col >= 0 && col < v) ? load_one(col) : -INFINITY;
     }
     return Elem<T>::pack(f);
   }
-  __device__ __forceinline__ u32x4 load(int c) const {
-    return whole(c) ? load16(base + (int64_t)c * EPV) : partial(c);
+  // one whole vector: the address space is spelled out, since behind the views' pointers the compiler
+  // takes the load for a flat one, whose wait is a wait for everything
+  __device__ __forceinline__ u32x4 load_whole(int c) const {
+    return *(const __attribute__((address_space(1))) u32x4*)(reinterpret_cast<const char*>(base) + (uint32_t)c * 16u);
   }
+  __device__ __forceinline__ u32x4 load(int c) const { return whole(c) ? load_whole(c) : partial(c); }
 };
 
 struct Cut {
@@ -98,30 +107,75 @@ struct Cut {
 
 template <int THREADS>
 struct SampleShared {
+  static constexpr int kList = 4 * THREADS;                  // candidates
+  static constexpr int kSegs = THREADS < 1024 ? 32 : 4160;   // segments of 64 vectors (v <= 2^20)
   union {
     struct {
       unsigned long long bins[kBins];
-      unsigned long long list[kList];
-      unsigned long long sorted[kList];
+      unsigned long long list[kList];       // (key << 32) | ~column: larger comes first
+      unsigned long long step[kStep];       // the candidates of one step or segment ...
+      unsigned long long mass[kStep];       // ... and their weights
     } h;
-    double seg[kMaxSegs];
+    double seg[kSegs];
   };
   double red[THREADS / 64];
-  float redf[2][THREADS / 64];
+  float redf[1][THREADS / 64];
   unsigned long long redu[THREADS / 64];
   int redi[THREADS / 64];
   int count;
   int at;
   int col;
+  uint32_t klo, khi;
   float x;
-  double mass;
+  double weight;
 };
 
-// exp((x - m) / T) = 2^((x - m) c), to 1.1e-12. The maximum's weight is exactly 1, so that rows of few
-// distinct values split evenly; that of -inf is zero.
+// exp((x - m) / T) = 2^((x - m) c) by the polynomial of exp2_64, written out for several elements at once:
+// seventeen operations each, the constants in scalar registers (the compiler otherwise copies each into
+// two vector registers for every use, which doubles the work), and n from the low bits of t + 1.5 * 2^52.
+// The maximum's weight is exactly 1, so that rows of few distinct values split evenly; that of -inf is 0.
 struct Weight {
   double m, c;
-  __device__ __forceinline__ double operator()(float x) const { return exp2_64(((double)x - m) * c); }
+  double k[9], magic, least;
+  __device__ __forceinline__ Weight(float max_x, float T) : m((double)max_x), c(kLog2ed / (double)T) {
+    k[8] = 1.3255224878668817e-06; k[7] = 1.5310079402249296e-05; k[6] = 0.00015403455852453838;
+    k[5] = 0.0013333450568000645; k[4] = 0.009618129159402558; k[3] = 0.05550410941205933;
+    k[2] = 0.2402265069581299; k[1] = 0.6931471805459335; k[0] = 1.0;
+    magic = 6755399441055744.0;
+    least = -1100.0;
+#pragma unroll
+    for (int i = 0; i < 9; ++i) asm("" : "+s"(k[i]));
+    asm("" : "+s"(magic), "+s"(least));
+  }
+  template <int N>
+  __device__ __forceinline__ void eval(const float* x, double* w) const {
+    double f[N], r[N];
+    int n[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      double t = ((double)x[i] - m) * c;
+      asm("v_max_f64 %0, %1, %2" : "=v"(t) : "v"(t), "s"(least));
+      const double s = t + magic;
+      n[i] = (int)(uint32_t)__builtin_bit_cast(uint64_t, s);
+      f[i] = t - (s - magic);
+      r[i] = k[8];
+    }
+#pragma unroll
+    for (int j = 7; j >= 0; --j) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = __builtin_fma(r[i], f[i], k[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[i] = __builtin_amdgcn_ldexp(r[i], n[i]);
+      if (N > 1) asm volatile("" : "+v"(w[i]));      // here, side by side, not where each is used
+    }
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    double w;
+    eval<1>(&x, &w);
+    return w;
+  }
 };
 
 // First of `n` non-negative entries (in LDS, in order) whose running sum reaches `target`
@@ -138,7 +192,7 @@ __device__ __forceinline__ int find_running(F entry, int n, double target, Sampl
   }
   const double incl = wave_incl64(mine);
   if ((tid & 63) == 63) sh.red[wave] = incl;
-  if (tid == 0) { sh.at = n; sh.mass = 0.0; }
+  if (tid == 0) { sh.at = n; sh.weight = 0.0; }
   __syncthreads();
   double ahead = 0.0;
 #pragma unroll
@@ -156,9 +210,9 @@ __device__ __forceinline__ int find_running(F entry, int n, double target, Sampl
   if (hit < n) atomicMin(&sh.at, hit);
   __syncthreads();
   const int found = sh.at;
-  if (hit < n && hit == found) sh.mass = hit_before;
+  if (hit < n && hit == found) sh.weight = hit_before;
   __syncthreads();
-  *before = sh.mass;
+  *before = sh.weight;
   __syncthreads();
   return found;
 }
@@ -171,7 +225,7 @@ __device__ __forceinline__ void each_vector(const RowView<T>& rv, F fn) {
     u32x4 raw[UN];
     if (any) {
 #pragma unroll
-      for (int i = 0; i < UN; ++i) raw[i] = load16(rv.base + (int64_t)rv.clamp(c0 + i * THREADS) * Elem<T>::kVec);
+      for (int i = 0; i < UN; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * THREADS));
     }
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
@@ -196,11 +250,11 @@ __device__ __forceinline__ void each_element(const RowView<T>& rv, F fn) {
 }
 
 // The token among the segments whose weights are in sh.seg (nseg of them): the first column whose
-// running weight exceeds `target`. weight_of(x, col) gives an element's weight. Rounding may leave the
+// running weight exceeds `target`. weights_of(x, col0, w) gives the weights of a vector. Rounding may leave the
 // target at the very end: then the last column with a weight. Returns the column; *w its weight.
 template <typename T, int THREADS, typename F>
-__device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double target, F weight_of, SampleShared<THREADS>& sh,
-                                    double* w) {
+__device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double target, F weights_of,
+                                    SampleShared<THREADS>& sh, double* w) {
   constexpr int EPV = Elem<T>::kVec;
   double before;
   int s = find_running<THREADS, true>([&](int i) { return sh.seg[i]; }, nseg, target, sh, &before);
@@ -222,10 +276,10 @@ __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double targe
     double wt[EPV];
     double mine = 0.0;
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) {
-      wt[e] = c < rv.nvec ? weight_of(x[e], rv.col0(c) + e) : 0.0;
-      mine += wt[e];
-    }
+    for (int e = 0; e < EPV; ++e) wt[e] = 0.0;
+    if (c < rv.nvec) weights_of(x, rv.col0(c), wt);
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) mine += wt[e];
     const double incl = wave_incl64(mine);
     double run = before + (incl - mine);
     int hit = -1, last = -1;
@@ -242,18 +296,18 @@ __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double targe
     else if (some != 0ull) from = 63 - __builtin_clzll(some);
     const int col = any != 0ull ? __shfl(hit, from, 64) : __shfl(last, from, 64);
     const double cw = any != 0ull ? __shfl(hit_w, from, 64) : __shfl(last_w, from, 64);
-    if (lane == 0) { sh.col = col; sh.mass = cw; }
+    if (lane == 0) { sh.col = col; sh.weight = cw; }
   }
   __syncthreads();
   const int col = sh.col;
-  *w = sh.mass;
+  *w = sh.weight;
   __syncthreads();
   return col;
 }
 
-// Segment sums (64 vectors, a wave each) of weight_of over the row into sh.seg.
+// Segment sums (64 vectors, a wave each) of weights_of(x, col0, w) over the row into sh.seg.
 template <typename T, int THREADS, int UN, typename F>
-__device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F weight_of, SampleShared<THREADS>& sh) {
+__device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F weights_of, SampleShared<THREADS>& sh) {
   constexpr int EPV = Elem<T>::kVec;
   __syncthreads();
   const bool any = rv.w0 < rv.w1;
@@ -261,7 +315,7 @@ __device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F w
     u32x4 raw[UN];
     if (any) {
 #pragma unroll
-      for (int i = 0; i < UN; ++i) raw[i] = load16(rv.base + (int64_t)rv.clamp(c0 + i * THREADS) * EPV);
+      for (int i = 0; i < UN; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * THREADS));
     }
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
@@ -272,9 +326,11 @@ __device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F w
       if (c < rv.nvec) {
         if (!rv.whole(c)) raw[i] = rv.partial(c);
         float x[EPV];
+        double w[EPV];
         Elem<T>::unpack(raw[i], x);
+        weights_of(x, rv.col0(c), w);
 #pragma unroll
-        for (int e = 0; e < EPV; ++e) mine += weight_of(x[e], rv.col0(c) + e);
+        for (int e = 0; e < EPV; ++e) mine += w[e];
       }
       mine = wave_sum64(mine);
       if ((threadIdx.x & 63) == 0) sh.seg[c >> 6] = mine;
@@ -283,26 +339,27 @@ __device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F w
   __syncthreads();
 }
 
-// Radix search over the whole row, from memory: the value of the element at which the running amount
-// (in descending order of value) reaches `target`, and the amount above that value. amount(x) is what
-// an element of value x adds, as an integer. Equal neighbours of a thread are added up before they go
-// to the histogram, so that a row of one value does not queue on one address.
+// Search by the bits of the value, over the row: the key among [lo, hi] at which the running amount, in
+// descending order of value and `ahead` at the start, reaches `goal`; *above gets the amount above that
+// key. amount(x) is what an element adds, an integer. 2048 equal ranges of keys a round. Equal
+// neighbours of a thread are added up before they go to the histogram, so that a row of few values does
+// not queue on few addresses.
 template <typename T, int THREADS, typename F>
-__device__ __forceinline__ uint32_t radix_cut(const RowView<T>& rv, double target, F amount, SampleShared<THREADS>& sh,
-                                              unsigned long long* above) {
-  uint32_t prefix = 0u;
-  unsigned long long sum_above = 0ull;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+__device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo, uint32_t hi, unsigned long long ahead,
+                                               double goal, F amount, SampleShared<THREADS>& sh,
+                                               unsigned long long* above) {
+  while (lo < hi) {
+    const int bits = 32 - __builtin_clz(hi - lo);
+    const int shift = bits > 11 ? bits - 11 : 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += THREADS) sh.h.bins[i] = 0ull;
+    for (int i = threadIdx.x; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
     __syncthreads();
     int open = -1;
     unsigned long long held = 0ull;
     each_element<T, THREADS>(rv, [&](float x, int col) {
-      if (col < 0 || col >= rv.v) return;
       const uint32_t key = key_of(x);
-      if (shift < 24 && ((key ^ prefix) >> (shift + 8)) != 0u) return;
-      const int b = (int)((key >> shift) & 255u);
+      if (key < lo || key > hi || col < 0 || col >= rv.v) return;
+      const int b = (int)((hi - key) >> shift);
       if (b != open) {
         if (open >= 0) atomicAdd(&sh.h.bins[open], held);
         open = b;
@@ -312,36 +369,38 @@ __device__ __forceinline__ uint32_t radix_cut(const RowView<T>& rv, double targe
     });
     if (open >= 0) atomicAdd(&sh.h.bins[open], held);
     __syncthreads();
-    if (threadIdx.x == 0) {
-      unsigned long long run = sum_above;
-      int b = 255, lowest = 0;
-      for (; b >= 0; --b) {
-        const unsigned long long w = sh.h.bins[b];
-        if (w != 0ull) lowest = b;
-        if (w != 0ull && (double)(run + w) >= target) break;
-        run += w;
-      }
-      if (b < 0) {       // rounding: everything is kept, the lowest value is the cut
-        b = lowest;
-        run -= sh.h.bins[b];
-      }
-      sh.at = b;
-      sh.redu[0] = run;
+    double before;
+    int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal - (double)ahead, sh, &before);
+    if (b == kBins) {       // rounding: everything stays, the lowest value is the cut
+      if (threadIdx.x == 0) sh.at = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < kBins; i += THREADS) if (sh.h.bins[i] != 0ull) atomicMax(&sh.at, i);
+      __syncthreads();
+      b = sh.at;
     }
-    __syncthreads();
-    prefix |= (uint32_t)sh.at << shift;
-    sum_above = sh.redu[0];
+    // the amount ahead of that range, as an integer
+    unsigned long long mine = 0ull;
+    for (int i = threadIdx.x; i < b; i += THREADS) mine += sh.h.bins[i];
+    ahead += block_sum_u64(mine, sh.redu, THREADS / 64);
+    const uint32_t top = hi - ((uint32_t)b << shift);
+    const uint32_t span = (1u << shift) - 1u;
+    lo = top - lo > span ? top - span : lo;
+    hi = top;
   }
   __syncthreads();
-  *above = sum_above;
-  return prefix;
+  *above = ahead;
+  return lo;
 }
 
-// Column of the c-th (1-based) element equal to x in index order; INT_MAX when there are no more than c.
+// Column of the c-th (1-based) element equal to x0 in index order; INT_MAX when there are no more than c.
 template <typename T, int THREADS>
 __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x0, double c, SampleShared<THREADS>& sh) {
-  auto equal = [&](float x, int col) { return x == x0 && col >= 0 && col < rv.v ? 1.0 : 0.0; };
-  segment_sums<T, THREADS, 1>(rv, nseg, equal, sh);
+  constexpr int EPV = Elem<T>::kVec;
+  auto equal = [&](const float* x, int col0, double* w) {
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) w[e] = x[e] == x0 && col0 + e >= 0 && col0 + e < rv.v ? 1.0 : 0.0;
+  };
+  segment_sums<T, THREADS, 2>(rv, nseg, equal, sh);
   double mine = 0.0;
   for (int i = threadIdx.x; i < nseg; i += THREADS) mine += sh.seg[i];
   const double all = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
@@ -350,10 +409,31 @@ __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x
   return pick<T, THREADS>(rv, nseg, c - 0.5, equal, sh, &w);
 }
 
+// sh.h.step[0 .. n) in descending order (n <= kStep), by the workgroup
+template <int THREADS>
+__device__ __forceinline__ void sort_step(SampleShared<THREADS>& sh, int n) {
+  int N = 2;
+  while (N < n) N *= 2;
+  for (int i = n + threadIdx.x; i < N; i += THREADS) sh.h.step[i] = 0ull;
+  __syncthreads();
+  for (int k = 2; k <= N; k *= 2) {
+    for (int j = k / 2; j > 0; j /= 2) {
+      for (int p = threadIdx.x; p < N / 2; p += THREADS) {
+        const int i = 2 * p - (p & (j - 1)), o = i + j;
+        const unsigned long long a = sh.h.step[i], b = sh.h.step[o];
+        const bool up = (i & k) != 0;            // ascending half
+        if ((a < b) != up) { sh.h.step[i] = b; sh.h.step[o] = a; }
+      }
+      __syncthreads();
+    }
+  }
+}
+
 template <typename T, int THREADS, int UN>
 __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ logits, SampleArgs a) {
   constexpr int EPV = Elem<T>::kVec;
   constexpr int NW = THREADS / 64;
+  constexpr int kList = SampleShared<THREADS>::kList;
   __shared__ SampleShared<THREADS> sh;
   const int64_t row = blockIdx.x;
   const RowView<T> rv(logits + row * (int64_t)a.v, a.v);
@@ -375,7 +455,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
 
   // 1: the maximum; NaN propagates
   float mx = -INFINITY;
-  each([&](const u32x4& r, int) {
+  each_vector<T, THREADS, 4>(rv, [&](const u32x4& r, int) {
     float x[EPV];
     Elem<T>::unpack(r, x);
 #pragma unroll
@@ -384,21 +464,26 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   float wm = mx;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) wm = __builtin_elementwise_maximum(wm, __shfl_xor(wm, o, 64));
-  // least of the threads' maxima, of those that have one: as many elements are not below it
-  const bool some = mx > -INFINITY;
-  const float wl = -group_reduce<64, OpMax>(some ? -mx : -INFINITY);
-  const int wn = __builtin_popcountll(__ballot(some));
-  if ((tid & 63) == 0) { sh.redf[0][tid >> 6] = wm; sh.redf[1][tid >> 6] = wl; sh.redi[tid >> 6] = wn; }
-  if (tid == 0) sh.count = 0;
+  // A value that at least k elements are not below: in each wave the ceil(k / waves)-th largest of the
+  // threads' maxima, found bit by bit with ballots, and the least of those over the waves.
+  uint32_t vouch = 0u;
+  if (use_k) {
+    const uint32_t key = key_of(mx);
+    const int q = (k + NW - 1) / NW;
+    for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1)
+      if (__builtin_popcountll(__ballot(key >= (vouch | bit))) >= q) vouch |= bit;
+  }
+  if ((tid & 63) == 0) { sh.redf[0][tid >> 6] = wm; sh.redi[tid >> 6] = (int)vouch; }
+  if (tid == 0) { sh.count = 0; sh.at = 0; }
   __syncthreads();
-  float m = sh.redf[0][0], least = sh.redf[1][0];
-  int vouched = sh.redi[0];
+  float m = sh.redf[0][0];
+  vouch = (uint32_t)sh.redi[0];
 #pragma unroll
   for (int i = 1; i < NW; ++i) {
     m = __builtin_elementwise_maximum(m, sh.redf[0][i]);
-    least = fminf(least, sh.redf[1][i]);
-    vouched += sh.redi[i];
+    vouch = (uint32_t)sh.redi[i] < vouch ? (uint32_t)sh.redi[i] : vouch;
   }
+  const float vouched_x = vouch <= 0x007FFFFFu ? -INFINITY : float_of_key(vouch);      // that is key_of(-inf)
   // (NaN compares false everywhere)
   if (!(m < INFINITY && m > -INFINITY) || !(T_ >= 0.f && T_ < INFINITY)) {
     if (tid == 0) {
@@ -427,17 +512,16 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     }
     return;
   }
-  const Weight weight{(double)m, 1.4426950408889634074 / (double)T_};
-
-  // 2: the cut
-  Cut cut{-INFINITY, 0x7fffffff};
-  if (use_k || use_p) {
-    // Steps of equal width below the maximum. For top-k over the range that the threads' maxima
-    // vouch for (when there are k of them), else over 24 T: what lies below weighs less than 4e-11.
-    float range = m - least;
-    if (!(use_k && k <= vouched) || !(range < INFINITY)) range = 24.f * T_;
-    float per = (float)(kBins - 2) / range;
-    if (!(per <= 1e30f)) per = 1e30f;
+  const Weight weight(m, T_);
+  Cut cut{-INFINITY, -1};           // -inf itself is never kept
+  float x_min = -INFINITY;          // min-p: the least value with a weight of min_p
+  if (use_m) {
+    const double xm = (double)m + (double)T_ * log((double)min_p);
+    x_min = (float)xm;                      // may be -inf: then everything stays
+    if ((double)x_min < xm) x_min = float_of_key(key_of(x_min) + 1u);      // the next float up
+    if (x_min > m) x_min = m;
+  }
+  if (use_k || use_p || use_m) {
     // 2^fx units of mass per 1: the sum of v weights of at most 1 stays below 2^62
     const int vbits = 62 - (32 - __builtin_clz((unsigned)a.v));
     const int fx = vbits < 50 ? vbits : 50;
@@ -446,111 +530,180 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     auto fixed = [&](double w) {
       return __builtin_bit_cast(unsigned long long, __builtin_fma(w, unit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
     };
-    for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
-    __syncthreads();
+    auto value = [](unsigned long long e) { return float_of_key((uint32_t)(e >> 32)); };
+    auto column = [](unsigned long long e) { return (int)~(uint32_t)e; };
+
+    // 2: the bound of the candidates, and where top-p alone has its cut
+    float bound = x_min;
+    if (use_k) bound = vouched_x;
+    // Steps of equal width from the maximum down to the bound, over 24 T where top-p is alone: what lies
+    // below weighs less than 4e-11.
+    float range = use_k ? m - bound : 24.f * T_;
+    if (!(range < INFINITY)) range = 24.f * T_;
+    float per = (float)(kBins - 2) / range;
+    if (!(per <= 1e30f)) per = 1e30f;
+    auto step_of = [&](float x) { return (m - x) * per; };       // grows as x falls; never NaN
     const float last_bin = (float)(kBins - 1);
-    double total = 0.0, target;
-    if (use_k) {
-      each([&](const u32x4& r, int c) {
-        float x[EPV];
-        Elem<T>::unpack(r, x);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) {
-          const float y = (m - x[e]) * per;
-          if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], 1ull);
-        }
-      });
-      target = (double)k;
-    } else {
-      each([&](const u32x4& r, int c) {
-        float x[EPV];
-        Elem<T>::unpack(r, x);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) {
-          const double w = weight(x[e]);
-          total += w;
-          const float y = (m - x[e]) * per;
-          if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], fixed(w));
-        }
-      });
-      total = block_reduce64<THREADS / 64, Sum64>(total, sh.red);
-      target = (double)p * total * unit;
-    }
-    __syncthreads();
-    double ahead;
-    const int bin = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, target, sh, &ahead);
-    bool listed = bin < kBins;
-    if (listed) {
-      // candidates: the step of the cut, and for top-k (whose order the nucleus may need) all above it
-      const float lo = use_k ? 0.f : (float)bin, hi = (float)(bin + 1);
-      each([&](const u32x4& r, int c) {
-        float x[EPV];
-        Elem<T>::unpack(r, x);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) {
-          const float y = (m - x[e]) * per;
-          if (y >= lo && y < hi) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kList) sh.h.list[at] = ((unsigned long long)key_of(x[e]) << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
-          }
-        }
-      });
+    double total = 0.0, ahead = 0.0, goal = 0.0;
+    int bin = kBins;
+    const bool from_row = use_p && !use_k;
+    if (from_row) {
+      for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
       __syncthreads();
-      const int n = sh.count;
-      listed = n <= kList;
-      if (listed) {
-        // order the candidates by counting those that come before each
-        for (int i = tid; i < n; i += THREADS) {
-          const unsigned long long me = sh.h.list[i];
-          int rank = 0;
-          for (int j = 0; j < n; ++j) rank += sh.h.list[j] > me ? 1 : 0;
-          sh.h.sorted[rank] = me;
+      each([&](const u32x4& r, int) {
+        float x[EPV];
+        Elem<T>::unpack(r, x);
+        double w[EPV];
+        weight.template eval<EPV>(x, w);
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) {
+          total += w[e];
+          const float y = step_of(x[e]);
+          if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], fixed(w[e]));
         }
-        __syncthreads();
-        auto value = [&](int i) { return float_of_key((uint32_t)(sh.h.sorted[i] >> 32)); };
-        int kept = use_k ? k : n;
-        if (use_p) {
-          double goal, base = 0.0;
-          if (use_k) {
-            double mine = 0.0;
-            for (int i = tid; i < k; i += THREADS) mine += weight(value(i));
-            goal = (double)p * block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
-          } else {
-            goal = (double)p * total;
-            base = ahead / unit;
-          }
-          // the first rank at which the mass reaches the goal is the last one kept
-          double unused;
-          const int r = find_running<THREADS, false>([&](int i) { return weight(value(i)); }, kept, goal - base,
-                                                     sh, &unused);
-          kept = r < kept ? r + 1 : kept;
-        }
-        cut.x = value(kept - 1);
-        cut.col = (int)~(uint32_t)sh.h.sorted[kept - 1];
-        __syncthreads();
-      }
+      });
+      total = block_reduce64<NW, Sum64>(total, sh.red);
+      goal = (double)p * total * unit;
+      __syncthreads();
+      bin = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal, sh, &ahead);
     }
-    if (!listed) {
+    if (tid == 0) { sh.at = 0; sh.klo = 0xFFFFFFFFu; sh.khi = 0u; }
+    __syncthreads();
+    const float lo = (float)bin, hi = (float)(bin + 1);
+    const bool found = !from_row || bin < kBins;
+    int nb = 0;
+    bool listed = false;
+    if (found) {
+      bool full = false;
+      uint32_t klo = 0xFFFFFFFFu, khi = 0u;      // keys of the step
+      each([&](const u32x4& r, int c) {
+        float x[EPV];
+        Elem<T>::unpack(r, x);
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+        if (__ballot(from_row ? step_of(top) < hi : top >= bound) == 0ull) return;
+        if (full && !from_row) return;
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) {
+          const float y = step_of(x[e]);
+          const bool cand = from_row ? y < hi : (x[e] >= bound && x[e] > -INFINITY);
+          const unsigned long long who = __ballot(cand);
+          if (who == 0ull) continue;
+          const uint32_t key = key_of(x[e]);
+          const unsigned long long entry = ((unsigned long long)key << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
+          if (!full) {
+            const int n = __builtin_popcountll(who);
+            int base = 0;
+            const int first = __builtin_ctzll(who);
+            if ((tid & 63) == first) base = atomicAdd(&sh.count, n);
+            base = __builtin_amdgcn_readlane(base, first);
+            const int at = base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+            if (cand && at < kList) sh.h.list[at] = entry;
+            full = base + n > kList;
+          }
+          if (from_row && cand && y >= lo) {
+            klo = key < klo ? key : klo;
+            khi = key > khi ? key : khi;
+            if (sh.at <= kStep) {       // counted past the end once: the step is too long
+              const int at = atomicAdd(&sh.at, 1);
+              if (at < kStep) sh.h.step[at] = entry;
+            }
+          }
+        }
+      });
+      if (from_row && klo <= khi) { atomicMin(&sh.klo, klo); atomicMax(&sh.khi, khi); }
+      __syncthreads();
+      nb = sh.at;
+      listed = sh.count <= kList;
+    }
+    const int n = sh.count < kList ? sh.count : kList;
+
+    // 3: the exact cut. `settle` takes the n_step elements in sh.h.step, the step that holds the cut with
+    // `before` ahead of it: the last element that stays is the first whose running amount reaches the goal.
+    auto settle = [&](int n_step, double before, double goal_, bool count) {
+      sort_step<THREADS>(sh, n_step);
+      auto amount = [&](int i) { return count ? 1.0 : (double)fixed(weight(value(sh.h.step[i]))); };
+      double unused;
+      int r = find_running<THREADS, false>(amount, n_step, goal_ - before, sh, &unused);
+      if (r >= n_step) r = n_step - 1;
+      cut.x = value(sh.h.step[r]);
+      cut.col = column(sh.h.step[r]);
+      __syncthreads();
+    };
+    auto kept = [&](unsigned long long e) {
+      const float x = value(e);
+      return x > cut.x || (x == cut.x && column(e) <= cut.col);
+    };
+    // the same from the list, for the elements of it that are still kept; false when the step is too long
+    auto settle_list = [&](double goal_or_p, bool count) {
+      for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
+      if (tid == 0) sh.at = 0;
+      __syncthreads();
+      unsigned long long mine = 0ull;
+#pragma unroll 1
+      for (int i = tid; i < n; i += THREADS) {
+        const unsigned long long e = sh.h.list[i];
+        if (!kept(e)) continue;
+        const unsigned long long w = count ? 1ull : fixed(weight(value(e)));
+        const float y = step_of(value(e));
+        atomicAdd(&sh.h.bins[y < last_bin ? (int)y : kBins - 1], w);
+        mine += w;
+      }
+      const double mass = (double)block_sum_u64(mine, sh.redu, NW);      // its barriers publish the histogram
+      const double goal_ = count ? goal_or_p : goal_or_p * mass;
+      double before;
+      int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal_, sh, &before);
+      if (b == kBins) return true;         // everything stays
+      if (tid == 0) sh.at = 0;
+      __syncthreads();
+#pragma unroll 1
+      for (int i = tid; i < n; i += THREADS) {
+        const unsigned long long e = sh.h.list[i];
+        const float y = step_of(value(e));
+        if (kept(e) && (y < last_bin ? (int)y : kBins - 1) == b) {
+          const int at = atomicAdd(&sh.at, 1);
+          if (at < kStep) sh.h.step[at] = e;
+        }
+      }
+      __syncthreads();
+      const int n_step = sh.at;
+      if (n_step > kStep) return false;
+      settle(n_step, before, goal_, count);
+      return true;
+    };
+    bool settled = !use_k && !use_p;
+    if (use_k && listed && (n >= k || bound == -INFINITY)) {      // (fewer than k: all that are not -inf)
+      settled = n < k || settle_list((double)k, true);
+      if (settled && use_p) settled = settle_list((double)p, false);
+    } else if (from_row && found && nb <= kStep) {
+      settle(nb, ahead, goal, false);
+      settled = true;
+    }
+    if (!settled) {
       double ties = 0.0;
       unsigned long long above;
+      cut = Cut{-INFINITY, -1};
       if (use_k) {
-        const uint32_t key = radix_cut<T, THREADS>(rv, (double)k, [](float) { return 1ull; }, sh, &above);
+        const uint32_t key = key_search<T, THREADS>(rv, 0u, 0xFFFFFFFEu, 0ull, (double)k, [](float) { return 1ull; }, sh, &above);
         cut.x = float_of_key(key);
         ties = (double)k - (double)above;
         if (use_p) {      // the mass of those k
           double mine = 0.0;
           each_element<T, THREADS>(rv, [&](float x, int) { if (x > cut.x) mine += weight(x); });
-          total = block_reduce64<THREADS / 64, Sum64>(mine, sh.red) + ties * weight(cut.x);
+          total = block_reduce64<NW, Sum64>(mine, sh.red) + ties * weight(cut.x);
         }
       }
       if (use_p) {
-        const double goal = (double)p * total * unit;
-        const uint32_t key = radix_cut<T, THREADS>(
-            rv, goal, [&](float x) { return fixed(weight(x)); }, sh, &above);
+        const double goal_p = (double)p * total * unit;
+        const bool in_step = from_row && found;
+        const uint32_t key = key_search<T, THREADS>(rv, in_step ? sh.klo : 0u, in_step ? sh.khi : 0xFFFFFFFEu,
+                                                    in_step ? (unsigned long long)ahead : 0ull, goal_p,
+                                                    [&](float x) { return fixed(weight(x)); }, sh, &above);
         const float xp = float_of_key(key);
         const double each_w = (double)fixed(weight(xp));
         // equal values that the mass still needs: the r-th stays iff above + r * weight < goal
-        double need = each_w > 0.0 ? ceil((goal - (double)above) / each_w) : 1.0;
+        double need = each_w > 0.0 ? ceil((goal_p - (double)above) / each_w) : 1.0;
         if (!(need >= 1.0)) need = 1.0;
         if (!use_k || xp > cut.x) {
           cut.x = xp;
@@ -560,32 +713,89 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         }
       }
       cut.col = nth_equal<T, THREADS>(rv, nseg, cut.x, ties, sh);
+      listed = false;          // the searches took the list's place
     }
-  }
-  if (use_m) {               // the least value with a weight of min_p; every equal one stays
-    const double xm = (double)m + (double)T_ * log((double)min_p);
-    float xf = (float)xm;                      // may be -inf: then everything stays
-    if ((double)xf < xm) xf = float_of_key(key_of(xf) + 1u);      // the next float up
-    if (xf > m) xf = m;
-    if (xf > cut.x) {
-      cut.x = xf;
+    if (x_min > cut.x) {       // every value equal to the bound stays
+      cut.x = x_min;
       cut.col = 0x7fffffff;
+    }
+
+    // 4 on the list
+    if (listed) {
+      constexpr int PER = (kList + THREADS - 1) / THREADS;
+      int shift = 6;
+      while ((rv.nvec >> shift) >= kBins) ++shift;
+      const uint32_t seg_bits = (EPV == 8 ? 3 : 2) + shift;             // a segment has at most kStep elements
+      __syncthreads();
+      for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
+      __syncthreads();
+      unsigned long long me[PER], w[PER], mine = 0ull;
+      int seg[PER];
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int i = j * THREADS + tid;
+        seg[j] = -1;
+        if (j * THREADS >= n) continue;
+        if (i >= n) continue;
+        me[j] = sh.h.list[i];
+        if (!kept(me[j])) continue;
+        w[j] = fixed(weight(value(me[j])));
+        seg[j] = (int)(((uint32_t)column(me[j]) + (uint32_t)rv.lead) >> seg_bits);
+        atomicAdd(&sh.h.bins[seg[j]], w[j]);
+        mine += w[j];
+      }
+      const double mass = (double)block_sum_u64(mine, sh.redu, NW);
+      const double target = u * mass;
+      const int s = find_running<THREADS, true>([&](int i) { return (double)sh.h.bins[i]; }, kBins, target, sh, &ahead);
+      if (tid == 0) { sh.at = 0; sh.col = -1; }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (seg[j] == s) {
+          const int at = atomicAdd(&sh.at, 1);
+          sh.h.step[at] = me[j];
+          sh.h.mass[at] = w[j];
+        }
+      }
+      __syncthreads();
+      const int ns = sh.at;
+      for (int i = tid; i < ns; i += THREADS) {
+        const int col = column(sh.h.step[i]);
+        unsigned long long before = 0ull;
+        for (int o = 0; o < ns; ++o) before += column(sh.h.step[o]) < col ? sh.h.mass[o] : 0ull;
+        if (ahead + (double)before <= target && target < ahead + (double)(before + sh.h.mass[i])) {
+          sh.col = col;
+          sh.x = value(sh.h.step[i]);
+        }
+      }
+      __syncthreads();
+      if (sh.col >= 0) {
+        if (tid == 0) {
+          a.token[row] = sh.col;
+          if (a.logprob != nullptr) a.logprob[row] = (float)log(weight(sh.x) * unit / mass);
+        }
+        return;
+      }
+      // rounding put the target between two segments: the sweep below decides
     }
   }
 
-  // 3: kept mass by segment, in index order
-  auto kept_weight = [&](float x, int col) {
-    return x > cut.x || (x == cut.x && col <= cut.col) ? weight(x) : 0.0;
+  // 4 over the row: kept mass by segment, in index order
+  auto kept_weights = [&](const float* x, int col0, double* w) {
+    weight.template eval<EPV>(x, w);
+#pragma unroll
+    for (int e = 0; e < EPV; ++e)
+      w[e] = x[e] > cut.x || (x[e] == cut.x && col0 + e <= cut.col) ? w[e] : 0.0;
   };
-  segment_sums<T, THREADS, UN>(rv, nseg, kept_weight, sh);
+  segment_sums<T, THREADS, UN>(rv, nseg, kept_weights, sh);
   double mine = 0.0;
   for (int i = tid; i < nseg; i += THREADS) mine += sh.seg[i];
-  const double kept = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
+  const double mass = block_reduce64<NW, Sum64>(mine, sh.red);
   double w;
-  const int col = pick<T, THREADS>(rv, nseg, u * kept, kept_weight, sh, &w);
+  const int col = pick<T, THREADS>(rv, nseg, u * mass, kept_weights, sh, &w);
   if (tid == 0) {
     a.token[row] = col;
-    if (a.logprob != nullptr) a.logprob[row] = (float)log(w / kept);
+    if (a.logprob != nullptr) a.logprob[row] = (float)log(w / mass);
   }
 }
 
@@ -593,8 +803,8 @@ template <typename T>
 void launch(const void* logits, const SampleArgs& a, int64_t n, hipStream_t st) {
   const int64_t nvec = a.v / Elem<T>::kVec + 2;
 #define GO(TH, UN) FM_LAUNCH((sample_kernel<T, TH, UN>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
-  if (nvec <= 1024) GO(256, 4);
-  else GO(1024, 4);
+  if (nvec <= 1024) GO(256, 2);
+  else GO(1024, 2);
 #undef GO
 }
 
