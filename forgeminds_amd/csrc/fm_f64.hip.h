@@ -3,6 +3,8 @@
 // hangs on is simply computed in 64 bits.
 #pragma once
 
+#include <type_traits>
+
 #include "fm_vocab.hip.h"
 
 namespace fm {
@@ -38,6 +40,45 @@ __device__ __forceinline__ double group_reduce64(double v) {
   return v;
 }
 __device__ __forceinline__ double wave_sum64(double v) { return group_reduce64<64, Sum64>(v); }
+
+// inclusive prefix sum over the wave in lane order: four shifts inside the rows of sixteen lanes, then
+// the rows' totals
+__device__ __forceinline__ double wave_incl64(double v) {
+  const int lane = lane_id(), in_row = lane & 15;
+  double t = dpp64<0x111>(v);            // row_shr:1
+  v += in_row >= 1 ? t : 0.0;
+  t = dpp64<0x112>(v);
+  v += in_row >= 2 ? t : 0.0;
+  t = dpp64<0x114>(v);
+  v += in_row >= 4 ? t : 0.0;
+  t = dpp64<0x118>(v);
+  v += in_row >= 8 ? t : 0.0;
+  const double a = readlane64(v, 15), b = readlane64(v, 31), c = readlane64(v, 47);
+  v += lane >= 48 ? (a + b) + c : (lane >= 32 ? a + b : (lane >= 16 ? a : 0.0));
+  return v;
+}
+// integer sum over the workgroup
+template <int NW>
+__device__ __forceinline__ unsigned long long block_sum_int64(unsigned long long v, unsigned long long* smem) {
+  auto add = [](unsigned long long x, unsigned long long y) { return x + y; };
+  auto dpp = [](unsigned long long x, auto ctrl) {
+    return __builtin_bit_cast(unsigned long long, dpp64<decltype(ctrl)::value>(__builtin_bit_cast(double, x)));
+  };
+  v = add(v, dpp(v, std::integral_constant<int, kDppXor1>{}));
+  v = add(v, dpp(v, std::integral_constant<int, kDppXor2>{}));
+  v = add(v, dpp(v, std::integral_constant<int, kDppHalfMirror>{}));
+  v = add(v, dpp(v, std::integral_constant<int, kDppMirror>{}));
+  unsigned long long s = 0ull;
+#pragma unroll
+  for (int r = 0; r < 64; r += 16) s += __builtin_bit_cast(unsigned long long, readlane64(__builtin_bit_cast(double, v), r));
+  if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = 0ull;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) s += smem[i];
+  __syncthreads();
+  return s;
+}
 
 // across the NW waves of a workgroup; the waves' results are combined by lanes rather than by every
 // thread reading all of them (32 registers beside a held row)

@@ -49,16 +49,6 @@ struct SampleArgs {
   int v;
 };
 
-__device__ __forceinline__ double wave_incl64(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double t = __shfl_up(v, o, 64);
-    if (lane >= o) v += t;
-  }
-  return v;
-}
-
 // A row as whole 16-byte vectors from the last 16-byte border at or before its first element; what
 // the first and the last vector hold outside the row reads as -inf (weight zero, never kept) and is
 // not loaded.
@@ -126,6 +116,9 @@ struct SampleShared {
   int at;
   int col;
   uint32_t klo, khi;
+  unsigned long long hits[4];
+  double hitw[4], lastw[4];
+  int lasts[4];
   float x;
   double weight;
 };
@@ -183,34 +176,42 @@ struct Weight {
 template <int THREADS, bool STRICT, typename F>
 __device__ __forceinline__ int find_running(F entry, int n, double target, SampleShared<THREADS>& sh, double* before) {
   constexpr int NW = THREADS / 64;
-  const int tid = threadIdx.x, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (n + THREADS - 1) / THREADS;
+  auto there = [&](double run) { return STRICT ? run > target : run >= target; };
   double mine = 0.0;
   for (int i = 0; i < per; ++i) {
     const int at = tid * per + i;
     if (at < n) mine += entry(at);
   }
   const double incl = wave_incl64(mine);
-  if ((tid & 63) == 63) sh.red[wave] = incl;
+  if (lane == 63) sh.red[wave] = incl;
   if (tid == 0) { sh.at = n; sh.weight = 0.0; }
   __syncthreads();
   double ahead = 0.0;
 #pragma unroll
   for (int i = 0; i < NW; ++i) if (i < wave) ahead += sh.red[i];
-  double run = ahead + (incl - mine);
-  int hit = n;
-  double hit_before = 0.0;
-  for (int i = 0; i < per; ++i) {
-    const int at = tid * per + i;
-    if (at >= n) break;
-    const double next = run + entry(at);
-    if (STRICT ? next > target : next >= target) { hit = at; hit_before = run; break; }
-    run = next;
+  // the sum ahead of a lane is the very number that the lane before it compares
+  const double mine_end = ahead + incl;
+  double mine_start = __shfl_up(mine_end, 1, 64);
+  if (lane == 0) mine_start = ahead;
+  int at = n;
+  double run = mine_start;
+  if (there(mine_end) && (tid == 0 || !there(mine_start))) {
+    at = tid * per;
+    for (int i = 0; i < per; ++i) {
+      const double end = i == per - 1 ? mine_end : run + entry(at);
+      if (i == per - 1 || there(end)) break;
+      run = end;
+      ++at;
+    }
+    at = at < n ? at : n - 1;
+    // (rounding may let the sums of neighbouring lanes dip: the first one counts)
+    atomicMin(&sh.at, at);
   }
-  if (hit < n) atomicMin(&sh.at, hit);
   __syncthreads();
   const int found = sh.at;
-  if (hit < n && hit == found) sh.weight = hit_before;
+  if (at < n && at == found) sh.weight = run;
   __syncthreads();
   *before = sh.weight;
   __syncthreads();
@@ -249,13 +250,36 @@ __device__ __forceinline__ void each_element(const RowView<T>& rv, F fn) {
   });
 }
 
+// A segment is G blocks of 64 vectors that one wave sweeps, a vector a lane: one reduction over the wave
+// for G vectors a lane.
+constexpr int seg_vecs(int G) { return 64 * G; }
+
+// The weights of this lane's vector of block `block` of the row (0 past its end) and their sum.
+template <typename T, typename F>
+__device__ __forceinline__ double block_weights(const RowView<T>& rv, int block, F weights_of, double* w) {
+  constexpr int EPV = Elem<T>::kVec;
+  const int c = block * 64 + (threadIdx.x & 63);
+  double mine = 0.0;
+#pragma unroll
+  for (int e = 0; e < EPV; ++e) w[e] = 0.0;
+  if (c < rv.nvec) {
+    float x[EPV];
+    Elem<T>::unpack(rv.load(c), x);
+    weights_of(x, rv.col0(c), w);
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) mine += w[e];
+  }
+  return mine;
+}
+
 // The token among the segments whose weights are in sh.seg (nseg of them): the first column whose
-// running weight exceeds `target`. weights_of(x, col0, w) gives the weights of a vector. Rounding may leave the
-// target at the very end: then the last column with a weight. Returns the column; *w its weight.
-template <typename T, int THREADS, typename F>
+// running weight exceeds `target`. weights_of(x, col0, w) gives the weights of a vector. Rounding may leave
+// the target at the very end: then the last column with a weight. Returns the column; *w its weight.
+template <typename T, int THREADS, int G, typename F>
 __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double target, F weights_of,
                                     SampleShared<THREADS>& sh, double* w) {
   constexpr int EPV = Elem<T>::kVec;
+  static_assert(G <= THREADS / 64, "a wave per block of the segment");
   double before;
   int s = find_running<THREADS, true>([&](int i) { return sh.seg[i]; }, nseg, target, sh, &before);
   const bool end = s == nseg;
@@ -265,64 +289,74 @@ __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double targe
     for (int i = threadIdx.x; i < nseg; i += THREADS) if (sh.seg[i] > 0.0) atomicMax(&sh.at, i);
     __syncthreads();
     s = sh.at;
+    __syncthreads();
   }
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    const int c = s * 64 + lane;
-    float x[EPV];
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) x[e] = -INFINITY;
-    if (c < rv.nvec) Elem<T>::unpack(rv.load(c), x);
-    double wt[EPV];
-    double mine = 0.0;
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) wt[e] = 0.0;
-    if (c < rv.nvec) weights_of(x, rv.col0(c), wt);
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) mine += wt[e];
-    const double incl = wave_incl64(mine);
+  // its blocks, a wave each
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double wt[EPV], mine = 0.0, incl = 0.0;
+  if (wave < G) {
+    mine = block_weights<T>(rv, s * G + wave, weights_of, wt);
+    incl = wave_incl64(mine);
+    if (lane == 63) sh.red[wave] = incl;
+  }
+  if (threadIdx.x == 0) sh.col = -1;
+  __syncthreads();
+  for (int g = 0; g < G; ++g) if (g < wave) before += sh.red[g];
+  int last = -1;
+  double last_w = 0.0;
+  if (wave < G) {
     double run = before + (incl - mine);
-    int hit = -1, last = -1;
-    double hit_w = 0.0, last_w = 0.0;
+    int hit = -1;
+    double hit_w = 0.0;
+    const int col0 = rv.col0((s * G + wave) * 64 + lane);
 #pragma unroll
     for (int e = 0; e < EPV; ++e) {
       run += wt[e];
-      if (wt[e] > 0.0) { last = rv.col0(c) + e; last_w = wt[e]; }
-      if (hit < 0 && wt[e] > 0.0 && run > target) { hit = rv.col0(c) + e; hit_w = wt[e]; }
+      if (wt[e] > 0.0) {
+        last = col0 + e;
+        last_w = wt[e];
+        if (!end && hit < 0 && run > target) { hit = col0 + e; hit_w = wt[e]; }
+      }
     }
-    const unsigned long long any = __ballot(!end && hit >= 0), some = __ballot(last >= 0);
-    int from = 0;
-    if (any != 0ull) from = __builtin_ctzll(any);
-    else if (some != 0ull) from = 63 - __builtin_clzll(some);
-    const int col = any != 0ull ? __shfl(hit, from, 64) : __shfl(last, from, 64);
-    const double cw = any != 0ull ? __shfl(hit_w, from, 64) : __shfl(last_w, from, 64);
-    if (lane == 0) { sh.col = col; sh.weight = cw; }
+    const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
+    // the first hit of the wave; the waves' ones by column, the first one again
+    if (any != 0ull && lane == __builtin_ctzll(any)) sh.hits[wave] = (unsigned long long)(uint32_t)hit;
+    else if (any == 0ull && lane == 0) sh.hits[wave] = ~0ull;
+    const int top = some != 0ull ? 63 - __builtin_clzll(some) : 0;
+    last = __shfl(last, top, 64);
+    last_w = __shfl(last_w, top, 64);
+    if (any != 0ull && lane == __builtin_ctzll(any)) sh.hitw[wave] = hit_w;
+    if (lane == 0) { sh.lasts[wave] = last; sh.lastw[wave] = last_w; }
   }
   __syncthreads();
-  const int col = sh.col;
-  *w = sh.weight;
+  int col = -1;
+  double cw = 0.0;
+  for (int g = G - 1; g >= 0; --g) if (sh.hits[g] != ~0ull) { col = (int)(uint32_t)sh.hits[g]; cw = sh.hitw[g]; }
+  if (col < 0)
+    for (int g = 0; g < G; ++g) if (sh.lasts[g] >= 0) { col = sh.lasts[g]; cw = sh.lastw[g]; }
   __syncthreads();
+  *w = cw;
   return col;
 }
 
-// Segment sums (64 vectors, a wave each) of weights_of(x, col0, w) over the row into sh.seg.
-template <typename T, int THREADS, int UN, typename F>
+// Segment sums of weights_of(x, col0, w) over the row into sh.seg.
+template <typename T, int THREADS, int G, typename F>
 __device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F weights_of, SampleShared<THREADS>& sh) {
   constexpr int EPV = Elem<T>::kVec;
   __syncthreads();
   const bool any = rv.w0 < rv.w1;
-  for (int c0 = threadIdx.x; (c0 >> 6) < nseg; c0 += THREADS * UN) {
-    u32x4 raw[UN];
+  for (int s = threadIdx.x >> 6; s < nseg; s += THREADS / 64) {
+    const int c0 = s * seg_vecs(G) + (threadIdx.x & 63);
+    u32x4 raw[G];
     if (any) {
 #pragma unroll
-      for (int i = 0; i < UN; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * THREADS));
+      for (int i = 0; i < G; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * 64));
     }
+    double mine = 0.0;
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int c = c0 + i * THREADS;
-      if ((c >> 6) >= nseg) break;
+    for (int i = 0; i < G; ++i) {
+      const int c = c0 + i * 64;
       if (any) touch_whole(raw[i]);
-      double mine = 0.0;
       if (c < rv.nvec) {
         if (!rv.whole(c)) raw[i] = rv.partial(c);
         float x[EPV];
@@ -332,9 +366,9 @@ __device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F w
 #pragma unroll
         for (int e = 0; e < EPV; ++e) mine += w[e];
       }
-      mine = wave_sum64(mine);
-      if ((threadIdx.x & 63) == 0) sh.seg[c >> 6] = mine;
     }
+    mine = wave_sum64(mine);
+    if ((threadIdx.x & 63) == 0) sh.seg[s] = mine;
   }
   __syncthreads();
 }
@@ -381,7 +415,7 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
     // the amount ahead of that range, as an integer
     unsigned long long mine = 0ull;
     for (int i = threadIdx.x; i < b; i += THREADS) mine += sh.h.bins[i];
-    ahead += block_sum_u64(mine, sh.redu, THREADS / 64);
+    ahead += block_sum_int64<THREADS / 64>(mine, sh.redu);
     const uint32_t top = hi - ((uint32_t)b << shift);
     const uint32_t span = (1u << shift) - 1u;
     lo = top - lo > span ? top - span : lo;
@@ -393,20 +427,20 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
 }
 
 // Column of the c-th (1-based) element equal to x0 in index order; INT_MAX when there are no more than c.
-template <typename T, int THREADS>
+template <typename T, int THREADS, int G>
 __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x0, double c, SampleShared<THREADS>& sh) {
   constexpr int EPV = Elem<T>::kVec;
   auto equal = [&](const float* x, int col0, double* w) {
 #pragma unroll
     for (int e = 0; e < EPV; ++e) w[e] = x[e] == x0 && col0 + e >= 0 && col0 + e < rv.v ? 1.0 : 0.0;
   };
-  segment_sums<T, THREADS, 2>(rv, nseg, equal, sh);
+  segment_sums<T, THREADS, G>(rv, nseg, equal, sh);
   double mine = 0.0;
   for (int i = threadIdx.x; i < nseg; i += THREADS) mine += sh.seg[i];
   const double all = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
   if (c >= all) return 0x7fffffff;
   double w;
-  return pick<T, THREADS>(rv, nseg, c - 0.5, equal, sh, &w);
+  return pick<T, THREADS, G>(rv, nseg, c - 0.5, equal, sh, &w);
 }
 
 // sh.h.step[0 .. n) in descending order (n <= kStep), by the workgroup
@@ -429,7 +463,7 @@ __device__ __forceinline__ void sort_step(SampleShared<THREADS>& sh, int n) {
   }
 }
 
-template <typename T, int THREADS, int UN>
+template <typename T, int THREADS, int UN, int G>
 __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ logits, SampleArgs a) {
   constexpr int EPV = Elem<T>::kVec;
   constexpr int NW = THREADS / 64;
@@ -455,7 +489,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
 
   // 1: the maximum; NaN propagates
   float mx = -INFINITY;
-  each_vector<T, THREADS, 4>(rv, [&](const u32x4& r, int) {
+  each_vector<T, THREADS, 8>(rv, [&](const u32x4& r, int) {
     float x[EPV];
     Elem<T>::unpack(r, x);
 #pragma unroll
@@ -492,7 +526,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     }
     return;
   }
-  const int nseg = (rv.nvec + 63) / 64;
+  const int nseg = (rv.nvec + seg_vecs(G) - 1) / seg_vecs(G);
   if (T_ == 0.f) {           // the first maximum
     __syncthreads();         // sh.redi
     int first = 0x7fffffff;
@@ -536,9 +570,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     // 2: the bound of the candidates, and where top-p alone has its cut
     float bound = x_min;
     if (use_k) bound = vouched_x;
-    // Steps of equal width from the maximum down to the bound, over 24 T where top-p is alone: what lies
-    // below weighs less than 4e-11.
-    float range = use_k ? m - bound : 24.f * T_;
+    // Steps of equal width from the maximum down to the bound; over 12 T where top-p is alone (24 T for a
+    // top-p past 0.99). A cut further down than that, where each element weighs less than 6e-6 of the
+    // largest, is left to the search.
+    const float nats = p <= 0.99f ? 12.f : 24.f;
+    float range = use_k ? m - bound : nats * T_;
     if (!(range < INFINITY)) range = 24.f * T_;
     float per = (float)(kBins - 2) / range;
     if (!(per <= 1e30f)) per = 1e30f;
@@ -650,7 +686,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         atomicAdd(&sh.h.bins[y < last_bin ? (int)y : kBins - 1], w);
         mine += w;
       }
-      const double mass = (double)block_sum_u64(mine, sh.redu, NW);      // its barriers publish the histogram
+      const double mass = (double)block_sum_int64<NW>(mine, sh.redu);      // its barriers publish the histogram
       const double goal_ = count ? goal_or_p : goal_or_p * mass;
       double before;
       int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal_, sh, &before);
@@ -712,7 +748,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
           ties = need;
         }
       }
-      cut.col = nth_equal<T, THREADS>(rv, nseg, cut.x, ties, sh);
+      cut.col = nth_equal<T, THREADS, G>(rv, nseg, cut.x, ties, sh);
       listed = false;          // the searches took the list's place
     }
     if (x_min > cut.x) {       // every value equal to the bound stays
@@ -744,7 +780,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         atomicAdd(&sh.h.bins[seg[j]], w[j]);
         mine += w[j];
       }
-      const double mass = (double)block_sum_u64(mine, sh.redu, NW);
+      const double mass = (double)block_sum_int64<NW>(mine, sh.redu);
       const double target = u * mass;
       const int s = find_running<THREADS, true>([&](int i) { return (double)sh.h.bins[i]; }, kBins, target, sh, &ahead);
       if (tid == 0) { sh.at = 0; sh.col = -1; }
@@ -780,19 +816,29 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     }
   }
 
-  // 4 over the row: kept mass by segment, in index order
+  // 4 over the row: kept mass by segment, in index order. Nothing cuts: every weight counts (that of -inf
+  // is 0). A cut: vectors without a kept element cost their comparison only.
+  auto all_weights = [&](const float* x, int, double* w) { weight.template eval<EPV>(x, w); };
   auto kept_weights = [&](const float* x, int col0, double* w) {
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) w[e] = 0.0;
+    if (__ballot(top >= cut.x) == 0ull) return;
     weight.template eval<EPV>(x, w);
 #pragma unroll
     for (int e = 0; e < EPV; ++e)
       w[e] = x[e] > cut.x || (x[e] == cut.x && col0 + e <= cut.col) ? w[e] : 0.0;
   };
-  segment_sums<T, THREADS, UN>(rv, nseg, kept_weights, sh);
+  const bool whole_row = cut.x == -INFINITY;
+  if (whole_row) segment_sums<T, THREADS, G>(rv, nseg, all_weights, sh);
+  else segment_sums<T, THREADS, G>(rv, nseg, kept_weights, sh);
   double mine = 0.0;
   for (int i = tid; i < nseg; i += THREADS) mine += sh.seg[i];
   const double mass = block_reduce64<NW, Sum64>(mine, sh.red);
   double w;
-  const int col = pick<T, THREADS>(rv, nseg, u * mass, kept_weights, sh, &w);
+  const int col = pick<T, THREADS, G>(rv, nseg, u * mass, kept_weights, sh, &w);
   if (tid == 0) {
     a.token[row] = col;
     if (a.logprob != nullptr) a.logprob[row] = (float)log(w / mass);
@@ -802,9 +848,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
 template <typename T>
 void launch(const void* logits, const SampleArgs& a, int64_t n, hipStream_t st) {
   const int64_t nvec = a.v / Elem<T>::kVec + 2;
-#define GO(TH, UN) FM_LAUNCH((sample_kernel<T, TH, UN>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
-  if (nvec <= 1024) GO(256, 2);
-  else GO(1024, 2);
+#define GO(TH, UN, G) FM_LAUNCH((sample_kernel<T, TH, UN, G>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
+  // a segment for every wave at least
+  if (nvec <= 1024) GO(256, 4, 1);
+  else if (nvec <= 4096) GO(1024, 4, 1);
+  else GO(1024, 4, 4);
 #undef GO
 }
 
