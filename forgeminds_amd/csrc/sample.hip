@@ -51,7 +51,7 @@ struct SampleArgs {
 
 // A row as whole 16-byte vectors from the last 16-byte border at or before its first element; what
 // the first and the last vector hold outside the row reads as -inf (weight zero, never kept) and is
-// not loaded.
+// not loaded: those two are put together in shared memory once.
 template <typename T>
 struct RowView {
   static constexpr int EPV = Elem<T>::kVec;
@@ -60,7 +60,8 @@ struct RowView {
   int v;
   int nvec;
   int w0, w1;       // vectors [w0, w1) lie inside the row
-  __device__ __forceinline__ RowView(const T* row, int v_) : v(v_) {
+  u32x4* edges;     // shared memory, two vectors
+  __device__ __forceinline__ RowView(const T* row, int v_, u32x4* edges_) : v(v_), edges(edges_) {
     lead = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
     base = row - lead;
     nvec = (v + lead + EPV - 1) / EPV;
@@ -70,17 +71,17 @@ struct RowView {
   __device__ __forceinline__ bool whole(int c) const { return c >= w0 && c < w1; }
   __device__ __forceinline__ int clamp(int c) const { return c < w0 ? w0 : (c < w1 ? c : w1 - 1); }
   __device__ __forceinline__ int col0(int c) const { return c * EPV - lead; }
-  __device__ __forceinline__ float load_one(int col) const {
-    return Elem<T>::load1(base + lead + col);
+  // the first and the last vector, by the workgroup's first threads (a barrier is due)
+  __device__ __forceinline__ void fill_edges() const {
+    const int t = threadIdx.x;
+    if (t >= 2 * EPV) return;
+    const int col = col0(t < EPV ? 0 : nvec - 1) + t % EPV;
+    const bool inside = col >= 0 && col < v;
+    Elem<T>::store1(reinterpret_cast<T*>(edges) + t, inside ? Elem<T>::load1(base + lead + col) : -INFINITY);
   }
   __device__ __forceinline__ u32x4 partial(int c) const {
-    float f[EPV];
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) {
-      const int col = col0(c) + e;
-      f[e] = (col >= 0 && col < v) ? load_one(col) : -INFINITY;
-    }
-    return Elem<T>::pack(f);
+    return reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
+        (const __attribute__((address_space(3))) void*)edges)[c < w0 ? 0 : 1];
   }
   // one whole vector: the address space is spelled out, since behind the views' pointers the compiler
   // takes the load for a flat one, whose wait is a wait for everything
@@ -88,6 +89,33 @@ struct RowView {
     return *(const __attribute__((address_space(1))) u32x4*)(reinterpret_cast<const char*>(base) + (uint32_t)c * 16u);
   }
   __device__ __forceinline__ u32x4 load(int c) const { return whole(c) ? load_whole(c) : partial(c); }
+};
+
+// a value that all lanes hold alike, in scalar registers: branches on it stay scalar
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+__device__ __forceinline__ double uniform(double v) { return readlane64(v, 0); }
+
+// the first element of a vector, which moves on by one
+template <typename T>
+__device__ __forceinline__ float pop_element(u32x4& r) {
+  float x[Elem<T>::kVec];
+  Elem<T>::unpack(r, x);
+  if constexpr (sizeof(T) == 4) {
+    r.x = r.y; r.y = r.z; r.z = r.w;
+  } else {
+    r.x = __builtin_amdgcn_alignbit(r.y, r.x, 16);
+    r.y = __builtin_amdgcn_alignbit(r.z, r.y, 16);
+    r.z = __builtin_amdgcn_alignbit(r.w, r.z, 16);
+    r.w >>= 16;
+  }
+  return x[0];
+}
+
+struct OpMaximum {      // NaN stays
+  __device__ static __forceinline__ float f(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 };
 
 struct Cut {
@@ -98,16 +126,16 @@ struct Cut {
 template <int THREADS>
 struct SampleShared {
   static constexpr int kList = 4 * THREADS;                  // candidates
-  static constexpr int kSegs = THREADS < 1024 ? 32 : 4160;   // segments of 64 vectors (v <= 2^20)
-  union {
-    struct {
-      unsigned long long bins[kBins];
-      unsigned long long list[kList];       // (key << 32) | ~column: larger comes first
-      unsigned long long step[kStep];       // the candidates of one step or segment ...
-      unsigned long long mass[kStep];       // ... and their weights
-    } h;
-    double seg[kSegs];
-  };
+  static constexpr int kSegs = 1040;   // segments (v <= 2^20)
+  struct {
+    unsigned long long bins[kBins];
+    unsigned long long list[kList];       // (key << 32) | ~column: larger comes first
+    unsigned long long step[kStep];       // the candidates of one step or segment ...
+    unsigned long long mass[kStep];       // ... and their weights
+  } h;
+  u32x4 edges[2];
+  double seg[kSegs];
+  float segm[kSegs];
   double red[THREADS / 64];
   float redf[1][THREADS / 64];
   unsigned long long redu[THREADS / 64];
@@ -123,23 +151,25 @@ struct SampleShared {
   double weight;
 };
 
-// exp((x - m) / T) = 2^((x - m) c) by the polynomial of exp2_64, written out for several elements at once:
+// exp((x - m) / T) = 2^((x - m) c), c = log2(e) / T, by the polynomial of exp2_64, written out for several elements at once:
 // seventeen operations each, the constants in scalar registers (the compiler otherwise copies each into
 // two vector registers for every use, which doubles the work), and n from the low bits of t + 1.5 * 2^52.
 // The maximum's weight is exactly 1, so that rows of few distinct values split evenly; that of -inf is 0.
 struct Weight {
   double m, c;
   double k[9], magic, least;
-  __device__ __forceinline__ Weight(float max_x, float T) : m((double)max_x), c(kLog2ed / (double)T) {
+  __device__ __forceinline__ Weight(double max_x, double c_) : m(max_x), c(c_) {
     k[8] = 1.3255224878668817e-06; k[7] = 1.5310079402249296e-05; k[6] = 0.00015403455852453838;
     k[5] = 0.0013333450568000645; k[4] = 0.009618129159402558; k[3] = 0.05550410941205933;
     k[2] = 0.2402265069581299; k[1] = 0.6931471805459335; k[0] = 1.0;
     magic = 6755399441055744.0;
     least = -1100.0;
 #pragma unroll
-    for (int i = 0; i < 9; ++i) asm("" : "+s"(k[i]));
-    asm("" : "+s"(magic), "+s"(least));
+    for (int i = 0; i < 9; ++i) asm volatile("" : "+s"(k[i]));
+    asm volatile("" : "+s"(magic), "+s"(least));
   }
+  // the same for one sweep: its constants take up scalar registers there only
+  __device__ __forceinline__ Weight fresh() const { return Weight(m, c); }
   template <int N>
   __device__ __forceinline__ void eval(const float* x, double* w) const {
     double f[N], r[N];
@@ -171,12 +201,20 @@ struct Weight {
   }
 };
 
+// The thread's number, formed anew at each use: otherwise every address made of it is kept in a register
+// of its own over the loop of the two cuts.
+__device__ __forceinline__ int thread_here() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // First of `n` non-negative entries (in LDS, in order) whose running sum reaches `target`
 // (strict: exceeds it); *before is the sum ahead of it. n when there is none. All threads call it.
 template <int THREADS, bool STRICT, typename F>
 __device__ __forceinline__ int find_running(F entry, int n, double target, SampleShared<THREADS>& sh, double* before) {
   constexpr int NW = THREADS / 64;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = thread_here(), lane = tid & 63, wave = tid >> 6;
   const int per = (n + THREADS - 1) / THREADS;
   auto there = [&](double run) { return STRICT ? run > target : run >= target; };
   double mine = 0.0;
@@ -210,10 +248,10 @@ __device__ __forceinline__ int find_running(F entry, int n, double target, Sampl
     atomicMin(&sh.at, at);
   }
   __syncthreads();
-  const int found = sh.at;
+  const int found = uniform(sh.at);
   if (at < n && at == found) sh.weight = run;
   __syncthreads();
-  *before = sh.weight;
+  *before = uniform(sh.weight);
   __syncthreads();
   return found;
 }
@@ -222,7 +260,7 @@ __device__ __forceinline__ int find_running(F entry, int n, double target, Sampl
 template <typename T, int THREADS, int UN, typename F>
 __device__ __forceinline__ void each_vector(const RowView<T>& rv, F fn) {
   const bool any = rv.w0 < rv.w1;
-  for (int c0 = threadIdx.x; c0 < rv.nvec; c0 += THREADS * UN) {
+  for (int c0 = thread_here(); c0 < rv.nvec; c0 += THREADS * UN) {
     u32x4 raw[UN];
     if (any) {
 #pragma unroll
@@ -286,7 +324,7 @@ __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double targe
   if (end) {          // the last segment with a weight
     if (threadIdx.x == 0) sh.at = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < nseg; i += THREADS) if (sh.seg[i] > 0.0) atomicMax(&sh.at, i);
+    for (int i = thread_here(); i < nseg; i += THREADS) if (sh.seg[i] > 0.0) atomicMax(&sh.at, i);
     __syncthreads();
     s = sh.at;
     __syncthreads();
@@ -339,14 +377,15 @@ __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double targe
   return col;
 }
 
-// Segment sums of weights_of(x, col0, w) over the row into sh.seg.
+// Segment sums over the row into sh.seg; sum_of(x, col0) is what a vector adds.
 template <typename T, int THREADS, int G, typename F>
-__device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F weights_of, SampleShared<THREADS>& sh) {
+__device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F sum_of, SampleShared<THREADS>& sh) {
   constexpr int EPV = Elem<T>::kVec;
   __syncthreads();
   const bool any = rv.w0 < rv.w1;
-  for (int s = threadIdx.x >> 6; s < nseg; s += THREADS / 64) {
-    const int c0 = s * seg_vecs(G) + (threadIdx.x & 63);
+  const int tid = thread_here();
+  for (int s = tid >> 6; s < nseg; s += THREADS / 64) {
+    const int c0 = s * seg_vecs(G) + (tid & 63);
     u32x4 raw[G];
     if (any) {
 #pragma unroll
@@ -360,15 +399,12 @@ __device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F w
       if (c < rv.nvec) {
         if (!rv.whole(c)) raw[i] = rv.partial(c);
         float x[EPV];
-        double w[EPV];
         Elem<T>::unpack(raw[i], x);
-        weights_of(x, rv.col0(c), w);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) mine += w[e];
+        mine += sum_of(x, rv.col0(c));
       }
     }
     mine = wave_sum64(mine);
-    if ((threadIdx.x & 63) == 0) sh.seg[s] = mine;
+    if ((tid & 63) == 0) sh.seg[s] = mine;
   }
   __syncthreads();
 }
@@ -386,7 +422,7 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
     const int bits = 32 - __builtin_clz(hi - lo);
     const int shift = bits > 11 ? bits - 11 : 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
+    for (int i = thread_here(); i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
     __syncthreads();
     int open = -1;
     unsigned long long held = 0ull;
@@ -408,14 +444,15 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
     if (b == kBins) {       // rounding: everything stays, the lowest value is the cut
       if (threadIdx.x == 0) sh.at = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < kBins; i += THREADS) if (sh.h.bins[i] != 0ull) atomicMax(&sh.at, i);
+      for (int i = thread_here(); i < kBins; i += THREADS) if (sh.h.bins[i] != 0ull) atomicMax(&sh.at, i);
       __syncthreads();
-      b = sh.at;
+      b = uniform(sh.at);
     }
     // the amount ahead of that range, as an integer
     unsigned long long mine = 0ull;
-    for (int i = threadIdx.x; i < b; i += THREADS) mine += sh.h.bins[i];
-    ahead += block_sum_int64<THREADS / 64>(mine, sh.redu);
+    for (int i = thread_here(); i < b; i += THREADS) mine += sh.h.bins[i];
+    mine = block_sum_int64<THREADS / 64>(mine, sh.redu);
+    ahead += ((unsigned long long)(uint32_t)uniform((int)(mine >> 32)) << 32) | (uint32_t)uniform((int)(uint32_t)mine);
     const uint32_t top = hi - ((uint32_t)b << shift);
     const uint32_t span = (1u << shift) - 1u;
     lo = top - lo > span ? top - span : lo;
@@ -426,17 +463,24 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
   return lo;
 }
 
-// Column of the c-th (1-based) element equal to x0 in index order; INT_MAX when there are no more than c.
+// Column of the c-th (1-based) element equal to x0 > -inf in index order; INT_MAX when there are no more
+// than c.
 template <typename T, int THREADS, int G>
 __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x0, double c, SampleShared<THREADS>& sh) {
   constexpr int EPV = Elem<T>::kVec;
-  auto equal = [&](const float* x, int col0, double* w) {
+  auto equal = [&](const float* x, int, double* w) {
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) w[e] = x[e] == x0 && col0 + e >= 0 && col0 + e < rv.v ? 1.0 : 0.0;
+    for (int e = 0; e < EPV; ++e) w[e] = x[e] == x0 ? 1.0 : 0.0;
   };
-  segment_sums<T, THREADS, G>(rv, nseg, equal, sh);
+  auto equal_count = [&](const float* x, int) {
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) n += x[e] == x0 ? 1 : 0;
+    return (double)n;
+  };
+  segment_sums<T, THREADS, G>(rv, nseg, equal_count, sh);
   double mine = 0.0;
-  for (int i = threadIdx.x; i < nseg; i += THREADS) mine += sh.seg[i];
+  for (int i = thread_here(); i < nseg; i += THREADS) mine += sh.seg[i];
   const double all = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
   if (c >= all) return 0x7fffffff;
   double w;
@@ -448,11 +492,11 @@ template <int THREADS>
 __device__ __forceinline__ void sort_step(SampleShared<THREADS>& sh, int n) {
   int N = 2;
   while (N < n) N *= 2;
-  for (int i = n + threadIdx.x; i < N; i += THREADS) sh.h.step[i] = 0ull;
+  for (int i = n + thread_here(); i < N; i += THREADS) sh.h.step[i] = 0ull;
   __syncthreads();
   for (int k = 2; k <= N; k *= 2) {
     for (int j = k / 2; j > 0; j /= 2) {
-      for (int p = threadIdx.x; p < N / 2; p += THREADS) {
+      for (int p = thread_here(); p < N / 2; p += THREADS) {
         const int i = 2 * p - (p & (j - 1)), o = i + j;
         const unsigned long long a = sh.h.step[i], b = sh.h.step[o];
         const bool up = (i & k) != 0;            // ascending half
@@ -470,7 +514,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   constexpr int kList = SampleShared<THREADS>::kList;
   __shared__ SampleShared<THREADS> sh;
   const int64_t row = blockIdx.x;
-  const RowView<T> rv(logits + row * (int64_t)a.v, a.v);
+  const RowView<T> rv(logits + row * (int64_t)a.v, a.v, sh.edges);
+  rv.fill_edges();
+  __syncthreads();
   const int tid = threadIdx.x;
 
   const float T_ = a.temp != nullptr ? a.temp[row] : a.temp0;
@@ -486,47 +532,103 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   const bool use_m = min_p > 0.f;
   min_p = fminf(min_p, 1.f);
   auto each = [&](auto fn) { each_vector<T, THREADS, UN>(rv, fn); };
-
-  // 1: the maximum; NaN propagates
-  float mx = -INFINITY;
-  each_vector<T, THREADS, 8>(rv, [&](const u32x4& r, int) {
-    float x[EPV];
-    Elem<T>::unpack(r, x);
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) mx = __builtin_elementwise_maximum(mx, x[e]);
-  });
-  float wm = mx;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) wm = __builtin_elementwise_maximum(wm, __shfl_xor(wm, o, 64));
-  // A value that at least k elements are not below: in each wave the ceil(k / waves)-th largest of the
-  // threads' maxima, found bit by bit with ballots, and the least of those over the waves.
-  uint32_t vouch = 0u;
-  if (use_k) {
-    const uint32_t key = key_of(mx);
-    const int q = (k + NW - 1) / NW;
-    for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1)
-      if (__builtin_popcountll(__ballot(key >= (vouch | bit))) >= q) vouch |= bit;
-  }
-  if ((tid & 63) == 0) { sh.redf[0][tid >> 6] = wm; sh.redi[tid >> 6] = (int)vouch; }
-  if (tid == 0) { sh.count = 0; sh.at = 0; }
-  __syncthreads();
-  float m = sh.redf[0][0];
-  vouch = (uint32_t)sh.redi[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) {
-    m = __builtin_elementwise_maximum(m, sh.redf[0][i]);
-    vouch = (uint32_t)sh.redi[i] < vouch ? (uint32_t)sh.redi[i] : vouch;
-  }
-  const float vouched_x = vouch <= 0x007FFFFFu ? -INFINITY : float_of_key(vouch);      // that is key_of(-inf)
-  // (NaN compares false everywhere)
-  if (!(m < INFINITY && m > -INFINITY) || !(T_ >= 0.f && T_ < INFINITY)) {
+  const int nseg = (rv.nvec + seg_vecs(G) - 1) / seg_vecs(G);
+  auto no_row = [&]() {            // no distribution
     if (tid == 0) {
       a.token[row] = -1;
       if (a.logprob != nullptr) a.logprob[row] = __builtin_nanf("");
     }
-    return;
+  };
+  auto total_of = [](const double* w) {
+    double t = w[0];
+#pragma unroll
+    for (int e = 1; e < EPV; ++e) t += w[e];
+    return t;
+  };
+  const bool t_ok = T_ >= 0.f && T_ < INFINITY;
+  float m;
+  uint32_t vouch = 0u;
+  const bool whole = t_ok && T_ > 0.f && !use_k && !use_p && !use_m;
+  if (whole) {
+    // Nothing cuts: one sweep, each segment's weights against its own maximum, brought together below.
+    const double c = kLog2ed / (double)T_;
+    const bool any = rv.w0 < rv.w1;
+    for (int s = tid >> 6; s < nseg; s += NW) {
+      const int c0 = s * seg_vecs(G) + (tid & 63);
+      u32x4 raw[G];
+      if (any) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * 64));
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        if (any) touch_whole(raw[i]);
+        if (c0 + i * 64 < rv.nvec) {
+          if (!rv.whole(c0 + i * 64)) raw[i] = rv.partial(c0 + i * 64);
+          float x[EPV];
+          Elem<T>::unpack(raw[i], x);
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+        }
+      }
+      top = group_reduce<64, OpMaximum>(top);
+      double mine = 0.0;
+      if (top > -INFINITY && top < INFINITY) {
+        const Weight seg_weight((double)top, c);
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          if (c0 + i * 64 < rv.nvec) {
+            float x[EPV];
+            double w[EPV];
+            Elem<T>::unpack(raw[i], x);
+            seg_weight.template eval<EPV>(x, w);
+            mine += total_of(w);
+          }
+        }
+      }
+      mine = wave_sum64(mine);
+      if ((tid & 63) == 0) { sh.seg[s] = mine; sh.segm[s] = top; }
+    }
+    __syncthreads();
+    m = -INFINITY;
+    for (int i = tid & 63; i < nseg; i += 64) m = __builtin_elementwise_maximum(m, sh.segm[i]);
+    m = uniform(group_reduce<64, OpMaximum>(m));
+    if (!(m < INFINITY && m > -INFINITY)) { no_row(); return; }
+    for (int i = tid; i < nseg; i += THREADS) sh.seg[i] *= exp2_64(((double)sh.segm[i] - (double)m) * c);
+    __syncthreads();
+  } else {
+    // 1: the maximum; NaN propagates
+    float mx = -INFINITY;
+    each_vector<T, THREADS, 8>(rv, [&](const u32x4& r, int) {
+      float x[EPV];
+      Elem<T>::unpack(r, x);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) mx = __builtin_elementwise_maximum(mx, x[e]);
+    });
+    const float wm = group_reduce<64, OpMaximum>(mx);
+    // A value that at least k elements are not below: in each wave the ceil(k / waves)-th largest of the
+    // threads' maxima, found bit by bit with ballots, and the least of those over the waves.
+    if (use_k && k <= 64 * NW) {
+      const uint32_t key = key_of(mx);
+      const int q = (k + NW - 1) / NW;
+      for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1)
+        if (__builtin_popcountll(__ballot(key >= (vouch | bit))) >= q) vouch |= bit;
+    }
+    if ((tid & 63) == 0) { sh.redf[0][tid >> 6] = wm; sh.redi[tid >> 6] = (int)vouch; }
+    __syncthreads();
+    m = sh.redf[0][0];
+    vouch = (uint32_t)sh.redi[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) {
+      m = __builtin_elementwise_maximum(m, sh.redf[0][i]);
+      vouch = (uint32_t)sh.redi[i] < vouch ? (uint32_t)sh.redi[i] : vouch;
+    }
+    m = uniform(m);
+    vouch = (uint32_t)uniform((int)vouch);
+    // (NaN compares false everywhere)
+    if (!(m < INFINITY && m > -INFINITY) || !t_ok) { no_row(); return; }
   }
-  const int nseg = (rv.nvec + seg_vecs(G) - 1) / seg_vecs(G);
   if (T_ == 0.f) {           // the first maximum
     __syncthreads();         // sh.redi
     int first = 0x7fffffff;
@@ -546,16 +648,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     }
     return;
   }
-  const Weight weight(m, T_);
+  const Weight base((double)m, uniform(kLog2ed / (double)T_));
   Cut cut{-INFINITY, -1};           // -inf itself is never kept
-  float x_min = -INFINITY;          // min-p: the least value with a weight of min_p
-  if (use_m) {
-    const double xm = (double)m + (double)T_ * log((double)min_p);
-    x_min = (float)xm;                      // may be -inf: then everything stays
-    if ((double)x_min < xm) x_min = float_of_key(key_of(x_min) + 1u);      // the next float up
-    if (x_min > m) x_min = m;
-  }
-  if (use_k || use_p || use_m) {
+  auto kept = [&](float x, int col) { return x > cut.x || (x == cut.x && col <= cut.col); };
+  if (!whole) {
+    float x_min = -INFINITY;          // min-p: the least value with a weight of min_p
+    if (use_m) {
+      const double xm = (double)m + (double)T_ * (log2_64((double)min_p) * kLn2d);
+      x_min = (float)xm;                      // may be -inf: then everything stays
+      if ((double)x_min < xm) x_min = float_of_key(key_of(x_min) + 1u);      // the next float up
+      if (x_min > m) x_min = m;
+    }
     // 2^fx units of mass per 1: the sum of v weights of at most 1 stays below 2^62
     const int vbits = 62 - (32 - __builtin_clz((unsigned)a.v));
     const int fx = vbits < 50 ? vbits : 50;
@@ -567,49 +670,25 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     auto value = [](unsigned long long e) { return float_of_key((uint32_t)(e >> 32)); };
     auto column = [](unsigned long long e) { return (int)~(uint32_t)e; };
 
-    // 2: the bound of the candidates, and where top-p alone has its cut
-    float bound = x_min;
-    if (use_k) bound = vouched_x;
-    // Steps of equal width from the maximum down to the bound; over 12 T where top-p is alone (24 T for a
-    // top-p past 0.99). A cut further down than that, where each element weighs less than 6e-6 of the
-    // largest, is left to the search.
-    const float nats = p <= 0.99f ? 12.f : 24.f;
-    float range = use_k ? m - bound : nats * T_;
-    if (!(range < INFINITY)) range = 24.f * T_;
-    float per = (float)(kBins - 2) / range;
-    if (!(per <= 1e30f)) per = 1e30f;
-    auto step_of = [&](float x) { return (m - x) * per; };       // grows as x falls; never NaN
+    // steps of equal width from the maximum down
+    float per = 0.f;
     const float last_bin = (float)(kBins - 1);
-    double total = 0.0, ahead = 0.0, goal = 0.0;
-    int bin = kBins;
-    const bool from_row = use_p && !use_k;
-    if (from_row) {
-      for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
-      __syncthreads();
-      each([&](const u32x4& r, int) {
-        float x[EPV];
-        Elem<T>::unpack(r, x);
-        double w[EPV];
-        weight.template eval<EPV>(x, w);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) {
-          total += w[e];
-          const float y = step_of(x[e]);
-          if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], fixed(w[e]));
-        }
-      });
-      total = block_reduce64<NW, Sum64>(total, sh.red);
-      goal = (double)p * total * unit;
-      __syncthreads();
-      bin = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal, sh, &ahead);
-    }
-    if (tid == 0) { sh.at = 0; sh.klo = 0xFFFFFFFFu; sh.khi = 0u; }
-    __syncthreads();
-    const float lo = (float)bin, hi = (float)(bin + 1);
-    const bool found = !from_row || bin < kBins;
-    int nb = 0;
+    auto steps_over = [&](float range) {
+      per = (float)(kBins - 2) / range;
+      if (!(per <= 1e30f)) per = 1e30f;
+    };
+    auto step_of = [&](float x) { return (m - x) * per; };       // grows as x falls; never NaN
+
+    // 2: the list of candidates -- those not below `bound`, or (by_step) those down to the end of the step
+    // [lo, hi), which is listed apart as well -- of what the cut so far keeps
+    float bound = x_min;
     bool listed = false;
-    if (found) {
+    int n = 0, nb = 0;
+    auto gather = [&](bool by_step, float lo, float hi) {
+      const bool restricted = cut.x > -INFINITY;
+      __syncthreads();
+      if (tid == 0) { sh.count = 0; sh.at = 0; sh.klo = 0xFFFFFFFFu; sh.khi = 0u; }
+      __syncthreads();
       bool full = false;
       uint32_t klo = 0xFFFFFFFFu, khi = 0u;      // keys of the step
       each([&](const u32x4& r, int c) {
@@ -618,27 +697,32 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         float top = x[0];
 #pragma unroll
         for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
-        if (__ballot(from_row ? step_of(top) < hi : top >= bound) == 0ull) return;
-        if (full && !from_row) return;
-#pragma unroll
+        if (__ballot(by_step ? step_of(top) < hi : top >= bound) == 0ull) return;
+        if (full && !by_step) return;
+        u32x4 rest = r;
+#pragma unroll 1
         for (int e = 0; e < EPV; ++e) {
-          const float y = step_of(x[e]);
-          const bool cand = from_row ? y < hi : (x[e] >= bound && x[e] > -INFINITY);
+          const float xe = pop_element<T>(rest);
+          const float y = step_of(xe);
+          const bool in_step = y >= lo && y < hi;
+          // (a full list takes no more, but the step still does)
+          bool cand = by_step ? (full ? in_step : y < hi) : (xe >= bound && xe > -INFINITY);
+          if (restricted) cand = cand && kept(xe, rv.col0(c) + e);
           const unsigned long long who = __ballot(cand);
           if (who == 0ull) continue;
-          const uint32_t key = key_of(x[e]);
+          const uint32_t key = key_of(xe);
           const unsigned long long entry = ((unsigned long long)key << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
           if (!full) {
-            const int n = __builtin_popcountll(who);
+            const int count = __builtin_popcountll(who);
             int base = 0;
             const int first = __builtin_ctzll(who);
-            if ((tid & 63) == first) base = atomicAdd(&sh.count, n);
+            if ((tid & 63) == first) base = atomicAdd(&sh.count, count);
             base = __builtin_amdgcn_readlane(base, first);
             const int at = base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
             if (cand && at < kList) sh.h.list[at] = entry;
-            full = base + n > kList;
+            full = base + count > kList;
           }
-          if (from_row && cand && y >= lo) {
+          if (by_step && cand && in_step) {
             klo = key < klo ? key : klo;
             khi = key > khi ? key : khi;
             if (sh.at <= kStep) {       // counted past the end once: the step is too long
@@ -648,109 +732,135 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
           }
         }
       });
-      if (from_row && klo <= khi) { atomicMin(&sh.klo, klo); atomicMax(&sh.khi, khi); }
+      if (by_step && klo <= khi) { atomicMin(&sh.klo, klo); atomicMax(&sh.khi, khi); }
       __syncthreads();
-      nb = sh.at;
-      listed = sh.count <= kList;
-    }
-    const int n = sh.count < kList ? sh.count : kList;
+      nb = uniform(sh.at);
+      n = uniform(sh.count);
+      listed = n <= kList;
+      __syncthreads();
+    };
 
-    // 3: the exact cut. `settle` takes the n_step elements in sh.h.step, the step that holds the cut with
-    // `before` ahead of it: the last element that stays is the first whose running amount reaches the goal.
-    auto settle = [&](int n_step, double before, double goal_, bool count) {
-      sort_step<THREADS>(sh, n_step);
-      auto amount = [&](int i) { return count ? 1.0 : (double)fixed(weight(value(sh.h.step[i]))); };
-      double unused;
-      int r = find_running<THREADS, false>(amount, n_step, goal_ - before, sh, &unused);
-      if (r >= n_step) r = n_step - 1;
-      cut.x = value(sh.h.step[r]);
-      cut.col = column(sh.h.step[r]);
+    // 3: the exact cuts, first by count, then by the mass of what that leaves. The cut is the first element,
+    // in descending order, at which the running amount reaches the goal.
+    if (use_k) {
+      bound = vouch <= 0x007FFFFFu ? -INFINITY : float_of_key(vouch);      // that is key_of(-inf)
+      const float range = m - bound;
+      steps_over(range < INFINITY ? range : 24.f * T_);
+    } else {
+      steps_over((p <= 0.99f ? 12.f : 24.f) * T_);
+    }
+    // (with top-p alone there is no bound to list by)
+    if (use_k ? bound > -INFINITY || a.v <= kList : !use_p) gather(false, 0.f, 0.f);
+    auto settle = [&](auto by_count) {
+      constexpr bool count = decltype(by_count)::value;
+      const int tid = thread_here();
+      if (count && listed && n < k) return;         // all of them stay
+      const bool by_list = listed;
+      const bool restricted = cut.x > -INFINITY;
+      if (!by_list && use_k && !count) steps_over(24.f * T_);
       __syncthreads();
-    };
-    auto kept = [&](unsigned long long e) {
-      const float x = value(e);
-      return x > cut.x || (x == cut.x && column(e) <= cut.col);
-    };
-    // the same from the list, for the elements of it that are still kept; false when the step is too long
-    auto settle_list = [&](double goal_or_p, bool count) {
       for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
-      if (tid == 0) sh.at = 0;
       __syncthreads();
-      unsigned long long mine = 0ull;
+      // the amount by step
+      const Weight weight = base.fresh();
+      double goal;
+      if (by_list) {
+        unsigned long long mine = 0ull;
 #pragma unroll 1
-      for (int i = tid; i < n; i += THREADS) {
-        const unsigned long long e = sh.h.list[i];
-        if (!kept(e)) continue;
-        const unsigned long long w = count ? 1ull : fixed(weight(value(e)));
-        const float y = step_of(value(e));
-        atomicAdd(&sh.h.bins[y < last_bin ? (int)y : kBins - 1], w);
-        mine += w;
-      }
-      const double mass = (double)block_sum_int64<NW>(mine, sh.redu);      // its barriers publish the histogram
-      const double goal_ = count ? goal_or_p : goal_or_p * mass;
-      double before;
-      int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal_, sh, &before);
-      if (b == kBins) return true;         // everything stays
-      if (tid == 0) sh.at = 0;
-      __syncthreads();
-#pragma unroll 1
-      for (int i = tid; i < n; i += THREADS) {
-        const unsigned long long e = sh.h.list[i];
-        const float y = step_of(value(e));
-        if (kept(e) && (y < last_bin ? (int)y : kBins - 1) == b) {
-          const int at = atomicAdd(&sh.at, 1);
-          if (at < kStep) sh.h.step[at] = e;
+        for (int i = tid; i < n; i += THREADS) {
+          const unsigned long long e = sh.h.list[i];
+          if (!kept(value(e), column(e))) continue;
+          const unsigned long long w = count ? 1ull : fixed(weight(value(e)));
+          const float y = step_of(value(e));
+          atomicAdd(&sh.h.bins[y < last_bin ? (int)y : kBins - 1], w);
+          mine += w;
         }
+        goal = (double)p * (double)block_sum_int64<NW>(mine, sh.redu);
+      } else {
+        double total = 0.0;
+        each([&](const u32x4& r, int c) {
+          float x[EPV];
+          Elem<T>::unpack(r, x);
+          if (restricted) {
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) x[e] = kept(x[e], rv.col0(c) + e) ? x[e] : -INFINITY;
+          }
+          if (count) {
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) {
+              const float y = step_of(x[e]);
+              if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], 1ull);
+            }
+          } else {
+            double w[EPV];
+            weight.template eval<EPV>(x, w);
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) {
+              total += w[e];
+              const float y = step_of(x[e]);
+              if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], fixed(w[e]));
+            }
+          }
+        });
+        goal = (double)p * block_reduce64<NW, Sum64>(total, sh.red) * unit;
       }
+      goal = count ? (double)k : uniform(goal);
       __syncthreads();
-      const int n_step = sh.at;
-      if (n_step > kStep) return false;
-      settle(n_step, before, goal_, count);
-      return true;
+      // the step that holds the cut, its elements in sh.h.step
+      double ahead;
+      const int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal, sh, &ahead);
+      if (by_list) {
+        if (b == kBins) return;         // everything stays
+        if (tid == 0) { sh.at = 0; sh.klo = 0xFFFFFFFFu; sh.khi = 0u; }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = tid; i < n; i += THREADS) {
+          const unsigned long long e = sh.h.list[i];
+          const float y = step_of(value(e));
+          if ((y < last_bin ? (int)y : kBins - 1) == b && kept(value(e), column(e))) {
+            const int at = atomicAdd(&sh.at, 1);
+            if (at < kStep) sh.h.step[at] = e;
+            atomicMin(&sh.klo, (uint32_t)(e >> 32));
+            atomicMax(&sh.khi, (uint32_t)(e >> 32));
+          }
+        }
+        __syncthreads();
+        nb = uniform(sh.at);
+      } else if (b < kBins) {
+        gather(true, (float)b, (float)(b + 1));
+      }
+      if (b < kBins && nb <= kStep) {
+        sort_step<THREADS>(sh, nb);
+        double unused;
+        int r = find_running<THREADS, false>(
+            [&](int i) { return count ? 1.0 : (double)fixed(weight(value(sh.h.step[i]))); }, nb, goal - ahead, sh, &unused);
+        r = r < nb ? r : nb - 1;
+        cut.x = uniform(value(sh.h.step[r]));
+        cut.col = uniform(column(sh.h.step[r]));
+        return;
+      }
+      // More elements than that: by the bits of the value, then by column among equal ones.
+      uint32_t lo = 0u, hi = 0xFFFFFFFEu;
+      unsigned long long above = 0ull;
+      if (b < kBins) {
+        lo = (uint32_t)uniform((int)sh.klo);
+        hi = (uint32_t)uniform((int)sh.khi);
+        above = (unsigned long long)ahead;
+      }
+      const uint32_t key = key_search<T, THREADS>(
+          rv, lo, hi, above, goal, [&](float x) { return count ? 1ull : fixed(weight(x)); }, sh, &above);
+      const float x = float_of_key(key);
+      const double each_w = count ? 1.0 : (double)fixed(weight(x));
+      // the r-th of the equal ones stays iff above + (r - 1) * weight < goal
+      double need = each_w > 0.0 ? ceil((goal - (double)above) / each_w) : 1.0;
+      need = uniform(need >= 1.0 ? need : 1.0);
+      int col = x > -INFINITY ? nth_equal<T, THREADS, G>(rv, nseg, x, need, sh) : -1;
+      if (x == cut.x && cut.col < col) col = cut.col;
+      if (x >= cut.x) cut = Cut{x, col};
+      listed = listed && b < kBins;
     };
-    bool settled = !use_k && !use_p;
-    if (use_k && listed && (n >= k || bound == -INFINITY)) {      // (fewer than k: all that are not -inf)
-      settled = n < k || settle_list((double)k, true);
-      if (settled && use_p) settled = settle_list((double)p, false);
-    } else if (from_row && found && nb <= kStep) {
-      settle(nb, ahead, goal, false);
-      settled = true;
-    }
-    if (!settled) {
-      double ties = 0.0;
-      unsigned long long above;
-      cut = Cut{-INFINITY, -1};
-      if (use_k) {
-        const uint32_t key = key_search<T, THREADS>(rv, 0u, 0xFFFFFFFEu, 0ull, (double)k, [](float) { return 1ull; }, sh, &above);
-        cut.x = float_of_key(key);
-        ties = (double)k - (double)above;
-        if (use_p) {      // the mass of those k
-          double mine = 0.0;
-          each_element<T, THREADS>(rv, [&](float x, int) { if (x > cut.x) mine += weight(x); });
-          total = block_reduce64<NW, Sum64>(mine, sh.red) + ties * weight(cut.x);
-        }
-      }
-      if (use_p) {
-        const double goal_p = (double)p * total * unit;
-        const bool in_step = from_row && found;
-        const uint32_t key = key_search<T, THREADS>(rv, in_step ? sh.klo : 0u, in_step ? sh.khi : 0xFFFFFFFEu,
-                                                    in_step ? (unsigned long long)ahead : 0ull, goal_p,
-                                                    [&](float x) { return fixed(weight(x)); }, sh, &above);
-        const float xp = float_of_key(key);
-        const double each_w = (double)fixed(weight(xp));
-        // equal values that the mass still needs: the r-th stays iff above + r * weight < goal
-        double need = each_w > 0.0 ? ceil((goal_p - (double)above) / each_w) : 1.0;
-        if (!(need >= 1.0)) need = 1.0;
-        if (!use_k || xp > cut.x) {
-          cut.x = xp;
-          ties = need;
-        } else if (xp == cut.x && need < ties) {
-          ties = need;
-        }
-      }
-      cut.col = nth_equal<T, THREADS, G>(rv, nseg, cut.x, ties, sh);
-      listed = false;          // the searches took the list's place
-    }
+    if (use_k) settle(std::true_type{});
+    if (use_p) settle(std::false_type{});
     if (x_min > cut.x) {       // every value equal to the bound stays
       cut.x = x_min;
       cut.col = 0x7fffffff;
@@ -765,6 +875,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       __syncthreads();
       for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
       __syncthreads();
+      const Weight weight = base.fresh();
       unsigned long long me[PER], w[PER], mine = 0ull;
       int seg[PER];
 #pragma unroll
@@ -774,14 +885,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         if (j * THREADS >= n) continue;
         if (i >= n) continue;
         me[j] = sh.h.list[i];
-        if (!kept(me[j])) continue;
+        if (!kept(value(me[j]), column(me[j]))) continue;
         w[j] = fixed(weight(value(me[j])));
         seg[j] = (int)(((uint32_t)column(me[j]) + (uint32_t)rv.lead) >> seg_bits);
         atomicAdd(&sh.h.bins[seg[j]], w[j]);
         mine += w[j];
       }
-      const double mass = (double)block_sum_int64<NW>(mine, sh.redu);
+      const double mass = uniform((double)block_sum_int64<NW>(mine, sh.redu));
       const double target = u * mass;
+      double ahead;
       const int s = find_running<THREADS, true>([&](int i) { return (double)sh.h.bins[i]; }, kBins, target, sh, &ahead);
       if (tid == 0) { sh.at = 0; sh.col = -1; }
       __syncthreads();
@@ -794,7 +906,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         }
       }
       __syncthreads();
-      const int ns = sh.at;
+      const int ns = uniform(sh.at);
       for (int i = tid; i < ns; i += THREADS) {
         const int col = column(sh.h.step[i]);
         unsigned long long before = 0ull;
@@ -808,7 +920,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       if (sh.col >= 0) {
         if (tid == 0) {
           a.token[row] = sh.col;
-          if (a.logprob != nullptr) a.logprob[row] = (float)log(weight(sh.x) * unit / mass);
+          if (a.logprob != nullptr) a.logprob[row] = (float)(log2_64(weight(sh.x) * unit / mass) * kLn2d);
         }
         return;
       }
@@ -816,9 +928,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     }
   }
 
-  // 4 over the row: kept mass by segment, in index order. Nothing cuts: every weight counts (that of -inf
-  // is 0). A cut: vectors without a kept element cost their comparison only.
-  auto all_weights = [&](const float* x, int, double* w) { weight.template eval<EPV>(x, w); };
+  // 4 over the row: kept mass by segment, in index order (the weight of -inf is 0). Vectors without a kept
+  // element cost their comparison only.
+  const Weight weight = base.fresh();
   auto kept_weights = [&](const float* x, int col0, double* w) {
     float top = x[0];
 #pragma unroll
@@ -828,12 +940,16 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     if (__ballot(top >= cut.x) == 0ull) return;
     weight.template eval<EPV>(x, w);
 #pragma unroll
-    for (int e = 0; e < EPV; ++e)
-      w[e] = x[e] > cut.x || (x[e] == cut.x && col0 + e <= cut.col) ? w[e] : 0.0;
+    for (int e = 0; e < EPV; ++e) w[e] = kept(x[e], col0 + e) ? w[e] : 0.0;
   };
-  const bool whole_row = cut.x == -INFINITY;
-  if (whole_row) segment_sums<T, THREADS, G>(rv, nseg, all_weights, sh);
-  else segment_sums<T, THREADS, G>(rv, nseg, kept_weights, sh);
+  if (!whole) {
+    auto kept_sum = [&](const float* x, int col0) {
+      double w[EPV];
+      kept_weights(x, col0, w);
+      return total_of(w);
+    };
+    segment_sums<T, THREADS, G>(rv, nseg, kept_sum, sh);
+  }
   double mine = 0.0;
   for (int i = tid; i < nseg; i += THREADS) mine += sh.seg[i];
   const double mass = block_reduce64<NW, Sum64>(mine, sh.red);
@@ -841,7 +957,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   const int col = pick<T, THREADS, G>(rv, nseg, u * mass, kept_weights, sh, &w);
   if (tid == 0) {
     a.token[row] = col;
-    if (a.logprob != nullptr) a.logprob[row] = (float)log(w / mass);
+    if (a.logprob != nullptr) a.logprob[row] = (float)(log2_64(w / mass) * kLn2d);
   }
 }
 
@@ -850,9 +966,11 @@ void launch(const void* logits, const SampleArgs& a, int64_t n, hipStream_t st) 
   const int64_t nvec = a.v / Elem<T>::kVec + 2;
 #define GO(TH, UN, G) FM_LAUNCH((sample_kernel<T, TH, UN, G>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
   // a segment for every wave at least
+  // Rows for which there is a compute unit each: all of its waves. More: half-size workgroups, two rows a
+  // unit in different phases ([1024,32000] bf16 top-p 0.9: 90 us with the large ones, 62 with these).
   if (nvec <= 1024) GO(256, 4, 1);
-  else if (nvec <= 4096) GO(1024, 4, 1);
-  else GO(1024, 4, 4);
+  else if (n <= fm_host::num_cus()) GO(1024, 4, 4);
+  else GO(512, 4, 4);
 #undef GO
 }
 
