@@ -468,6 +468,30 @@ def test_produced_lists_train_a_head():
 
 
 @gpu
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_small_bucket_losses_keep_their_digits(dt):
+    """The unlisted columns hold nearly all mass, listed ones have twice the student's probability: a
+    loss of 1e-4 that is a difference of terms of size 1. With d_r, d_l the relative errors of the two
+    running sums the loss is off by (p_r - q_r) d_r + p_l d_l, and |p_r - q_r| = p_l. At 2048 columns a
+    thread adds 8 weights or 16: arguments below 16 in base 2 are rounded by 2^-21 (3.3e-7 of the
+    weight), the exponential by 2^-23, a rescale by 2^-23, at most 16 adds by 2^-24 each: 1.6e-6. The
+    scale's own rounding, 2^-24, shifts sum (q - p) z by less than 2 * 16 * 2^-24 * p_l. Together below
+    2 * 1.6e-6 * p_l + 2e-6 * p_l, and the fp32 result's 2^-24.
+    """
+    n, v, k, T = 64, 2048, 4, 2.0
+    g = torch.Generator().manual_seed(5)
+    s = (torch.randn(n, v, generator=g) * 1.5).to(dt)
+    p = torch.softmax(s.double() / T, 1)
+    pl, idx = p.topk(k, dim=1, largest=False)
+    q = (2 * pl).float()
+    ref = O.kl_topk(s, idx, q, None, True, "bucket", T)[0]
+    got = fm.kernels.kl_div_topk(*to_dev(s, idx, q), probs=True, tail="bucket", temperature=T, reduction="none")
+    tol = 5.2e-6 * pl.sum(1) + ref.abs() * 2.0 ** -23
+    err = (got.double().cpu() - ref).abs()
+    assert (err <= tol).all(), (err / tol).max()
+
+
+@gpu
 def test_another_device_than_the_current_one_is_refused_or_served():
     s, idx, t, _ = make(2, 50, 3)
     with pytest.raises(ValueError):
