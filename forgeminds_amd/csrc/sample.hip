@@ -88,6 +88,14 @@ struct RowView {
   __device__ __forceinline__ u32x4 load_whole(int c) const {
     return *(const __attribute__((address_space(1))) u32x4*)(reinterpret_cast<const char*>(base) + (uint32_t)c * 16u);
   }
+  // vectors c, c + STRIDE, ...; where one is not whole, some other that is (or nothing, in a row that has none)
+  template <int STRIDE, int N>
+  __device__ __forceinline__ void load_some(int c, u32x4 (&raw)[N]) const {
+    if (w0 < w1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = load_whole(clamp(c + i * STRIDE));
+    }
+  }
   __device__ __forceinline__ u32x4 load(int c) const { return whole(c) ? load_whole(c) : partial(c); }
 };
 
@@ -98,19 +106,15 @@ __device__ __forceinline__ float uniform(float v) {
 }
 __device__ __forceinline__ double uniform(double v) { return readlane64(v, 0); }
 
-// the first element of a vector, which moves on by one
+// element e of a vector
 template <typename T>
-__device__ __forceinline__ float pop_element(u32x4& r) {
+__device__ __forceinline__ float element(const u32x4& r, int e) {
+  constexpr int per = 4 / sizeof(T);             // elements a register
+  const int i = e / per;
+  const uint32_t lo = i & 1 ? r.y : r.x, hi = i & 1 ? r.w : r.z;
+  u32x4 one = {(i & 2 ? hi : lo) >> (e % per * 16), 0u, 0u, 0u};
   float x[Elem<T>::kVec];
-  Elem<T>::unpack(r, x);
-  if constexpr (sizeof(T) == 4) {
-    r.x = r.y; r.y = r.z; r.z = r.w;
-  } else {
-    r.x = __builtin_amdgcn_alignbit(r.y, r.x, 16);
-    r.y = __builtin_amdgcn_alignbit(r.z, r.y, 16);
-    r.z = __builtin_amdgcn_alignbit(r.w, r.z, 16);
-    r.w >>= 16;
-  }
+  Elem<T>::unpack(one, x);
   return x[0];
 }
 
@@ -256,20 +260,22 @@ __device__ __forceinline__ int find_running(F entry, int n, double target, Sampl
   return found;
 }
 
-// fn(vector, its index) for the vectors of the row, UN loads of a thread in flight.
+// fn(vector, its index) for the vectors of the row, UN loads of a thread in flight while UN vectors are
+// worked on.
 template <typename T, int THREADS, int UN, typename F>
 __device__ __forceinline__ void each_vector(const RowView<T>& rv, F fn) {
-  const bool any = rv.w0 < rv.w1;
-  for (int c0 = thread_here(); c0 < rv.nvec; c0 += THREADS * UN) {
+  const int tid = thread_here();
+  u32x4 next[UN];
+  rv.template load_some<THREADS, UN>(tid, next);
+  for (int c0 = tid; c0 < rv.nvec; c0 += THREADS * UN) {
     u32x4 raw[UN];
-    if (any) {
 #pragma unroll
-      for (int i = 0; i < UN; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * THREADS));
-    }
+    for (int i = 0; i < UN; ++i) raw[i] = next[i];
+    rv.template load_some<THREADS, UN>(c0 + THREADS * UN, next);
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
       const int c = c0 + i * THREADS;
-      if (any) touch_whole(raw[i]);
+      touch_whole(raw[i]);
       if (c < rv.nvec) {
         if (!rv.whole(c)) raw[i] = rv.partial(c);
         fn(raw[i], c);
@@ -310,25 +316,28 @@ __device__ __forceinline__ double block_weights(const RowView<T>& rv, int block,
   return mine;
 }
 
-// The token among the segments whose weights are in sh.seg (nseg of them): the first column whose
-// running weight exceeds `target`. weights_of(x, col0, w) gives the weights of a vector. Rounding may leave
-// the target at the very end: then the last column with a weight. Returns the column; *w its weight.
-template <typename T, int THREADS, int G, typename F>
-__device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double target, F weights_of,
-                                    SampleShared<THREADS>& sh, double* w) {
+// The first column whose running weight exceeds `target`, from the weights of the nseg segments:
+// weights_of(x, col0, w) gives those of a vector. Rounding may leave the target at the very end: then the
+// last column with a weight. Returns the column; *w is its weight, *seg its segment, *ahead the weight in
+// front of that.
+template <typename T, int THREADS, int G, typename E, typename F>
+__device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, E entry, double target, F weights_of,
+                                    SampleShared<THREADS>& sh, double* w, int* seg, double* ahead) {
   constexpr int EPV = Elem<T>::kVec;
   static_assert(G <= THREADS / 64, "a wave per block of the segment");
   double before;
-  int s = find_running<THREADS, true>([&](int i) { return sh.seg[i]; }, nseg, target, sh, &before);
+  int s = find_running<THREADS, true>(entry, nseg, target, sh, &before);
   const bool end = s == nseg;
   if (end) {          // the last segment with a weight
     if (threadIdx.x == 0) sh.at = 0;
     __syncthreads();
-    for (int i = thread_here(); i < nseg; i += THREADS) if (sh.seg[i] > 0.0) atomicMax(&sh.at, i);
+    for (int i = thread_here(); i < nseg; i += THREADS) if (entry(i) > 0.0) atomicMax(&sh.at, i);
     __syncthreads();
-    s = sh.at;
+    s = uniform(sh.at);
     __syncthreads();
   }
+  *seg = s;
+  *ahead = before;
   // its blocks, a wave each
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   double wt[EPV], mine = 0.0, incl = 0.0;
@@ -377,36 +386,31 @@ __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, double targe
   return col;
 }
 
-// Segment sums over the row into sh.seg; sum_of(x, col0) is what a vector adds.
-template <typename T, int THREADS, int G, typename F>
-__device__ __forceinline__ void segment_sums(const RowView<T>& rv, int nseg, F sum_of, SampleShared<THREADS>& sh) {
-  constexpr int EPV = Elem<T>::kVec;
-  __syncthreads();
-  const bool any = rv.w0 < rv.w1;
+// fn(vector, its index) for the vectors of each segment, a wave a segment, and done(segment) behind them;
+// the next segment's loads are in flight meanwhile.
+template <typename T, int THREADS, int G, typename F, typename D>
+__device__ __forceinline__ void each_segment(const RowView<T>& rv, int nseg, F fn, D done) {
   const int tid = thread_here();
-  for (int s = tid >> 6; s < nseg; s += THREADS / 64) {
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  u32x4 next[G];
+  rv.template load_some<64, G>(wave * seg_vecs(G) + (tid & 63), next);
+  for (int s = wave; s < nseg; s += THREADS / 64) {
     const int c0 = s * seg_vecs(G) + (tid & 63);
     u32x4 raw[G];
-    if (any) {
 #pragma unroll
-      for (int i = 0; i < G; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * 64));
-    }
-    double mine = 0.0;
+    for (int i = 0; i < G; ++i) raw[i] = next[i];
+    rv.template load_some<64, G>(c0 + THREADS * G, next);
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const int c = c0 + i * 64;
-      if (any) touch_whole(raw[i]);
+      touch_whole(raw[i]);
       if (c < rv.nvec) {
         if (!rv.whole(c)) raw[i] = rv.partial(c);
-        float x[EPV];
-        Elem<T>::unpack(raw[i], x);
-        mine += sum_of(x, rv.col0(c));
+        fn(raw[i], c);
       }
     }
-    mine = wave_sum64(mine);
-    if ((tid & 63) == 0) sh.seg[s] = mine;
+    done(s);
   }
-  __syncthreads();
 }
 
 // Search by the bits of the value, over the row: the key among [lo, hi] at which the running amount, in
@@ -468,23 +472,32 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
 template <typename T, int THREADS, int G>
 __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x0, double c, SampleShared<THREADS>& sh) {
   constexpr int EPV = Elem<T>::kVec;
-  auto equal = [&](const float* x, int, double* w) {
+  auto equal = [&](float* x, int, double* w) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < EPV; ++e) w[e] = x[e] == x0 ? 1.0 : 0.0;
   };
-  auto equal_count = [&](const float* x, int) {
-    int n = 0;
+  int count = 0;
+  __syncthreads();
+  each_segment<T, THREADS, G>(rv, nseg,
+      [&](const u32x4& r, int) {
+        float x[EPV];
+        Elem<T>::unpack(r, x);
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) n += x[e] == x0 ? 1 : 0;
-    return (double)n;
-  };
-  segment_sums<T, THREADS, G>(rv, nseg, equal_count, sh);
+        for (int e = 0; e < EPV; ++e) count += x[e] == x0 ? 1 : 0;
+      },
+      [&](int s) {
+        const float all = wave_sum((float)count);
+        if ((threadIdx.x & 63) == 0) sh.seg[s] = (double)all;
+        count = 0;
+      });
+  __syncthreads();
   double mine = 0.0;
   for (int i = thread_here(); i < nseg; i += THREADS) mine += sh.seg[i];
   const double all = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
   if (c >= all) return 0x7fffffff;
-  double w;
-  return pick<T, THREADS, G>(rv, nseg, c - 0.5, equal, sh, &w);
+  double w, before;
+  int s;
+  return pick<T, THREADS, G>(rv, nseg, [&](int i) { return sh.seg[i]; }, c - 0.5, equal, sh, &w, &s, &before);
 }
 
 // sh.h.step[0 .. n) in descending order (n <= kStep), by the workgroup
@@ -552,18 +565,19 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   if (whole) {
     // Nothing cuts: one sweep, each segment's weights against its own maximum, brought together below.
     const double c = kLog2ed / (double)T_;
-    const bool any = rv.w0 < rv.w1;
-    for (int s = tid >> 6; s < nseg; s += NW) {
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    u32x4 next[G];
+    rv.template load_some<64, G>(wave * seg_vecs(G) + (tid & 63), next);
+    for (int s = wave; s < nseg; s += NW) {
       const int c0 = s * seg_vecs(G) + (tid & 63);
       u32x4 raw[G];
-      if (any) {
 #pragma unroll
-        for (int i = 0; i < G; ++i) raw[i] = rv.load_whole(rv.clamp(c0 + i * 64));
-      }
+      for (int i = 0; i < G; ++i) raw[i] = next[i];
+      rv.template load_some<64, G>(c0 + THREADS * G, next);
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        if (any) touch_whole(raw[i]);
+        touch_whole(raw[i]);
         if (c0 + i * 64 < rv.nvec) {
           if (!rv.whole(c0 + i * 64)) raw[i] = rv.partial(c0 + i * 64);
           float x[EPV];
@@ -600,7 +614,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   } else {
     // 1: the maximum; NaN propagates
     float mx = -INFINITY;
-    each_vector<T, THREADS, 8>(rv, [&](const u32x4& r, int) {
+    each_vector<T, THREADS, 4>(rv, [&](const u32x4& r, int) {
       float x[EPV];
       Elem<T>::unpack(r, x);
 #pragma unroll
@@ -651,6 +665,18 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   const Weight base((double)m, uniform(kLog2ed / (double)T_));
   Cut cut{-INFINITY, -1};           // -inf itself is never kept
   auto kept = [&](float x, int col) { return x > cut.x || (x == cut.x && col <= cut.col); };
+  // a vector's elements that are cut become -inf: one comparison each but in the vector of cut.col itself
+  auto mask = [&](float* x, int col0) __attribute__((always_inline)) {
+    const float from = col0 + EPV - 1 <= cut.col ? cut.x : float_of_key(key_of(cut.x) + 1u);
+    if (col0 <= cut.col && cut.col < col0 + EPV - 1) {
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) x[e] = kept(x[e], col0 + e) ? x[e] : -INFINITY;
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) x[e] = x[e] >= from ? x[e] : -INFINITY;
+    }
+  };
+  double ties = 0.0;                // > 0: so many of the elements equal to cut.x stay, and cut.col is not known
   if (!whole) {
     float x_min = -INFINITY;          // min-p: the least value with a weight of min_p
     if (use_m) {
@@ -677,6 +703,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       per = (float)(kBins - 2) / range;
       if (!(per <= 1e30f)) per = 1e30f;
     };
+    // What lies further below the maximum than T log(n / (1 - p)) has less than 1 - p of the mass of n
+    // elements: top-p cuts above that.
+    auto reach = [&](int n) { return T_ * (0.6931472f * fast_log2((float)n / fmaxf(1.f - p, 5.9604645e-8f)) + 0.01f); };
     auto step_of = [&](float x) { return (m - x) * per; };       // grows as x falls; never NaN
 
     // 2: the list of candidates -- those not below `bound`, or (by_step) those down to the end of the step
@@ -684,55 +713,87 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     float bound = x_min;
     bool listed = false;
     int n = 0, nb = 0;
-    auto gather = [&](bool by_step, float lo, float hi) {
+    // `entry` of the lanes `who` behind what the waves before this one put there; false past the end
+    auto put = [&](int& count, unsigned long long* to, int room, unsigned long long who, bool mine, unsigned long long entry) __attribute__((always_inline)) {
+      int base = 0;
+      const int first = __builtin_ctzll(who);
+      if ((threadIdx.x & 63) == first) base = atomicAdd(&count, (int)__builtin_popcountll(who));
+      base = __builtin_amdgcn_readlane(base, first);
+      const int at = base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+      if (mine && at < room) to[at] = entry;
+      return base + (int)__builtin_popcountll(who) <= room;
+    };
+    // (full, over: known beforehand to hold more than there is room for)
+    auto gather = [&](bool by_step, float lo, float hi, bool full, bool over) __attribute__((always_inline)) {
       const bool restricted = cut.x > -INFINITY;
       __syncthreads();
-      if (tid == 0) { sh.count = 0; sh.at = 0; sh.klo = 0xFFFFFFFFu; sh.khi = 0u; }
+      if (tid == 0) {
+        sh.count = full ? kList + 1 : 0;
+        sh.at = over ? kStep + 1 : 0;
+        sh.klo = 0xFFFFFFFFu;
+        sh.khi = 0u;
+      }
       __syncthreads();
-      bool full = false;
-      uint32_t klo = 0xFFFFFFFFu, khi = 0u;      // keys of the step
+      float step_min = INFINITY, step_max = -INFINITY;
       each([&](const u32x4& r, int c) {
+        if (full && !by_step) return;
         float x[EPV];
         Elem<T>::unpack(r, x);
-        float top = x[0];
+        if (restricted) mask(x, rv.col0(c));
+        if (!full) {
+          float top = x[0];
 #pragma unroll
-        for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
-        if (__ballot(by_step ? step_of(top) < hi : top >= bound) == 0ull) return;
-        if (full && !by_step) return;
-        u32x4 rest = r;
-#pragma unroll 1
-        for (int e = 0; e < EPV; ++e) {
-          const float xe = pop_element<T>(rest);
-          const float y = step_of(xe);
-          const bool in_step = y >= lo && y < hi;
-          // (a full list takes no more, but the step still does)
-          bool cand = by_step ? (full ? in_step : y < hi) : (xe >= bound && xe > -INFINITY);
-          if (restricted) cand = cand && kept(xe, rv.col0(c) + e);
-          const unsigned long long who = __ballot(cand);
-          if (who == 0ull) continue;
-          const uint32_t key = key_of(xe);
-          const unsigned long long entry = ((unsigned long long)key << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
-          if (!full) {
-            const int count = __builtin_popcountll(who);
-            int base = 0;
-            const int first = __builtin_ctzll(who);
-            if ((tid & 63) == first) base = atomicAdd(&sh.count, count);
-            base = __builtin_amdgcn_readlane(base, first);
-            const int at = base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
-            if (cand && at < kList) sh.h.list[at] = entry;
-            full = base + count > kList;
+          for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+          if (__ballot(by_step ? step_of(top) < hi : top >= bound) == 0ull) return;
+        }
+        if (full && over) {          // only the ends of the step's values are wanted
+          float low = INFINITY, high = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < EPV; ++e) {
+            const float y = step_of(x[e]);
+            const bool in = y >= lo && y < hi;
+            low = __builtin_elementwise_minimum(low, in ? x[e] : INFINITY);
+            high = __builtin_elementwise_maximum(high, in ? x[e] : -INFINITY);
           }
-          if (by_step && cand && in_step) {
-            klo = key < klo ? key : klo;
-            khi = key > khi ? key : khi;
-            if (sh.at <= kStep) {       // counted past the end once: the step is too long
-              const int at = atomicAdd(&sh.at, 1);
-              if (at < kStep) sh.h.step[at] = entry;
-            }
+          step_min = __builtin_elementwise_minimum(step_min, low);
+          step_max = __builtin_elementwise_maximum(step_max, high);
+          return;
+        }
+        uint32_t todo = 0u, in_step = 0u;       // a bit per element
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) {
+          if (by_step) {
+            const float y = step_of(x[e]);
+            const bool in = y >= lo && y < hi;
+            step_min = __builtin_elementwise_minimum(step_min, in ? x[e] : INFINITY);
+            step_max = __builtin_elementwise_maximum(step_max, in ? x[e] : -INFINITY);
+            in_step |= in ? 1u << e : 0u;
+            todo |= y < hi ? 1u << e : 0u;
+          } else {
+            todo |= x[e] >= bound && x[e] > -INFINITY ? 1u << e : 0u;
+          }
+        }
+        if (full) todo = in_step;      // a full list takes no more, but the step still does
+        while (true) {
+          const unsigned long long who = __ballot(todo != 0u);
+          if (who == 0ull) break;
+          const bool mine = todo != 0u;
+          const int e = mine ? __builtin_ctz(todo) : 0;
+          todo &= todo - 1u;
+          const unsigned long long entry =
+              ((unsigned long long)key_of(element<T>(r, e)) << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
+          if (!full) full = !put(sh.count, sh.h.list, kList, who, mine, entry);
+          if (by_step && !over) {
+            const bool in = mine && (in_step >> e & 1u) != 0u;
+            const unsigned long long ins = __ballot(in);
+            if (ins != 0ull) over = !put(sh.at, sh.h.step, kStep, ins, in, entry);
           }
         }
       });
-      if (by_step && klo <= khi) { atomicMin(&sh.klo, klo); atomicMax(&sh.khi, khi); }
+      if (by_step && step_min <= step_max) {
+        atomicMin(&sh.klo, key_of(step_min));
+        atomicMax(&sh.khi, key_of(step_max));
+      }
       __syncthreads();
       nb = uniform(sh.at);
       n = uniform(sh.count);
@@ -747,17 +808,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       const float range = m - bound;
       steps_over(range < INFINITY ? range : 24.f * T_);
     } else {
-      steps_over((p <= 0.99f ? 12.f : 24.f) * T_);
+      steps_over(reach(a.v));
     }
     // (with top-p alone there is no bound to list by)
-    if (use_k ? bound > -INFINITY || a.v <= kList : !use_p) gather(false, 0.f, 0.f);
-    auto settle = [&](auto by_count) {
+    if (use_k ? bound > -INFINITY || a.v <= kList : !use_p) gather(false, 0.f, 0.f, false, false);
+    auto settle = [&](auto by_count) __attribute__((always_inline)) {
       constexpr bool count = decltype(by_count)::value;
       const int tid = thread_here();
       if (count && listed && n < k) return;         // all of them stay
       const bool by_list = listed;
       const bool restricted = cut.x > -INFINITY;
-      if (!by_list && use_k && !count) steps_over(24.f * T_);
+      if (!by_list && use_k && !count) steps_over(reach(k));
       __syncthreads();
       for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
       __syncthreads();
@@ -781,10 +842,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         each([&](const u32x4& r, int c) {
           float x[EPV];
           Elem<T>::unpack(r, x);
-          if (restricted) {
-#pragma unroll
-            for (int e = 0; e < EPV; ++e) x[e] = kept(x[e], rv.col0(c) + e) ? x[e] : -INFINITY;
-          }
+          if (restricted) mask(x, rv.col0(c));
           if (count) {
 #pragma unroll
             for (int e = 0; e < EPV; ++e) {
@@ -827,7 +885,18 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         __syncthreads();
         nb = uniform(sh.at);
       } else if (b < kBins) {
-        gather(true, (float)b, (float)(b + 1));
+        // How many there are at least, from the mass and the largest weight of each step: rows whose list or
+        // step is sure to overflow spare the way there.
+        float most = 0.f, in_b = 0.f;
+        for (int i = tid; i <= b; i += THREADS) {
+          const float least = count ? (float)sh.h.bins[i]
+                                    : (float)sh.h.bins[i] * fast_exp2((float)i / per * (float)base.c - (float)fx);
+          most += least;
+          if (i == b) in_b = least;
+        }
+        most = (float)block_reduce64<NW, Sum64>((double)most, sh.red);
+        in_b = (float)block_reduce64<NW, Sum64>((double)in_b, sh.red);
+        gather(true, (float)b, (float)(b + 1), uniform(most) > 1.01f * kList, uniform(in_b) > 1.01f * kStep);
       }
       if (b < kBins && nb <= kStep) {
         sort_step<THREADS>(sh, nb);
@@ -854,14 +923,22 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       // the r-th of the equal ones stays iff above + (r - 1) * weight < goal
       double need = each_w > 0.0 ? ceil((goal - (double)above) / each_w) : 1.0;
       need = uniform(need >= 1.0 ? need : 1.0);
-      int col = x > -INFINITY ? nth_equal<T, THREADS, G>(rv, nseg, x, need, sh) : -1;
-      if (x == cut.x && cut.col < col) col = cut.col;
-      if (x >= cut.x) cut = Cut{x, col};
+      if (!count || !use_p) {       // the last cut: the sweep below counts the equal ones by the way
+        listed = false;
+        if (x > cut.x) {
+          cut = Cut{x, -1};
+          ties = need;
+          return;
+        }
+      }
+      const int col = x >= cut.x && x > -INFINITY ? nth_equal<T, THREADS, G>(rv, nseg, x, need, sh) : -1;
+      if (x > cut.x || (x == cut.x && col < cut.col)) cut = Cut{x, col};
       listed = listed && b < kBins;
     };
     if (use_k) settle(std::true_type{});
     if (use_p) settle(std::false_type{});
     if (x_min > cut.x) {       // every value equal to the bound stays
+      ties = 0.0;
       cut.x = x_min;
       cut.col = 0x7fffffff;
     }
@@ -931,30 +1008,65 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   // 4 over the row: kept mass by segment, in index order (the weight of -inf is 0). Vectors without a kept
   // element cost their comparison only.
   const Weight weight = base.fresh();
-  auto kept_weights = [&](const float* x, int col0, double* w) {
+  auto kept_weights = [&](float* x, int col0, double* w) __attribute__((always_inline)) {
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
 #pragma unroll
     for (int e = 0; e < EPV; ++e) w[e] = 0.0;
     if (__ballot(top >= cut.x) == 0ull) return;
+    mask(x, col0);
     weight.template eval<EPV>(x, w);
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) w[e] = kept(x[e], col0 + e) ? w[e] : 0.0;
   };
+  auto equal = [&](float* x, int, double* w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) w[e] = x[e] == cut.x ? 1.0 : 0.0;
+  };
+  int at_seg;
+  double w, ahead;
   if (!whole) {
-    auto kept_sum = [&](const float* x, int col0) {
-      double w[EPV];
-      kept_weights(x, col0, w);
-      return total_of(w);
-    };
-    segment_sums<T, THREADS, G>(rv, nseg, kept_sum, sh);
+    __syncthreads();
+    double mine = 0.0;
+    int equals = 0;
+    each_segment<T, THREADS, G>(rv, nseg,
+        [&](const u32x4& r, int c) {
+          float x[EPV];
+          Elem<T>::unpack(r, x);
+          if (ties > 0.0) {
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) equals += x[e] == cut.x ? 1 : 0;
+          }
+          double w[EPV];
+          kept_weights(x, rv.col0(c), w);
+          mine += total_of(w);
+        },
+        [&](int s) {
+          mine = wave_sum64(mine);
+          const float all_equals = ties > 0.0 ? wave_sum((float)equals) : 0.f;
+          if ((tid & 63) == 0) { sh.seg[s] = mine; sh.segm[s] = all_equals; }
+          mine = 0.0;
+          equals = 0;
+        });
+    __syncthreads();
+    if (ties > 0.0) {
+      double mine = 0.0;
+      for (int i = tid; i < nseg; i += THREADS) mine += (double)sh.segm[i];
+      int s_cut = nseg;
+      double before = 0.0;
+      cut.col = 0x7fffffff;
+      if (ties < uniform(block_reduce64<NW, Sum64>(mine, sh.red)))
+        cut.col = pick<T, THREADS, G>(rv, nseg, [&](int i) { return (double)sh.segm[i]; }, ties - 0.5, equal, sh, &w, &s_cut, &before);
+      const double each_w = weight(cut.x);
+      __syncthreads();
+      for (int i = tid; i < nseg; i += THREADS)
+        sh.seg[i] += each_w * (i < s_cut ? (double)sh.segm[i] : i == s_cut ? ties - before : 0.0);
+      __syncthreads();
+    }
   }
   double mine = 0.0;
   for (int i = tid; i < nseg; i += THREADS) mine += sh.seg[i];
   const double mass = block_reduce64<NW, Sum64>(mine, sh.red);
-  double w;
-  const int col = pick<T, THREADS, G>(rv, nseg, u * mass, kept_weights, sh, &w);
+  const int col = pick<T, THREADS, G>(rv, nseg, [&](int i) { return sh.seg[i]; }, u * mass, kept_weights, sh, &w, &at_seg, &ahead);
   if (tid == 0) {
     a.token[row] = col;
     if (a.logprob != nullptr) a.logprob[row] = (float)(log2_64(w / mass) * kLn2d);
