@@ -492,6 +492,32 @@ def test_small_bucket_losses_keep_their_digits(dt):
 
 
 @gpu
+def test_rows_past_two_to_the_31_elements():
+    # rows repeat every 64: the same loss and gradient wherever they stand
+    n, v, k, m = 16800, 128256, 32, 64
+    assert n * v > 2 ** 31
+    g = torch.Generator().manual_seed(8)
+    s = (2 * torch.randn(m, v, generator=g)).to(BF16)
+    t, idx = (s.float() + 0.5 * torch.randn(m, v, generator=g)).topk(k)
+    lse = torch.logsumexp(t, 1) + 0.3
+    rows = torch.arange(n, device=DEV) % m
+    sd, idx, t, lse = to_dev(s, idx, t, lse)
+    big = sd.repeat((n + m - 1) // m, 1)[:n].requires_grad_(True)
+    for reduction in ("none", "sum"):
+        big.grad = None
+        loss = fm.kernels.kl_div_topk(big, idx[rows], t[rows], teacher_lse=lse[rows], tail="bucket", reduction=reduction)
+        loss.sum().backward()
+        small = sd.clone().requires_grad_(True)
+        want = fm.kernels.kl_div_topk(small, idx, t, teacher_lse=lse, tail="bucket", reduction="none")
+        want.sum().backward()
+        if reduction == "none":
+            assert (loss - want[rows]).abs().max() <= 2.0 ** -20 * want.abs().max()
+        for at in (0, 37, 2 ** 31 // v - 1, 2 ** 31 // v, 2 ** 31 // v + 1, n - 1):
+            a, b = big.grad[at].float(), small.grad[at % m].float()
+            assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 1e-30).all(), (reduction, at)
+
+
+@gpu
 def test_another_device_than_the_current_one_is_refused_or_served():
     s, idx, t, _ = make(2, 50, 3)
     with pytest.raises(ValueError):

@@ -274,6 +274,56 @@ def test_a_row_does_not_depend_on_its_batch_stream_or_replay():
 
 
 @gpu
+@pytest.mark.parametrize("kw", [dict(top_p=0.5), dict(top_p=0.99), dict(top_p=0.9999), dict(top_k=2000), dict(top_k=30000),
+                                dict(top_k=6000, top_p=0.9), dict(top_k=900, top_p=0.99), dict(min_p=0.3), dict(min_p=1e-6),
+                                dict(top_p=0.9, min_p=0.2), dict(top_k=50, min_p=0.9), dict(temperature=0.3, top_p=0.95)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_flat_rows_and_long_lists(dt, kw):
+    # steps with thousands of different values, lists that overflow, cuts deep in the row, candidates side
+    # by side at one end, rows with fewer values left than top_k asks for
+    g = torch.Generator().manual_seed(12)
+    v = 60001
+    x = torch.stack([0.02 * torch.randn(v, generator=g), 0.5 * torch.randn(v, generator=g) + 14, 3 * torch.randn(v, generator=g),
+                     torch.linspace(9, -9, v), torch.linspace(-3, 3, v).square(), torch.full((v,), -float("inf"))])
+    x[5, 11::29] = torch.randn(len(range(11, v, 29)), generator=g)
+    x = x.to(dt)
+    u = torch.tensor([.41, .97, .03, .55, .5, .76])
+    tok, lp = fm.kernels.sample_tokens(x.to(DEV), u.to(DEV), **kw)
+    check(x, u, tok, lp, **kw)
+
+
+@gpu
+@pytest.mark.parametrize("n", [2, 300])
+@pytest.mark.parametrize("dt,v", [(F32, 2 ** 20), (BF16, 2 ** 20), (F16, 2 ** 20 - 3)])
+def test_the_longest_rows(dt, v, n):
+    # one element off a 16-byte border, more rows than compute units among the counts; the rows past the
+    # second repeat it
+    x, u = zipf(2, v, 21, dt)
+    flat = torch.full((n * v + 1,), float("nan"), device=DEV, dtype=dt)
+    xd = flat[1:].view(n, v)
+    xd[0], xd[1:] = x[0].to(DEV), x[1].to(DEV)
+    ud = torch.cat([u[:1], u[1:].expand(n - 1)]).to(DEV)
+    for kw in (dict(), dict(top_p=0.9), dict(top_k=40), dict(top_k=100000, top_p=0.999), dict(min_p=0.001)):
+        tok, lp = fm.kernels.sample_tokens(xd, ud, **kw)
+        assert (tok[1:] == tok[1]).all() and (lp[1:] == lp[1]).all()
+        check(x, u, tok[:2], lp[:2], **kw)
+
+
+@gpu
+def test_rows_past_two_to_the_31_elements():
+    n, v = 16800, 128256
+    assert n * v > 2 ** 31
+    x, u = zipf(64, v, 31, BF16)
+    xd = x.to(DEV).repeat((n + 63) // 64, 1)[:n]
+    ud = u.to(DEV).repeat((n + 63) // 64)[:n]
+    for kw in (dict(top_k=50, top_p=0.9), dict(top_p=0.9)):
+        tok, lp = fm.kernels.sample_tokens(xd, ud, **kw)
+        want = fm.kernels.sample_tokens(xd[:64], ud[:64], **kw)
+        rows = torch.arange(n, device=DEV) % 64
+        assert torch.equal(tok, want[0][rows]) and torch.equal(lp, want[1][rows])
+
+
+@gpu
 def test_sampled_listed_and_trained_on():
     # on-policy distillation: the student's token, the teacher's list at that position, the loss
     g = torch.Generator().manual_seed(2)
