@@ -767,8 +767,9 @@ int check(const char* what, int64_t n, int64_t v, int k, int dtype, int index_bi
   FM_CHECK_ARG(kind == FM_TEACHER_LOGITS || kind == FM_TEACHER_PROBS, "%s: bad teacher_kind %d", what, kind);
   FM_CHECK_ARG(tail == FM_TAIL_RENORM || tail == FM_TAIL_DROP || tail == FM_TAIL_BUCKET, "%s: bad tail %d", what, tail);
   FM_CHECK_ARG(temperature > 0.0 && temperature <= 3.0e38, "%s: temperature must be positive and finite", what);
-  if (n > 0x7fffffffLL || v > 0x7fffffffLL || k > kMaxList) {
-    fm_host::set_error("%s: n and v must be below 2^31 and k at most %d", what, kMaxList);
+  // (a launch has less than 2^32 threads, and a row up to 1024; offsets inside a row are 32 bits of bytes)
+  if (n >= (1LL << 22) || v >= (1LL << 30) || k > kMaxList) {
+    fm_host::set_error("%s: n must be below 2^22, v below 2^30 and k at most %d", what, kMaxList);
     return FM_ERR_UNSUPPORTED;
   }
   return FM_OK;
@@ -835,7 +836,7 @@ void launch_bwd(const void* student, const ListArgs& a, const float* stats, cons
 #define GO(TH, UN)                                                                                            \
   do {                                                                                                        \
     int64_t chunks = (nvec + TH * UN - 1) / (TH * UN);                                                        \
-    if (chunks < 1 || n * chunks > 0x7fffffffLL) chunks = 1;                                                  \
+    if (chunks < 1 || n * chunks >= (1LL << 32) / TH) chunks = 1;                                                \
     FM_LAUNCH((kl_topk_bwd_kernel<T, TH, KCAP, UN>), dim3((unsigned)(n * chunks)), dim3(TH), 0, st,           \
               static_cast<const T*>(student), a, stats, n_valid, grad_out, per_row, static_cast<T*>(dstudent), \
               v, vec_ok, (int)chunks);                                                                        \

@@ -15,14 +15,27 @@
 //   1  maximum of the row (NaN propagates)
 //   2  candidates: the elements from the maximum down to a bound at or below the cut, into a list in LDS.
 //      top-k: the waves' thread maxima vouch for k elements above the bound. min-p: its own bound. top-p
-//      alone: a histogram of the row's masses (64-bit fixed point: integer adds give the same sum in any
-//      order) over 2048 equal steps of the logit names the step that holds the cut
-//   3  the exact cut: histograms of the list narrow it to one step, whose elements are put in order
+//      alone (and a top-k whose list overflows): a histogram of the row's masses (or counts) over 2048 equal
+//      steps of the logit names the step that holds the cut; masses are 64-bit fixed point, so that the sum
+//      is the same in any order
+//   3  the exact cut: histograms of the list narrow it to one step, whose elements are put in order. A step
+//      with more elements than that is searched by the bits of the value; among equal values the cut is a
+//      count, which the last sweep turns into a column
 //   4  token: masses of the segments in index order, the segment that holds u, the token in it -- from the
-//      list, or over the row again where the list is too long (flat rows) or nothing cuts
-// Weights are computed for the candidates only, unless the mass of the whole row is asked for. Steps with
-// more elements than the ordering takes (runs of equal values) and cuts far below the maximum are searched
-// by the bits of the value, over the row.
+//      list, or over the row again where the list is too long (flat rows)
+// Where nothing cuts, one sweep does: each segment's masses against its own maximum.
+// Weights are computed for the candidates only, unless the mass of the whole row is asked for.
+//
+// What bounds it: the arithmetic of those weights, some 27 instructions an element with the histogram, on
+// the row's one compute unit; memory is far (256 rows of 128256 bf16 are 10 us of reading). Measured, bf16,
+// [1,128256]: unfiltered 28 us, min-p 15, top-k 50 25, top-p 0.9 43 (maximum 4, histogram 23, list 8, cut,
+// token and launch 8), 88 on a flat row, whose every element is kept. [256,128256]: 33, 27, 37, 58, 100.
+// [512,128256]: 55, 42, 49, 92, 167. [1024,32000]: 36, 29, 50, 65, 108. Splitting a row over workgroups
+// would divide the 23 us alone, for a second launch and partial histograms in memory: 10 us at best.
+//
+// What keeps it small counts too: the code that a call runs through fits the instruction cache (64 KB for
+// two compute units). Putting the row's two partial vectors together in place, in every sweep, made each
+// sweep 2 to 15 us longer; they stand in shared memory instead.
 #include "../../include/fm_hip_tokens.h"
 #include "fm_f64.hip.h"
 #include "fm_topk.hip.h"
@@ -260,18 +273,14 @@ __device__ __forceinline__ int find_running(F entry, int n, double target, Sampl
   return found;
 }
 
-// fn(vector, its index) for the vectors of the row, UN loads of a thread in flight while UN vectors are
-// worked on.
-template <typename T, int THREADS, int UN, typename F>
+// fn(vector, its index) for the vectors of the row, four loads of a thread in flight. (Loading the next four
+// ahead of the work gained nothing here: [512,128256] top-p 0.9 93 us with it, 92 without.)
+template <typename T, int THREADS, typename F>
 __device__ __forceinline__ void each_vector(const RowView<T>& rv, F fn) {
-  const int tid = thread_here();
-  u32x4 next[UN];
-  rv.template load_some<THREADS, UN>(tid, next);
-  for (int c0 = tid; c0 < rv.nvec; c0 += THREADS * UN) {
+  constexpr int UN = 4;
+  for (int c0 = thread_here(); c0 < rv.nvec; c0 += THREADS * UN) {
     u32x4 raw[UN];
-#pragma unroll
-    for (int i = 0; i < UN; ++i) raw[i] = next[i];
-    rv.template load_some<THREADS, UN>(c0 + THREADS * UN, next);
+    rv.template load_some<THREADS, UN>(c0, raw);
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
       const int c = c0 + i * THREADS;
@@ -286,7 +295,7 @@ __device__ __forceinline__ void each_vector(const RowView<T>& rv, F fn) {
 template <typename T, int THREADS, typename F>
 __device__ __forceinline__ void each_element(const RowView<T>& rv, F fn) {
   constexpr int EPV = Elem<T>::kVec;
-  each_vector<T, THREADS, 1>(rv, [&](const u32x4& r, int c) {
+  each_vector<T, THREADS>(rv, [&](const u32x4& r, int c) {
     float x[EPV];
     Elem<T>::unpack(r, x);
 #pragma unroll
@@ -387,7 +396,7 @@ __device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, E entry, dou
 }
 
 // fn(vector, its index) for the vectors of each segment, a wave a segment, and done(segment) behind them;
-// the next segment's loads are in flight meanwhile.
+// the next segment's loads are in flight meanwhile ([512,128256] min-p on flat rows: 94 us without, 92 with).
 template <typename T, int THREADS, int G, typename F, typename D>
 __device__ __forceinline__ void each_segment(const RowView<T>& rv, int nseg, F fn, D done) {
   const int tid = thread_here();
@@ -520,7 +529,7 @@ __device__ __forceinline__ void sort_step(SampleShared<THREADS>& sh, int n) {
   }
 }
 
-template <typename T, int THREADS, int UN, int G>
+template <typename T, int THREADS, int G>
 __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ logits, SampleArgs a) {
   constexpr int EPV = Elem<T>::kVec;
   constexpr int NW = THREADS / 64;
@@ -544,7 +553,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   if (!(p > 0.f)) p = 0.f;
   const bool use_m = min_p > 0.f;
   min_p = fminf(min_p, 1.f);
-  auto each = [&](auto fn) { each_vector<T, THREADS, UN>(rv, fn); };
+  auto each = [&](auto fn) { each_vector<T, THREADS>(rv, fn); };
   const int nseg = (rv.nvec + seg_vecs(G) - 1) / seg_vecs(G);
   auto no_row = [&]() {            // no distribution
     if (tid == 0) {
@@ -614,7 +623,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   } else {
     // 1: the maximum; NaN propagates
     float mx = -INFINITY;
-    each_vector<T, THREADS, 4>(rv, [&](const u32x4& r, int) {
+    each_vector<T, THREADS>(rv, [&](const u32x4& r, int) {
       float x[EPV];
       Elem<T>::unpack(r, x);
 #pragma unroll
@@ -1076,13 +1085,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
 template <typename T>
 void launch(const void* logits, const SampleArgs& a, int64_t n, hipStream_t st) {
   const int64_t nvec = a.v / Elem<T>::kVec + 2;
-#define GO(TH, UN, G) FM_LAUNCH((sample_kernel<T, TH, UN, G>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
-  // a segment for every wave at least
-  // Rows for which there is a compute unit each: all of its waves. More: half-size workgroups, two rows a
-  // unit in different phases ([1024,32000] bf16 top-p 0.9: 90 us with the large ones, 62 with these).
-  if (nvec <= 1024) GO(256, 4, 1);
-  else if (n <= fm_host::num_cus()) GO(1024, 4, 4);
-  else GO(512, 4, 4);
+#define GO(TH, G) FM_LAUNCH((sample_kernel<T, TH, G>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
+  // Short rows: four waves, a block of 64 vectors a segment, so that each wave has segments to sweep
+  // ([2048,8000] bf16 top-p 0.9: 70 us with 512 threads, 56 with these). Rows for which there is a compute
+  // unit each: all of its waves ([1,128256] top-p 0.9: 51 us with 512 threads, 45 with these; a short list
+  // costs 6 us more). More rows: half-size workgroups, two rows a unit in different phases ([1024,32000]
+  // top-p 0.9: 99 us with the large ones, 66 with these).
+  if (nvec <= 1024) GO(256, 1);
+  else if (n <= fm_host::num_cus()) GO(1024, 4);
+  else GO(512, 4);
 #undef GO
 }
 
@@ -1094,8 +1105,9 @@ extern "C" int fm_sample(const void* logits, const float* u, const float* temper
                          fm_stream_t stream) {
   FM_CHECK_ARG(n >= 0 && v > 0, "fm_sample: bad shape n=%lld v=%lld", (long long)n, (long long)v);
   FM_CHECK_ARG(dtype == FM_F32 || dtype == FM_F16 || dtype == FM_BF16, "fm_sample: bad dtype %d", dtype);
-  if (n > 0x7fffffffLL || v > kMaxCols) {
-    fm_host::set_error("fm_sample: n must be below 2^31 and v at most %lld", (long long)kMaxCols);
+  // (a launch has less than 2^32 threads, and a row up to 1024)
+  if (n >= (1LL << 22) || v > kMaxCols) {
+    fm_host::set_error("fm_sample: n must be below 2^22 and v at most %lld", (long long)kMaxCols);
     return FM_ERR_UNSUPPORTED;
   }
   if (n == 0) return FM_OK;

@@ -310,6 +310,9 @@ def kl_div_logits_topk(student: torch.Tensor, teacher: torch.Tensor, k: int,
 # ------------------------------------------------------------------ from a teacher's list
 #: longest list a row may have on the kernel path
 MAX_LIST = 1024
+#: the kernel path takes fewer rows than this in one call, and fewer columns
+MAX_LIST_ROWS = 1 << 22
+MAX_LIST_COLS = 1 << 30
 _TAILS = ("renorm", "drop", "bucket")
 
 
@@ -415,7 +418,8 @@ def kl_div_topk(student: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor,
     if any(t.device != student.device for t in others):
         raise ValueError("kl_div_topk: student, idx, teacher and teacher_lse must be on one device")
     temperature = float(temperature)
-    if student.numel() == 0 or idx.shape[-1] > MAX_LIST or tracing():
+    if (student.numel() == 0 or idx.shape[-1] > MAX_LIST or tracing()
+            or student.shape[-1] >= MAX_LIST_COLS or student.numel() // student.shape[-1] >= MAX_LIST_ROWS):
         _note("kl_div_topk shape")
         return fb.kl_div_topk(student, idx, teacher, teacher_lse, probs, tail, reduction, temperature)
     if not _kernel_ok(student, teacher):

@@ -19,6 +19,8 @@ from ._common import _note, fast_ok, tracing
 
 #: widest row of the kernel path; wider ones run the torch expression
 MAX_VOCAB = 1 << 20
+#: the kernel path takes fewer rows than this in one call
+MAX_ROWS = 1 << 22
 
 
 def _setting(name: str, x, lead, like: torch.Tensor, dtype):
@@ -85,7 +87,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
         token, logprob = fb.sample_tokens(x2, u1, *(c.unsqueeze(-1) for c in cols))
         return token.view(lead), logprob.view(lead)
 
-    if logits.numel() == 0 or v > MAX_VOCAB or tracing():
+    if logits.numel() == 0 or v > MAX_VOCAB or x2.shape[0] >= MAX_ROWS or tracing():
         _note("sample_tokens shape")
         return torch_path()
     if logits.numel() >= 2 ** 31 * 4:
@@ -97,4 +99,4 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     return token.view(lead), logprob.view(lead)
 
 
-__all__ = ["sample_tokens", "MAX_VOCAB"]
+__all__ = ["sample_tokens", "MAX_VOCAB", "MAX_ROWS"]

@@ -32,7 +32,8 @@ extern "C" {
  * row_loss: fp32 [n]. stats: fp32 [n, 4] for fm_kl_topk_bwd (running maximum and sum of the whole
  * row, then of its unlisted columns, base 2). loss, n_valid: fp32 device scalars; loss = sum of
  * row_loss (FM_REDUCE_SUM) or that / n_valid (FM_REDUCE_MEAN), n_valid = max(1, rows not skipped);
- * both may be NULL for FM_REDUCE_NONE, which writes neither. 1 <= k <= 1024, k may exceed v. */
+ * both may be NULL for FM_REDUCE_NONE, which writes neither. 1 <= k <= 1024, k may exceed v;
+ * n < 2^22, v < 2^30 (FM_ERR_UNSUPPORTED past those). */
 enum fm_teacher { FM_TEACHER_LOGITS = 0, FM_TEACHER_PROBS = 1 };
 enum fm_tail { FM_TAIL_RENORM = 0, FM_TAIL_DROP = 1, FM_TAIL_BUCKET = 2 };
 
@@ -75,7 +76,8 @@ int fm_kl_topk_bwd(const void* student, const void* idx, const void* teacher, co
  * NaN: off. Logits of -inf are never taken.
  * u: fp32 [n]. temperature, top_p, min_p: fp32 [n] or NULL for the number behind them for every row;
  * top_k: int32 [n] or NULL likewise. token: int64 [n]; logprob: fp32 [n] or NULL. logits may have any
- * alignment of their type. Weights and sums are held in 64 bits. v <= 2^20. */
+ * alignment of their type. Weights and sums are held in 64 bits. v <= 2^20, n < 2^22 (FM_ERR_UNSUPPORTED
+ * past those). */
 int fm_sample(const void* logits, const float* u, const float* temperature, const int32_t* top_k,
               const float* top_p, const float* min_p, float temperature0, int top_k0, float top_p0,
               float min_p0, int64_t* token, float* logprob, int64_t n, int64_t v, int dtype,

@@ -214,6 +214,7 @@ def test_declarations_exports_and_argument_validation():
             assert f(**kw) == 1, (f.__name__, kw)
             assert lib.fm_last_error()
         assert f(k=1025) == 2 and f(v=2 ** 31) == 2
+        assert f(n=2 ** 22) == 2 and f(v=2 ** 30) == 2
     assert both(red=0) == 1 and fwd(red=7) == 1 and bwd(n=0) == 0 and fwd(n=0, red=0) == 0
     # the gradient of saved stats needs a buffer of its own, and a gradient per row needs grad_out
     p = ctypes.c_void_p(64)

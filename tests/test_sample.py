@@ -178,6 +178,7 @@ def test_entry_point_validation():
     def f(n=2, v=8, dt=2, p=None):
         return lib.fm_sample(p, p, None, None, None, None, 1.0, 0, 1.0, 0.0, p, None, n, v, dt, None)
     assert f() == 1 and f(n=-1) == 1 and f(v=0) == 1 and f(dt=7) == 1 and f(v=2 ** 20 + 1) == 2 and f(n=2 ** 31) == 2
+    assert f(n=2 ** 22) == 2
     assert f(n=0) == 0 and f(p=ctypes.c_void_p(65), dt=0) == 1
 
 
@@ -307,6 +308,16 @@ def test_the_longest_rows(dt, v, n):
         tok, lp = fm.kernels.sample_tokens(xd, ud, **kw)
         assert (tok[1:] == tok[1]).all() and (lp[1:] == lp[1]).all()
         check(x, u, tok[:2], lp[:2], **kw)
+
+
+@gpu
+def test_more_rows_than_a_launch_takes():
+    n, v = 2 ** 22, 3
+    x = torch.tensor([[0.0, 3.0, 1.0]], device=DEV).repeat(n, 1)
+    u = torch.full((n,), 0.5, device=DEV)
+    for m in (n - 1, n):
+        tok, lp = fm.kernels.sample_tokens(x[:m], u[:m], top_k=1)
+        assert tok.shape == (m,) and (tok == 1).all() and (lp == 0).all()
 
 
 @gpu
