@@ -575,14 +575,10 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     // Nothing cuts: one sweep, each segment's weights against its own maximum, brought together below.
     const double c = kLog2ed / (double)T_;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    u32x4 next[G];
-    rv.template load_some<64, G>(wave * seg_vecs(G) + (tid & 63), next);
     for (int s = wave; s < nseg; s += NW) {
       const int c0 = s * seg_vecs(G) + (tid & 63);
       u32x4 raw[G];
-#pragma unroll
-      for (int i = 0; i < G; ++i) raw[i] = next[i];
-      rv.template load_some<64, G>(c0 + THREADS * G, next);
+      rv.template load_some<64, G>(c0, raw);
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
@@ -717,11 +713,13 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     auto reach = [&](int n) { return T_ * (0.6931472f * fast_log2((float)n / fmaxf(1.f - p, 5.9604645e-8f)) + 0.01f); };
     auto step_of = [&](float x) { return (m - x) * per; };       // grows as x falls; never NaN
 
-    // 2: the list of candidates -- those not below `bound`, or (by_step) those down to the end of the step
-    // [lo, hi), which is listed apart as well -- of what the cut so far keeps
+    // 2: the list of candidates
     float bound = x_min;
     bool listed = false;
     int n = 0, nb = 0;
+    auto entry_of = [&](const u32x4& r, int c, int e) __attribute__((always_inline)) {
+      return ((unsigned long long)key_of(element<T>(r, e)) << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
+    };
     // `entry` of the lanes `who` behind what the waves before this one put there; false past the end
     auto put = [&](int& count, unsigned long long* to, int room, unsigned long long who, bool mine, unsigned long long entry) __attribute__((always_inline)) {
       int base = 0;
@@ -732,81 +730,73 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       if (mine && at < room) to[at] = entry;
       return base + (int)__builtin_popcountll(who) <= room;
     };
-    // (full, over: known beforehand to hold more than there is room for)
-    auto gather = [&](bool by_step, float lo, float hi, bool full, bool over) __attribute__((always_inline)) {
+    // The list: what the cut so far keeps and is not below `bound`, or (by_step) lies in the steps before `hi`.
+    auto list_up = [&](bool by_step, float hi) __attribute__((always_inline)) {
       const bool restricted = cut.x > -INFINITY;
       __syncthreads();
-      if (tid == 0) {
-        sh.count = full ? kList + 1 : 0;
-        sh.at = over ? kStep + 1 : 0;
-        sh.klo = 0xFFFFFFFFu;
-        sh.khi = 0u;
-      }
+      if (tid == 0) sh.count = 0;
       __syncthreads();
-      float step_min = INFINITY, step_max = -INFINITY;
+      bool full = false;
       each([&](const u32x4& r, int c) {
-        if (full && !by_step) return;
+        if (full) return;
         float x[EPV];
         Elem<T>::unpack(r, x);
         if (restricted) mask(x, rv.col0(c));
-        if (!full) {
-          float top = x[0];
+        float top = x[0];
 #pragma unroll
-          for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
-          if (__ballot(by_step ? step_of(top) < hi : top >= bound) == 0ull) return;
-        }
-        if (full && over) {          // only the ends of the step's values are wanted
-          float low = INFINITY, high = -INFINITY;
+        for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+        if (__ballot(by_step ? step_of(top) < hi : top >= bound) == 0ull) return;
+        uint32_t todo = 0u;       // a bit per element
 #pragma unroll
-          for (int e = 0; e < EPV; ++e) {
-            const float y = step_of(x[e]);
-            const bool in = y >= lo && y < hi;
-            low = __builtin_elementwise_minimum(low, in ? x[e] : INFINITY);
-            high = __builtin_elementwise_maximum(high, in ? x[e] : -INFINITY);
-          }
-          step_min = __builtin_elementwise_minimum(step_min, low);
-          step_max = __builtin_elementwise_maximum(step_max, high);
-          return;
-        }
-        uint32_t todo = 0u, in_step = 0u;       // a bit per element
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) {
-          if (by_step) {
-            const float y = step_of(x[e]);
-            const bool in = y >= lo && y < hi;
-            step_min = __builtin_elementwise_minimum(step_min, in ? x[e] : INFINITY);
-            step_max = __builtin_elementwise_maximum(step_max, in ? x[e] : -INFINITY);
-            in_step |= in ? 1u << e : 0u;
-            todo |= y < hi ? 1u << e : 0u;
-          } else {
-            todo |= x[e] >= bound && x[e] > -INFINITY ? 1u << e : 0u;
-          }
-        }
-        if (full) todo = in_step;      // a full list takes no more, but the step still does
-        while (true) {
+        for (int e = 0; e < EPV; ++e)
+          todo |= (by_step ? step_of(x[e]) < hi : x[e] >= bound && x[e] > -INFINITY) ? 1u << e : 0u;
+        while (!full) {
           const unsigned long long who = __ballot(todo != 0u);
           if (who == 0ull) break;
-          const bool mine = todo != 0u;
-          const int e = mine ? __builtin_ctz(todo) : 0;
+          const int e = todo != 0u ? __builtin_ctz(todo) : 0;
+          full = !put(sh.count, sh.h.list, kList, who, todo != 0u, entry_of(r, c, e));
           todo &= todo - 1u;
-          const unsigned long long entry =
-              ((unsigned long long)key_of(element<T>(r, e)) << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
-          if (!full) full = !put(sh.count, sh.h.list, kList, who, mine, entry);
-          if (by_step && !over) {
-            const bool in = mine && (in_step >> e & 1u) != 0u;
-            const unsigned long long ins = __ballot(in);
-            if (ins != 0ull) over = !put(sh.at, sh.h.step, kStep, ins, in, entry);
-          }
         }
       });
-      if (by_step && step_min <= step_max) {
+      __syncthreads();
+      n = uniform(sh.count);
+      listed = n <= kList;
+      __syncthreads();
+    };
+    // One step from the row: its elements, unless they are known to be too many (over), and their ends.
+    auto step_up = [&](float lo, float hi, bool over) __attribute__((always_inline)) {
+      const bool restricted = cut.x > -INFINITY;
+      __syncthreads();
+      if (tid == 0) { sh.at = over ? kStep + 1 : 0; sh.klo = 0xFFFFFFFFu; sh.khi = 0u; }
+      __syncthreads();
+      float step_min = INFINITY, step_max = -INFINITY;
+      each([&](const u32x4& r, int c) {
+        float x[EPV];
+        Elem<T>::unpack(r, x);
+        if (restricted) mask(x, rv.col0(c));
+        uint32_t todo = 0u;
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) {
+          const float y = step_of(x[e]);
+          const bool in = y >= lo && y < hi;
+          step_min = __builtin_elementwise_minimum(step_min, in ? x[e] : INFINITY);
+          step_max = __builtin_elementwise_maximum(step_max, in ? x[e] : -INFINITY);
+          if (!over) todo |= in ? 1u << e : 0u;
+        }
+        while (!over) {
+          const unsigned long long who = __ballot(todo != 0u);
+          if (who == 0ull) break;
+          const int e = todo != 0u ? __builtin_ctz(todo) : 0;
+          over = !put(sh.at, sh.h.step, kStep, who, todo != 0u, entry_of(r, c, e));
+          todo &= todo - 1u;
+        }
+      });
+      if (step_min <= step_max) {
         atomicMin(&sh.klo, key_of(step_min));
         atomicMax(&sh.khi, key_of(step_max));
       }
       __syncthreads();
       nb = uniform(sh.at);
-      n = uniform(sh.count);
-      listed = n <= kList;
       __syncthreads();
     };
 
@@ -820,7 +810,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       steps_over(reach(a.v));
     }
     // (with top-p alone there is no bound to list by)
-    if (use_k ? bound > -INFINITY || a.v <= kList : !use_p) gather(false, 0.f, 0.f, false, false);
+    if (use_k ? bound > -INFINITY || a.v <= kList : !use_p) list_up(false, 0.f);
     auto settle = [&](auto by_count) __attribute__((always_inline)) {
       constexpr bool count = decltype(by_count)::value;
       const int tid = thread_here();
@@ -876,8 +866,23 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       // the step that holds the cut, its elements in sh.h.step
       double ahead;
       const int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal, sh, &ahead);
-      if (by_list) {
-        if (b == kBins) return;         // everything stays
+      if (by_list && b == kBins) return;         // everything stays
+      if (!by_list && b < kBins) {
+        // How many there are at least, from the mass and the largest weight of each step: rows whose list or
+        // step is sure to overflow spare the way there.
+        float most = 0.f, in_b = 0.f;
+        for (int i = tid; i <= b; i += THREADS) {
+          const float least = count ? (float)sh.h.bins[i]
+                                    : (float)sh.h.bins[i] * fast_exp2((float)i / per * (float)base.c - (float)fx);
+          most += least;
+          if (i == b) in_b = least;
+        }
+        most = (float)block_reduce64<NW, Sum64>((double)most, sh.red);
+        in_b = (float)block_reduce64<NW, Sum64>((double)in_b, sh.red);
+        if (uniform(most) <= 1.01f * kList) list_up(true, (float)(b + 1));
+        if (!listed) step_up((float)b, (float)(b + 1), uniform(in_b) > 1.01f * kStep);
+      }
+      if (listed) {
         if (tid == 0) { sh.at = 0; sh.klo = 0xFFFFFFFFu; sh.khi = 0u; }
         __syncthreads();
 #pragma unroll 1
@@ -893,19 +898,6 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         }
         __syncthreads();
         nb = uniform(sh.at);
-      } else if (b < kBins) {
-        // How many there are at least, from the mass and the largest weight of each step: rows whose list or
-        // step is sure to overflow spare the way there.
-        float most = 0.f, in_b = 0.f;
-        for (int i = tid; i <= b; i += THREADS) {
-          const float least = count ? (float)sh.h.bins[i]
-                                    : (float)sh.h.bins[i] * fast_exp2((float)i / per * (float)base.c - (float)fx);
-          most += least;
-          if (i == b) in_b = least;
-        }
-        most = (float)block_reduce64<NW, Sum64>((double)most, sh.red);
-        in_b = (float)block_reduce64<NW, Sum64>((double)in_b, sh.red);
-        gather(true, (float)b, (float)(b + 1), uniform(most) > 1.01f * kList, uniform(in_b) > 1.01f * kStep);
       }
       if (b < kBins && nb <= kStep) {
         sort_step<THREADS>(sh, nb);
