@@ -28,9 +28,9 @@
 //
 // What bounds it: the arithmetic of those weights, some 27 instructions an element with the histogram, on
 // the row's one compute unit; memory is far (256 rows of 128256 bf16 are 10 us of reading). Measured, bf16,
-// [1,128256]: unfiltered 28 us, min-p 15, top-k 50 25, top-p 0.9 43 (maximum 4, histogram 23, list 8, cut,
-// token and launch 8), 88 on a flat row, whose every element is kept. [256,128256]: 33, 27, 37, 58, 100.
-// [512,128256]: 55, 42, 49, 92, 167. [1024,32000]: 36, 29, 50, 65, 108. Splitting a row over workgroups
+// [1,128256]: unfiltered 28 us, min-p 15, top-k 50 25, top-p 0.9 43 (maximum 4, histogram 23, list 6, cut,
+// token and launch 8), 88 on a flat row, most of whose elements are kept. [256,128256]: 33, 26, 35, 57, 101.
+// [512,128256]: 55, 42, 48, 89, 171. [1024,32000]: 35, 28, 50, 59, 109. Splitting a row over workgroups
 // would divide the 23 us alone, for a second launch and partial histograms in memory: 10 us at best.
 //
 // What keeps it small counts too: the code that a call runs through fits the instruction cache (64 KB for
