@@ -28,9 +28,9 @@
 //
 // What bounds it: the arithmetic of those weights, some 27 instructions an element with the histogram, on
 // the row's one compute unit; memory is far (256 rows of 128256 bf16 are 10 us of reading). Measured, bf16,
-// [1,128256]: unfiltered 28 us, min-p 15, top-k 50 25, top-p 0.9 43 (maximum 4, histogram 23, list 6, cut,
-// token and launch 8), 88 on a flat row, most of whose elements are kept. [256,128256]: 33, 26, 35, 57, 101.
-// [512,128256]: 55, 42, 48, 89, 171. [1024,32000]: 35, 28, 50, 59, 109. Splitting a row over workgroups
+// [1,128256]: unfiltered 28 us, min-p 12, top-k 50 25, top-p 0.9 39 (maximum 4, histogram 23, list 6, cut,
+// token and launch 6), 88 on a flat row, most of whose elements are kept. [256,128256]: 33, 24, 36, 54, 101.
+// [512,128256]: 55, 41, 48, 87, 171. [1024,32000]: 35, 25, 51, 54, 110. Splitting a row over workgroups
 // would divide the 23 us alone, for a second launch and partial histograms in memory: 10 us at best.
 //
 // What keeps it small counts too: the code that a call runs through fits the instruction cache (64 KB for
@@ -39,6 +39,7 @@
 #include "../../include/fm_hip_tokens.h"
 #include "fm_f64.hip.h"
 #include "fm_topk.hip.h"
+#include <type_traits>
 
 using namespace fm;
 
@@ -46,6 +47,7 @@ namespace {
 
 constexpr int kBins = 2048;
 constexpr int kStep = 1024;          // candidates of one step (or one segment)
+constexpr int kFew = 256;            // as many are ordered by comparing each with each
 constexpr int64_t kMaxCols = 1 << 20;
 
 struct SampleArgs {
@@ -509,6 +511,32 @@ __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x
   return pick<T, THREADS, G>(rv, nseg, [&](int i) { return sh.seg[i]; }, c - 0.5, equal, sh, &w, &s, &before);
 }
 
+// Few entries, their amounts in sh.h.mass: fn(i, amount ahead of entry i, its own, all) for each of them, on
+// every lane of the eight that share it, where `ahead` counts the entries that are larger than it as
+// `key` puts them. Each is compared with each, which for a few hundred is quicker than a histogram with a
+// search in it, or a sort ([1,128256] bf16 min-p: 12 us, 15 without; top-p 0.9: 39, 43 without). The amounts
+// are integers, the sums exact.
+template <int THREADS, typename K, typename F>
+__device__ __forceinline__ void each_of_few(const unsigned long long* from, int n, SampleShared<THREADS>& sh, K key, F fn) {
+  const int tid = thread_here(), part = tid & 7;
+  for (int i0 = 0; i0 < n; i0 += THREADS / 8) {
+    const int i = i0 + (tid >> 3);
+    const auto mine = key(from[i < n ? i : n - 1]);
+    unsigned long long ahead = 0ull, all = 0ull;
+    for (int o = part; o < n; o += 8) {
+      const unsigned long long w = sh.h.mass[o];
+      all += w;
+      ahead += key(from[o]) > mine ? w : 0ull;
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) {
+      ahead += __shfl_xor(ahead, d, 64);
+      all += __shfl_xor(all, d, 64);
+    }
+    if (i < n) fn(i, ahead, sh.h.mass[i], all);
+  }
+}
+
 // sh.h.step[0 .. n) in descending order (n <= kStep), by the workgroup
 template <int THREADS>
 __device__ __forceinline__ void sort_step(SampleShared<THREADS>& sh, int n) {
@@ -800,6 +828,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       __syncthreads();
     };
 
+    // the amounts of entries, 0 for what the cut so far does not keep, into sh.h.mass
+    auto amounts = [&](const unsigned long long* from, int many, auto by_count) __attribute__((always_inline)) {
+      const Weight weight = base.fresh();
+#pragma unroll 1
+      for (int i = tid; i < many; i += THREADS) {
+        const unsigned long long e = from[i];
+        sh.h.mass[i] = !kept(value(e), column(e)) ? 0ull : decltype(by_count)::value ? 1ull : fixed(weight(value(e)));
+      }
+      __syncthreads();
+    };
+
     // 3: the exact cuts, first by count, then by the mass of what that leaves. The cut is the first element,
     // in descending order, at which the running amount reaches the goal.
     if (use_k) {
@@ -813,7 +852,6 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     if (use_k ? bound > -INFINITY || a.v <= kList : !use_p) list_up(false, 0.f);
     auto settle = [&](auto by_count) __attribute__((always_inline)) {
       constexpr bool count = decltype(by_count)::value;
-      const int tid = thread_here();
       if (count && listed && n < k) return;         // all of them stay
       const bool by_list = listed;
       const bool restricted = cut.x > -INFINITY;
@@ -899,6 +937,22 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         __syncthreads();
         nb = uniform(sh.at);
       }
+      if (b < kBins && nb <= kFew) {
+        amounts(sh.h.step, nb, by_count);
+        if (tid == 0) sh.at = 0;
+        __syncthreads();
+        const double left = goal - ahead;
+        each_of_few<THREADS>(sh.h.step, nb, sh, [](unsigned long long e) { return e; },
+            [&](int i, unsigned long long before, unsigned long long w, unsigned long long all) {
+              // the first whose running amount reaches the goal, or else the last
+              if (w > 0ull && (before == 0ull || (double)before < left) && ((double)(before + w) >= left || before + w == all)) sh.at = i;
+            });
+        __syncthreads();
+        cut.x = uniform(value(sh.h.step[sh.at]));
+        cut.col = uniform(column(sh.h.step[sh.at]));
+        __syncthreads();
+        return;
+      }
       if (b < kBins && nb <= kStep) {
         sort_step<THREADS>(sh, nb);
         double unused;
@@ -945,6 +999,21 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     }
 
     // 4 on the list
+    if (listed && n <= kFew) {
+      amounts(sh.h.list, n, std::false_type{});
+      // larger: of a lower index
+      each_of_few<THREADS>(sh.h.list, n, sh, [](unsigned long long e) { return (uint32_t)e; },
+          [&](int i, unsigned long long ahead, unsigned long long w, unsigned long long all) {
+            const double target = u * (double)all;
+            if ((tid & 7) == 0 && (double)ahead <= target && target < (double)(ahead + w)) {
+              const unsigned long long e = sh.h.list[i];
+              a.token[row] = column(e);
+              if (a.logprob != nullptr)
+                a.logprob[row] = (float)(log2_64(base(value(e)) * unit / (double)all) * kLn2d);
+            }
+          });
+      return;
+    }
     if (listed) {
       constexpr int PER = (kList + THREADS - 1) / THREADS;
       int shift = 6;
@@ -1080,8 +1149,8 @@ void launch(const void* logits, const SampleArgs& a, int64_t n, hipStream_t st) 
 #define GO(TH, G) FM_LAUNCH((sample_kernel<T, TH, G>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
   // Short rows: four waves, a block of 64 vectors a segment, so that each wave has segments to sweep
   // ([2048,8000] bf16 top-p 0.9: 70 us with 512 threads, 56 with these). Rows for which there is a compute
-  // unit each: all of its waves ([1,128256] top-p 0.9: 51 us with 512 threads, 45 with these; a short list
-  // costs 6 us more). More rows: half-size workgroups, two rows a unit in different phases ([1024,32000]
+  // unit each: all of its waves ([1,128256] top-p 0.9: 51 us with 512 threads when it was 45 with these; a
+  // short list costs up to 6 us more). More rows: half-size workgroups, two rows a unit in different phases ([1024,32000]
   // top-p 0.9: 99 us with the large ones, 66 with these).
   if (nvec <= 1024) GO(256, 1);
   else if (n <= fm_host::num_cus()) GO(1024, 4);
