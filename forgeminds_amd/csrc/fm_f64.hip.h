@@ -26,7 +26,6 @@ __device__ __forceinline__ double readlane64(double v, int l) {
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 struct Sum64 { __device__ static __forceinline__ double f(double a, double b) { return a + b; } };
-struct Max64 { __device__ static __forceinline__ double f(double a, double b) { return b > a ? b : a; } };
 
 // over aligned groups of G lanes (1, 2, 4, 8, 16 or 64), the result in every lane, fixed order
 template <int G, typename Op>
