@@ -29,6 +29,8 @@ namespace {
 constexpr int kMaxList = 1024;
 constexpr int kSmallList = 128;
 constexpr uint16_t kEnd = 0xFFFFu;
+// up to this many rows every workgroup counts the listed rows itself; beyond, one launch counts
+constexpr int kCountInKernel = 256;
 
 struct ListArgs {
   const void* idx;
@@ -494,8 +496,15 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   // the list's loads go first: waiting for them then waits for nothing of the row
   SlotBits bits[SL];
   list_load<THREADS, SL>(a, row, bits);
-  // where the rows are few, every workgroup counts those with a list itself
-  const int first = GRAD ? slot_sign(a, (int64_t)(tid < count_n ? tid : 0) * a.k) : 0;
+  // where the rows are few (count_n <= kCountInKernel), every workgroup counts those with a list itself,
+  // kCount of them a thread
+  constexpr int kCount = GRAD ? (kCountInKernel + THREADS - 1) / THREADS : 1;
+  int first[kCount];
+#pragma unroll
+  for (int j = 0; j < kCount; ++j) {
+    const int r = j * THREADS + tid;
+    first[j] = GRAD ? slot_sign(a, (int64_t)(r < count_n ? r : 0) * a.k) : 0;
+  }
   const float nv = *(GRAD && n_valid != nullptr ? n_valid : static_cast<const float*>(a.idx));
   const float lse_t = *(a.teacher_lse != nullptr ? a.teacher_lse + row : static_cast<const float*>(a.idx));
   const T* vp = rp + sp.head;              // 16-byte aligned where there are vectors
@@ -514,7 +523,9 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   const uint16_t head = sh.head[tid];
 
   if (GRAD && count_n > 0) {
-    const int c = __builtin_popcountll(__ballot(tid < count_n && first >= 0));
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) c += __builtin_popcountll(__ballot(j * THREADS + tid < count_n && first[j] >= 0));
     if ((tid & 63) == 0) sh.count[tid >> 6] = c;
   }
 
@@ -757,9 +768,6 @@ __global__ __launch_bounds__(1024) void kl_topk_reduce_kernel(const float* __res
     if (LOSS) *loss = (float)(mean ? s / (double)nv : s);
   }
 }
-
-// up to this many rows every workgroup counts the listed rows itself; beyond, one launch counts
-constexpr int64_t kCountInKernel = 256;
 
 int check(const char* what, int64_t n, int64_t v, int k, int dtype, int index_bits, int teacher_dtype, int kind,
           int tail, double temperature) {

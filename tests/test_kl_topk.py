@@ -525,3 +525,24 @@ def test_another_device_than_the_current_one_is_refused_or_served():
         fm.kernels.kl_div_topk(s.to(DEV), idx, t.to(DEV))
     with pytest.raises(ValueError):
         fm.kernels.kl_div_topk(s.to(DEV), idx.to(DEV), t)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("v", [1000, 4096, 8200, 16384])
+def test_the_mean_counts_every_row(dt, v):
+    """The gradient of the mean is divided by the rows that have a list, however many rows there are
+    beside the threads of a workgroup and whichever of them are skipped."""
+    n, k = 257, 64
+    s, idx, t, lse = make(n, v, k, dt, "logits", "renorm", seed=v)
+    _loss, grad, size, _valid = O.kl_topk(s, idx, t)
+    sd, di, td = to_dev(s, idx, t)
+    for m in (1, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257):
+        for skipped in (range(0), range(0, m, 3), range(min(m, 64)), range(min(m, 128)), range(64, m), range(1, m)):
+            live = torch.ones(m, dtype=torch.bool)
+            live[list(skipped)] = False
+            gone = torch.where(live.to(DEV)[:, None], di[:m], -1)
+            x = sd[:m].clone().requires_grad_(True)
+            fm.kernels.kl_div_topk(x, gone, td[:m]).backward()
+            scale = live[:, None].double() / max(int(live.sum()), 1)
+            check_grad(x.grad, grad[:m] * scale, size[:m] * scale, dt, v, what=f"{m} rows, {m - int(live.sum())} skipped")
