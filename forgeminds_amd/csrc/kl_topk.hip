@@ -116,11 +116,30 @@ __device__ __forceinline__ uint32_t bits_of(float f) {
   else return pack_f16(f, 0.f) & 0xffffu;
 }
 
-// A running (maximum, sum) whose sum is held in 64 bits.
+// A running (maximum, sum) whose sum is held in 64 bits. Where x * c is so large that fp32 cannot tell the
+// maximum from its neighbours (|x c| > 2^31, a row or all of its unlisted columns masked with the type's
+// lowest value), the sum is negative and the maximum is the logit itself (exact_pairs).
 struct Pair64 {
   float m;
   double s;
+  __device__ __forceinline__ double top(float c) const { return s < 0.0 ? (double)m * (double)c : (double)m; }
+  __device__ __forceinline__ double sum() const { return __builtin_fabs(s); }
+  // the largest weight of a row is 1, off by 2^-25 |x c| in the exponent
+  __device__ __forceinline__ bool sound() const { return s >= 0.5 && s <= 1e12; }
 };
+// An unlisted column's weight is exp2(x * c - m).
+struct Sweep {
+  float c, m;
+};
+__device__ __forceinline__ Sweep sweep_of(const Pair64& rest, float c) {
+  if (!(rest.s < 0.0)) return Sweep{c, rest.m};
+  // 2^7 or more between neighbouring logits: the weight is 1 for the maximum and 0 for everything else,
+  // which a power of two in place of c shows without rounding
+  int e = 120 - __builtin_amdgcn_frexp_expf(rest.m);
+  e = e < 127 ? e : 127;
+  const float p = __builtin_amdgcn_ldexpf(1.f, e);
+  return Sweep{p, rest.m * p};
+}
 template <int NW>
 struct MergeShared {
   double s[2][NW];
@@ -371,13 +390,15 @@ __device__ __forceinline__ void walk(const ListShared<THREADS, KCAP>& sh, uint16
 
 // What the merged pairs and the list make of a row.
 struct RowTerms {
-  double lse2;       // base-2 log-sum-exp of the whole row
+  double x0, lse2;   // log2 p = (x - x0) c - lse2: the base-2 log-sum-exp of the whole row, of its
+                     // differences to x0 where the maximum is a logit
   double q_r;        // probability of the bucket
   double total;      // sum of q and the bucket
 };
 __device__ __forceinline__ RowTerms row_terms(const ListArgs& a, const Pair64& all, double sum_q, int unique, int v) {
   RowTerms t;
-  t.lse2 = (double)all.m + log2_64(all.s);
+  t.x0 = all.s < 0.0 ? (double)all.m : 0.0;
+  t.lse2 = (all.s < 0.0 ? 0.0 : (double)all.m) + log2_64(all.sum());
   t.q_r = 0.0;
   if (a.tail == FM_TAIL_BUCKET && unique < v) {
     t.q_r = 1.0 - sum_q;
@@ -387,7 +408,7 @@ __device__ __forceinline__ RowTerms row_terms(const ListArgs& a, const Pair64& a
   return t;
 }
 // The listed columns' gradients into sh.g, as stored bits (a barrier ends it); returns the coefficient
-// of an unlisted column, whose gradient is coef * exp2(x * c - rest.m).
+// of an unlisted column, which its weight (sweep_of) is multiplied by.
 template <typename T, int THREADS, int KCAP, int SL>
 __device__ __forceinline__ float row_gradient(const ListArgs& a, ListShared<THREADS, KCAP>& sh, const Mine<SL>& mine,
                                               const Pair64& all, const Pair64& rest, const RowTerms& t, double scale) {
@@ -395,29 +416,31 @@ __device__ __forceinline__ float row_gradient(const ListArgs& a, ListShared<THRE
   for (int j = 0; j < SL; ++j) {
     if (mine.col[j] < 0) continue;
     const int s = j * THREADS + (int)threadIdx.x;
-    const double lp2 = (double)sh.x[s] * (double)a.c - t.lse2;
+    const double lp2 = ((double)sh.x[s] - t.x0) * (double)a.c - t.lse2;
     sh.g[s] = bits_of<T>((float)((exp2_64(lp2) * t.total - mine.q[j]) * scale));
   }
   __syncthreads();
-  double coef = t.total * exp2_64((double)rest.m - (double)all.m) / all.s;
-  if (!(t.q_r == 0.0)) coef -= t.q_r / rest.s;
+  double coef = t.total * exp2_64(rest.top(a.c) - all.top(a.c)) / all.sum();
+  if (!(t.q_r == 0.0)) coef -= t.q_r / rest.sum();
   // no unlisted column with any probability: their logits are -inf and their gradient 0
   if (rest.s == 0.0 && t.q_r == 0.0) coef = 0.0;
   return (float)(coef * scale);
 }
 template <int THREADS, int KCAP, int SL>
 __device__ __forceinline__ void row_loss_of(const ListArgs& a, ListShared<THREADS, KCAP>& sh, const Mine<SL>& mine,
-                                            const Pair64& rest, const RowTerms& t, double sum_q, float* loss_at) {
+                                            const Pair64& all, const Pair64& rest, const RowTerms& t, double sum_q,
+                                            float* loss_at) {
   double term = 0.0;
 #pragma unroll
   for (int j = 0; j < SL; ++j) {
     if (mine.col[j] < 0 || mine.q[j] == 0.0) continue;
-    const double lp2 = (double)sh.x[j * THREADS + (int)threadIdx.x] * (double)a.c - t.lse2;
+    const double lp2 = ((double)sh.x[j * THREADS + (int)threadIdx.x] - t.x0) * (double)a.c - t.lse2;
     term += mine.q[j] * (log2_64(mine.q[j]) - lp2);
   }
   term = block_reduce64<THREADS / 64, Sum64>(term, sh.red);
   if (threadIdx.x == 0) {
-    if (!(t.q_r == 0.0)) term += t.q_r * (log2_64(t.q_r) - ((double)rest.m + log2_64(rest.s) - t.lse2));
+    if (!(t.q_r == 0.0))
+      term += t.q_r * (log2_64(t.q_r) - ((rest.top(a.c) - all.top(a.c)) + (log2_64(rest.sum()) - log2_64(all.sum()))));
     *loss_at = (float)(sum_q != sum_q ? sum_q : term * kLn2d);
   }
 }
@@ -445,16 +468,91 @@ __device__ __forceinline__ void store_bits(T* p, uint32_t bits) {
   else *reinterpret_cast<uint16_t*>(p) = (uint16_t)bits;
 }
 
+// The two pairs of a row from its logits' differences to their maxima, in 64 bits: two more readings of the
+// row, for rows whose pairs in fp32 are not sound -- x * c beyond fp32 or so large that the rounding of its
+// maximum weighs more than the weights. NaN and +inf make the sum NaN. All threads of the workgroup call it.
+template <typename T, int THREADS, int KCAP>
+__device__ __forceinline__ void exact_pairs(const T* rp, const RowSplit& sp, int ne, float c, bool bucket, uint32_t mask,
+                                            uint16_t head, ListShared<THREADS, KCAP>& sh, Pair64* rest, Pair64* all) {
+  constexpr int EPV = Elem<T>::kVec;
+  constexpr int NW = THREADS / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // fn(logit, whether it is one of the listed columns that count apart)
+  auto own = [&](auto fn) {
+#pragma unroll 1
+    for (int i = tid; i < sp.nvec; i += THREADS) {
+      uint32_t hit = 0u;
+      const int col0 = sp.head + i * EPV;
+      if (bucket && ((mask >> ((i / THREADS) % 31)) & 1u))
+        walk<EPV, THREADS, KCAP>(sh, head, col0, [&](int d, int) { hit |= 1u << d; });
+      float x[EPV];
+      Elem<T>::unpack(load16(rp + col0), x);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) fn(x[e], (hit >> e) & 1u);
+    }
+#pragma unroll 1
+    for (int e = tid; e < ne; e += THREADS) {
+      uint32_t hit = 0u;
+      const int col = edge_col(sp, e);
+      if (bucket && (mask >> 31)) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int) { hit = 1u; });
+      fn(Elem<T>::load1(rp + col), hit);
+    }
+  };
+  float top = -INFINITY, top_l = -INFINITY;
+  own([&](float x, uint32_t hit) {
+    const float y = x == x ? x : INFINITY;
+    top = fmaxf(top, hit ? -INFINITY : y);
+    top_l = fmaxf(top_l, hit ? y : -INFINITY);
+  });
+  top = wave_max(top);
+  top_l = wave_max(top_l);
+  __syncthreads();
+  if (lane == 0) { sh.merge.m[0][wave] = top; sh.merge.m[1][wave] = top_l; }
+  __syncthreads();
+  top = group_reduce<NW, OpMax>(sh.merge.m[0][lane & (NW - 1)]);
+  top_l = group_reduce<NW, OpMax>(sh.merge.m[1][lane & (NW - 1)]);
+  double sum = 0.0, sum_l = 0.0;
+  own([&](float x, uint32_t hit) {
+    if (x == -INFINITY) return;            // (top may be -inf itself)
+    const double w = exp2_64(((double)x - (double)(hit ? top_l : top)) * (double)c);
+    sum += hit ? 0.0 : w;
+    sum_l += hit ? w : 0.0;
+  });
+  sum = wave_sum64(sum);
+  sum_l = wave_sum64(sum_l);
+  if (lane == 0) { sh.merge.s[0][wave] = sum; sh.merge.s[1][wave] = sum_l; }
+  __syncthreads();
+  sum = group_reduce64<NW, Sum64>(sh.merge.s[0][lane & (NW - 1)]);
+  sum_l = group_reduce64<NW, Sum64>(sh.merge.s[1][lane & (NW - 1)]);
+  if (top == INFINITY) sum = __builtin_nan("");
+  if (top_l == INFINITY) sum_l = __builtin_nan("");
+  auto pair = [&](float m, double s) {
+    if (s == 0.0) return Pair64{kNegBig, 0.0};
+    const double t = (double)m * (double)c;
+    if (!(__builtin_fabs(t) <= 2147483648.0) && s == s) return Pair64{m, -s};
+    const float f = (float)t;
+    return Pair64{f, s * exp2_64(t - (double)f)};
+  };
+  *rest = pair(top, sum);
+  *all = *rest;
+  if (sum_l != 0.0) {
+    const float m = fmaxf(top, top_l);
+    double s = sum_l * exp2_64(((double)top_l - (double)m) * (double)c);
+    if (sum != 0.0) s += sum * exp2_64(((double)top - (double)m) * (double)c);
+    *all = pair(m, s);
+  }
+}
+
 // the gradient of vector c (its first column col0), packed
 template <typename T, int THREADS, int KCAP>
-__device__ __forceinline__ u32x4 grad_of(const u32x4& r, float scale, float m, float coef,
+__device__ __forceinline__ u32x4 grad_of(const u32x4& r, const Sweep& w, float coef,
                                          const ListShared<THREADS, KCAP>& sh, uint32_t mask, uint16_t head, int c,
                                          int col0) {
   constexpr int EPV = Elem<T>::kVec;
   float x[EPV];
   Elem<T>::unpack(r, x);
 #pragma unroll
-  for (int e = 0; e < EPV; ++e) x[e] = coef * fast_exp2(__builtin_fmaf(x[e], scale, -m));
+  for (int e = 0; e < EPV; ++e) x[e] = coef * fast_exp2(__builtin_fmaf(x[e], w.c, -w.m));
   u32x4 o = Elem<T>::pack(x);
   if ((mask >> ((c / THREADS) % 31)) & 1u)
     walk<EPV, THREADS, KCAP>(sh, head, col0, [&](int d, int s) { set_elem<T>(o, d, sh.g[s]); });
@@ -589,6 +687,16 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
   }
   Pair64 rest, all;
   merge_pairs<NW>(run, listed, bucket, sh.merge, &rest, &all);      // its barrier also publishes sh.x
+  // (alike in all lanes, and the compiler has to know: behind a lane's branch the row's registers stay taken)
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(rest.sound() && all.sound()) == 0, 0)) {
+    exact_pairs<T, THREADS, KCAP>(rp, sp, ne, a.c, bucket, mask, head, sh, &rest, &all);
+    if constexpr (GRAD && VEC) {       // the row's registers were free meanwhile, and so were its addresses'
+      int me = tid;
+      asm volatile("" : "+v"(me));
+#pragma unroll
+      for (int i = 0; i < RI; ++i) raw[i] = load16(at(clamp_col(i * THREADS + me, sp.nvec)));
+    }
+  }
   const RowTerms terms = row_terms(a, all, sum_q, unique, v);
   if (tid == 0 && stats != nullptr) {
     stats[row * 4] = all.m;
@@ -611,10 +719,11 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     int me = tid;
     asm volatile("" : "+v"(near.e0), "+v"(near.e1), "+v"(near.more), "+v"(mask), "+v"(me));
     T* vg = gp + sp.head;
+    const Sweep w = sweep_of(rest, a.c);
     auto put = [&](const u32x4& r, int c) {
       if (c >= sp.nvec) return;
       store16_stream(reinterpret_cast<T*>(reinterpret_cast<char*>(vg) + (uint32_t)c * 16u),
-                     grad_of<T, THREADS, KCAP>(r, a.c, rest.m, coef, sh, mask, head, c, sp.head + c * EPV));
+                     grad_of<T, THREADS, KCAP>(r, w, coef, sh, mask, head, c, sp.head + c * EPV));
     };
     if constexpr (VEC) {
 #pragma unroll
@@ -622,7 +731,7 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
         touch_whole(raw[i]);
         const int c = i * THREADS + me;
         if (c >= sp.nvec) continue;
-        u32x4 o = grad_of<T, THREADS, KCAP>(raw[i], a.c, rest.m, coef, sh, near.more, head, c, sp.head + c * EPV);
+        u32x4 o = grad_of<T, THREADS, KCAP>(raw[i], w, coef, sh, near.more, head, c, sp.head + c * EPV);
         if ((mask >> (i % 31)) & 1u) {
           if ((near.e0 & 255u) == (uint32_t)i) set_elem<T>(o, (near.e0 >> 8) & 15u, g0);
           if ((near.e1 & 255u) == (uint32_t)i) set_elem<T>(o, (near.e1 >> 8) & 15u, g1);
@@ -642,14 +751,14 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     }
     for (int e = tid; e < ne; e += THREADS) {
       const int col = edge_col(sp, e);
-      float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), a.c, -rest.m));
+      float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), w.c, -w.m));
       uint32_t one = bits_of<T>(o);
       if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { one = sh.g[s]; });
       store_bits(gp + col, one);
     }
   }
   // last: the reduction runs while the stores drain
-  row_loss_of<THREADS, KCAP, SL>(a, sh, mine, rest, terms, sum_q, row_loss + row);
+  row_loss_of<THREADS, KCAP, SL>(a, sh, mine, all, rest, terms, sum_q, row_loss + row);
 }
 
 // The gradient from saved stats. chunks > 1: a workgroup takes one tile of THREADS * UN vectors of a
@@ -698,6 +807,7 @@ __global__ __launch_bounds__(THREADS) void kl_topk_bwd_kernel(const T* student, 
   const uint32_t mask = sh.mask[tid];
   const uint16_t head = sh.head[tid];
   const float coef = row_gradient<T, THREADS, KCAP, SL>(a, sh, mine, all, rest, row_terms(a, all, sum_q, unique, v), scale);
+  const Sweep w = sweep_of(rest, a.c);
   for (int c0 = c_begin; c0 < c_end; c0 += THREADS * UN) {
     u32x4 raw[UN];
 #pragma unroll
@@ -709,12 +819,12 @@ __global__ __launch_bounds__(THREADS) void kl_topk_bwd_kernel(const T* student, 
       touch_whole(raw[u]);
       if (c < c_end)
         store16_stream(gp + sp.head + (int64_t)c * EPV,
-                       grad_of<T, THREADS, KCAP>(raw[u], a.c, rest.m, coef, sh, mask, head, c, sp.head + c * EPV));
+                       grad_of<T, THREADS, KCAP>(raw[u], w, coef, sh, mask, head, c, sp.head + c * EPV));
     }
   }
   for (int e = tid; e < ne; e += THREADS) {
     const int col = edge_col(sp, e);
-    float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), a.c, -rest.m));
+    float o = coef * fast_exp2(__builtin_fmaf(Elem<T>::load1(rp + col), w.c, -w.m));
     uint32_t one = bits_of<T>(o);
     if (mask >> 31) walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) { one = sh.g[s]; });
     store_bits(gp + col, one);

@@ -30,7 +30,8 @@ extern "C" {
  * The listed columns and the row's loss are computed in 64 bits (the loss is a small difference),
  * the sweep over the row in fp32.
  * row_loss: fp32 [n]. stats: fp32 [n, 4] for fm_kl_topk_bwd (running maximum and sum of the whole
- * row, then of its unlisted columns, base 2). loss, n_valid: fp32 device scalars; loss = sum of
+ * row, then of its unlisted columns, base 2; a negative sum goes with a maximum that is the logit itself,
+ * where masks with the lowest values leave nothing else). loss, n_valid: fp32 device scalars; loss = sum of
  * row_loss (FM_REDUCE_SUM) or that / n_valid (FM_REDUCE_MEAN), n_valid = max(1, rows not skipped);
  * both may be NULL for FM_REDUCE_NONE, which writes neither. 1 <= k <= 1024, k may exceed v;
  * n < 2^22, v < 2^30 (FM_ERR_UNSUPPORTED past those). */

@@ -546,3 +546,118 @@ def test_the_mean_counts_every_row(dt, v):
             fm.kernels.kl_div_topk(x, gone, td[:m]).backward()
             scale = live[:, None].double() / max(int(live.sum()), 1)
             check_grad(x.grad, grad[:m] * scale, size[:m] * scale, dt, v, what=f"{m} rows, {m - int(live.sum())} skipped")
+
+
+def agrees(got, want, tol):
+    """Within ``tol``, or both past the largest fp32 value."""
+    got = got.detach().double().cpu()
+    return (((got - want).abs() <= tol) | ((got == float("inf")) & torch.isinf(want.float()))).all()
+
+
+def low_reference(s, idx, q, T):
+    """Row losses and gradient of their sum for tail="bucket", float64, from differences to the maxima
+    (``oracle.tokens`` goes through log p, where 3e38 leaves no digit of the other terms)."""
+    n, v = s.shape
+    loss, grad, size = torch.zeros(n), torch.zeros(n, v), torch.zeros(n, v)
+    loss, grad, size = loss.double(), grad.double(), size.double()
+    for i in range(n):
+        z, c, w = s[i].double() / T, idx[i], q[i].double()
+        m = z.max()
+        p = torch.exp(z - m)
+        ls = torch.log(p.sum())
+        p = p / p.sum()
+        out = torch.ones(v, dtype=torch.bool)
+        out[c] = False
+        left = max(0.0, 1.0 - math.fsum(w.tolist()))
+        mr = z[out].max()
+        share = torch.where(out, torch.exp(z - mr), 0.0)
+        ls_r = torch.log(share.sum())
+        loss[i] = (w * (torch.log(w) - ((z[c] - m) - ls))).sum() + left * (math.log(left) - ((mr - m) + (ls_r - ls)))
+        share = share / share.sum()
+        grad[i] = p * (w.sum() + left) - left * share
+        size[i] = p * (w.sum() + left) + left * share
+        grad[i, c] -= w
+        size[i, c] += w
+    return loss, grad / T, size / T
+
+
+@gpu
+@pytest.mark.parametrize("T", [0.7, 1.0, 2.0])
+@pytest.mark.parametrize("dt,v", [(F32, 300), (BF16, 300), (BF16, 5003), (F32, 70001), (BF16, 140000)])
+def test_bucket_over_logits_masked_with_the_lowest_value(dt, v, T):
+    """Finite rows have a finite gradient, however low their masks. Where the low logits take part the
+    loss is q_r times 3.4e38 / T: off by the rounding of log2(e) / T and of the result, half a step each,
+    and of q_r, which the reference shares. A loss past the largest fp32 value is rounded to inf (at
+    T = 0.7 listed probabilities of 0.9 at masked logits: 4.4e38)."""
+    k, low = 64, torch.finfo(dt).min
+    g = torch.Generator().manual_seed(v)
+    s = torch.randn(7, v, generator=g)
+    idx = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(7)])
+    q = torch.softmax(torch.randn(7, k, generator=g), -1) * 0.9
+    out = torch.ones(7, v, dtype=torch.bool).scatter_(1, idx, False)
+    s[0][out[0]] = low                                # everything unlisted masked
+    s[1][out[1]] = low
+    q[1] = q[1] * (1 - 2.0 ** -20) / q[1].double().sum()        # a bucket of rounding
+    s[2] = low                                        # the whole row masked: even
+    s[3][out[3]] = low                                # some of the unlisted ones out altogether
+    s[3, ::2] = torch.where(out[3, ::2], -float("inf"), s[3, ::2])
+    s[4][~out[4]] = low                               # everything listed masked
+    s[5][~out[5]] = low                               # half as low outside
+    s[5][out[5]] = low / 2
+    s = s.to(dt)
+    loss, grad, size = low_reference(s, idx, q, T)
+    assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+    tol = loss_tol(v, loss) + U * loss.abs()
+    sd, di, dq = to_dev(s, idx, q)
+    odd = torch.zeros(7 * v + 1, device=DEV, dtype=dt)[1:].view(7, v)
+    odd.copy_(sd)
+    kw = dict(probs=True, tail="bucket", temperature=T)
+    for base in (sd, odd):
+        x = base.detach().requires_grad_(True)
+        rows = fm.kernels.kl_div_topk(x, di, dq, reduction="none", **kw)
+        assert agrees(rows, loss, tol)
+        (gr,) = torch.autograd.grad(rows, x, torch.ones(7, device=DEV))
+        check_grad(gr, grad, size, dt, v, what="from stats")
+        total = fm.kernels.kl_div_topk(x, di, dq, reduction="sum", **kw)
+        assert agrees(total, loss.sum(), tol.sum() + U * loss.sum().abs())
+        (gr,) = torch.autograd.grad(total, x)
+        check_grad(gr, grad, size, dt, v, what="with the loss")
+    h = sd.clone().requires_grad_(True)
+    (gr,) = torch.autograd.grad(fm.kernels.kl_div_topk(h * 1.0, di, dq, reduction="sum", reuse=True, **kw), h)
+    check_grad(gr, grad, size, dt, v, what="in place")
+    # the other tails: the whole row is one sum
+    for tail in ("drop", "renorm"):
+        x = sd[[2, 6]].clone().requires_grad_(True)
+        rows = fm.kernels.kl_div_topk(x, di[[2, 6]], dq[[2, 6]], probs=True, tail=tail, reduction="none", temperature=T)
+        ref = O.kl_topk(s[[2, 6]], idx[[2, 6]], q[[2, 6]], None, True, tail, T)
+        assert ((rows.detach().double().cpu() - ref[0]).abs() <= loss_tol(v, ref[0])).all()
+        (gr,) = torch.autograd.grad(rows, x, torch.ones(2, device=DEV))
+        check_grad(gr, ref[1], ref[2], dt, v, what=tail)
+
+
+@gpu
+@pytest.mark.parametrize("level", [-1e4, -1e6, -1e8, -1e9, -3e9, -1e12, -1e30, 1e9, 3e38])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_rows_at_one_far_level(dt, level):
+    # whatever the level of a row, or of its unlisted columns, or of its listed ones (the sum at 3e38 is 4.3e38)
+    n, v, k, T = 4, 3001, 32, 1.0
+    g = torch.Generator().manual_seed(6)
+    s = torch.randn(n, v, generator=g)
+    idx = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(n)])
+    q = torch.softmax(torch.randn(n, k, generator=g), -1) * 0.5
+    out = torch.ones(n, v, dtype=torch.bool).scatter_(1, idx, False)
+    s[0] = level
+    s[1][out[1]] = level
+    s[2][~out[2]] = level
+    s[3] = torch.where(torch.rand(v, generator=g) < 0.5, level, -abs(level) * 1.1)
+    s = s.to(dt)
+    loss, grad, size = low_reference(s, idx, q, T)
+    tol = loss_tol(v, loss) + U * loss.abs()
+    sd, di, dq = to_dev(s, idx, q)
+    x = sd.clone().requires_grad_(True)
+    for reduction in ("none", "sum"):
+        out = fm.kernels.kl_div_topk(x, di, dq, probs=True, tail="bucket", reduction=reduction)
+        want, t = (loss, tol) if reduction == "none" else (loss.sum(), tol.sum() + U * loss.sum().abs())
+        assert agrees(out, want, t)
+        (gr,) = torch.autograd.grad(out.sum(), x)
+        check_grad(gr, grad, size, dt, v, what=reduction)
