@@ -422,8 +422,9 @@ __device__ __forceinline__ float row_gradient(const ListArgs& a, ListShared<THRE
   __syncthreads();
   double coef = t.total * exp2_64(rest.top(a.c) - all.top(a.c)) / all.sum();
   if (!(t.q_r == 0.0)) coef -= t.q_r / rest.sum();
-  // no unlisted column with any probability: their logits are -inf and their gradient 0
-  if (rest.s == 0.0 && t.q_r == 0.0) coef = 0.0;
+  // no unlisted column with any probability: their logits are -inf and their gradient 0 (a row of nothing
+  // but -inf is no distribution: NaN, as its loss)
+  if (rest.s == 0.0 && t.q_r == 0.0) coef = all.s == 0.0 ? __builtin_nan("") : 0.0;
   return (float)(coef * scale);
 }
 template <int THREADS, int KCAP, int SL>

@@ -21,7 +21,7 @@ extern "C" {
  * idx: [n, k] int32 or int64 (index_bits). A negative entry is an empty slot; a row whose slot 0
  * is empty is skipped: loss 0, gradient 0, not counted by the mean, its logits not read. A column
  * that a row lists more than once counts once, with the sum of its probabilities. A column >= v
- * makes the row's loss and gradient NaN. With FM_TAIL_BUCKET and every column listed, q_r = 0.
+ * makes the row's loss and gradient NaN, and so does a NaN or +inf among the logits, or nothing but -inf. With FM_TAIL_BUCKET and every column listed, q_r = 0.
  * teacher: [n, k] of teacher_dtype.
  *   FM_TEACHER_LOGITS  q = softmax(teacher / temperature) over the row's slots (FM_TAIL_RENORM), or
  *                      exp(teacher / temperature - teacher_lse[row]) (the other two; teacher_lse:

@@ -661,3 +661,18 @@ def test_rows_at_one_far_level(dt, level):
         assert agrees(out, want, t)
         (gr,) = torch.autograd.grad(out.sum(), x)
         check_grad(gr, grad, size, dt, v, what=reduction)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("dt,v", [(F32, 40), (BF16, 3000)])
+def test_a_row_without_a_finite_logit_has_no_gradient_to_give(dt, v, dev):
+    # -inf everywhere is no distribution: loss and gradient are NaN, listed or not, in that row alone
+    s, idx, t, _ = make(3, v, 5, dt, seed=4)
+    s[1] = -float("inf")
+    for tail, kw in (("renorm", {}), ("bucket", {"teacher_lse": torch.full((3,), 9.0, device=dev)})):
+        for reduction in ("none", "sum"):
+            x = s.to(dev).requires_grad_(True)
+            out = fm.kernels.kl_div_topk(x, idx.to(dev), t.to(dev), tail=tail, reduction=reduction, **kw)
+            (g,) = torch.autograd.grad(out.sum(), x)
+            assert out.isnan()[1].item() if reduction == "none" else out.isnan().item()
+            assert g[1].isnan().all() and not g[[0, 2]].isnan().any(), (tail, reduction)
