@@ -125,7 +125,7 @@ struct Pair64 {
   __device__ __forceinline__ double top(float c) const { return s < 0.0 ? (double)m * (double)c : (double)m; }
   __device__ __forceinline__ double sum() const { return __builtin_fabs(s); }
   // the largest weight of a row is 1, off by 2^-25 |x c| in the exponent
-  __device__ __forceinline__ bool sound() const { return s >= 0.5 && s <= 1e12; }
+  __device__ __forceinline__ bool sound() const { return s >= 0.25 && s <= 1e12; }
 };
 // An unlisted column's weight is exp2(x * c - m).
 struct Sweep {
@@ -145,35 +145,32 @@ struct MergeShared {
   double s[2][NW];
   float m[2][NW];
 };
-// Workgroup merge of two running pairs per thread, the unlisted columns' and the listed ones': one
-// barrier, the sums in 64 bits, fixed order. `all` is both together. The factors that bring the sums to a
-// common maximum are formed in 64 bits too: the fp32 one is off by up to 6e-8, and with the bucket the two
-// pairs' quotient goes into the loss as it is (2e-5 of a loss of 2e-4).
+// Workgroup merge of a running pair per thread: one barrier, the sums in 64 bits, fixed order. The factors
+// that bring the sums to a common maximum are formed in 64 bits too: the fp32 one is off by up to 6e-8, and
+// with the bucket the quotient of two such sums goes into the loss as it is (2e-5 of a loss of 2e-4).
 template <int NW>
-__device__ __forceinline__ void merge_pairs(const MaxSum& rest_, const MaxSum& listed_, bool with_listed,
-                                            MergeShared<NW>& sh, Pair64* rest, Pair64* all) {
+__device__ __forceinline__ Pair64 merge_pairs(const MaxSum& run, MergeShared<NW>& sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float rm = wave_max(rest_.m);
-  const double rs = wave_sum64((double)rest_.s * exp2_64((double)(rest_.m - rm)));
-  if (lane == 0) { sh.m[0][wave] = rm; sh.s[0][wave] = rs; }
-  if (with_listed) {
-    const float lm = wave_max(listed_.m);
-    const double ls = wave_sum64((double)listed_.s * exp2_64((double)(listed_.m - lm)));
-    if (lane == 0) { sh.m[1][wave] = lm; sh.s[1][wave] = ls; }
-  }
+  const float wm = wave_max(run.m);
+  const double ws = wave_sum64((double)run.s * exp2_64((double)(run.m - wm)));
+  if (lane == 0) { sh.m[0][wave] = wm; sh.s[0][wave] = ws; }
   __syncthreads();
-  const int w = lane & (NW - 1);
-  const float mr = sh.m[0][w];
-  rest->m = group_reduce<NW, OpMax>(mr);
-  rest->s = group_reduce64<NW, Sum64>(sh.s[0][w] * exp2_64((double)(mr - rest->m)));
-  *all = *rest;
-  if (with_listed) {
-    const float ml = sh.m[1][w];
-    const float lm = group_reduce<NW, OpMax>(ml);
-    all->m = fmaxf(rest->m, lm);
-    const double ls = group_reduce64<NW, Sum64>(sh.s[1][w] * exp2_64((double)(ml - all->m)));
-    all->s = rest->s * exp2_64((double)(rest->m - all->m)) + ls;
-  }
+  const float mine = sh.m[0][lane & (NW - 1)];
+  const float m = group_reduce<NW, OpMax>(mine);
+  return Pair64{m, group_reduce64<NW, Sum64>(sh.s[0][lane & (NW - 1)] * exp2_64((double)(mine - m)))};
+}
+// The pair of the unlisted columns with `more`, of the thread's listed ones against rest.m, added: another
+// barrier. A sum past fp32 (more than a few hundred between the two) is not sound.
+template <int NW>
+__device__ __forceinline__ Pair64 with_listed(const Pair64& rest, double more, MergeShared<NW>& sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  more = wave_sum64(more);
+  if (lane == 0) sh.s[1][wave] = more;
+  __syncthreads();
+  const double s = rest.s + group_reduce64<NW, Sum64>(sh.s[1][lane & (NW - 1)]);
+  const double top = (double)rest.m + (double)__builtin_amdgcn_frexp_exp(s);
+  const float m = (float)top;
+  return Pair64{m, __builtin_amdgcn_frexp_mant(s) * exp2_64(top - (double)m)};
 }
 // one element into a running pair
 __device__ __forceinline__ void fold1(MaxSum& run, float x, float c) {
@@ -628,15 +625,13 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     if ((tid & 63) == 0) sh.count[tid >> 6] = c;
   }
 
-  // The sweep leaves the listed logits in sh.x and, for the bucket, folds the two kinds of columns apart.
-  MaxSum run{kNegBig, 0.f}, listed{kNegBig, 0.f};
+  // The sweep leaves the listed logits in sh.x and, for the bucket, folds the others only. (The listed ones are
+  // added from there, by slot: a chain's order is that in which the waves got to its head.)
+  MaxSum run{kNegBig, 0.f};
   auto meet = [&](u32x4& r, int d, int s) {
     const float x = get_elem<T>(r, d);
     sh.x[s] = x;
-    if (bucket) {
-      fold1(listed, x, a.c);
-      set_elem<T>(r, d, bits_of<T>(-INFINITY));
-    }
+    if (bucket) set_elem<T>(r, d, bits_of<T>(-INFINITY));
   };
   auto take = [&](u32x4 r, int c) {       // what the registers of near_of do not cover
     if (c >= sp.nvec) return;
@@ -678,16 +673,20 @@ __global__ __launch_bounds__(THREADS) void kl_topk_kernel(const T* student, List
     if (mask >> 31) {
       walk<1, THREADS, KCAP>(sh, head, col, [&](int, int s) {
         sh.x[s] = x;
-        if (bucket) {
-          fold1(listed, x, a.c);
-          x = -INFINITY;
-        }
+        if (bucket) x = -INFINITY;
       });
     }
     fold1(run, x, a.c);
   }
-  Pair64 rest, all;
-  merge_pairs<NW>(run, listed, bucket, sh.merge, &rest, &all);      // its barrier also publishes sh.x
+  Pair64 rest = merge_pairs<NW>(run, sh.merge);      // its barrier also publishes sh.x
+  Pair64 all = rest;
+  if (bucket) {
+    double more = 0.0;
+#pragma unroll
+    for (int j = 0; j < SL; ++j)
+      if (mine.col[j] >= 0) more += exp2_64((double)sh.x[j * THREADS + tid] * (double)a.c - (double)rest.m);
+    all = with_listed<NW>(rest, more, sh.merge);
+  }
   // (alike in all lanes, and the compiler has to know: behind a lane's branch the row's registers stay taken)
   if (__builtin_expect(__builtin_amdgcn_readfirstlane(rest.sound() && all.sound()) == 0, 0)) {
     exact_pairs<T, THREADS, KCAP>(rp, sp, ne, a.c, bucket, mask, head, sh, &rest, &all);

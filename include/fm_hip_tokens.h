@@ -29,8 +29,8 @@ extern "C" {
  *   FM_TEACHER_PROBS   q = teacher (already at the temperature), divided by its sum for FM_TAIL_RENORM
  * The listed columns and the row's loss are computed in 64 bits (the loss is a small difference),
  * the sweep over the row in fp32.
- * row_loss: fp32 [n]. stats: fp32 [n, 4] for fm_kl_topk_bwd (running maximum and sum of the whole
- * row, then of its unlisted columns, base 2; a negative sum goes with a maximum that is the logit itself,
+ * row_loss: fp32 [n]. stats: fp32 [n, 4] for fm_kl_topk_bwd (base-2 exponent and the sum of weights
+ * against it, of the whole row, then of its unlisted columns; a negative sum goes with the largest logit itself,
  * where masks with the lowest values leave nothing else). loss, n_valid: fp32 device scalars; loss = sum of
  * row_loss (FM_REDUCE_SUM) or that / n_valid (FM_REDUCE_MEAN), n_valid = max(1, rows not skipped);
  * both may be NULL for FM_REDUCE_NONE, which writes neither. 1 <= k <= 1024, k may exceed v;

@@ -676,3 +676,42 @@ def test_a_row_without_a_finite_logit_has_no_gradient_to_give(dt, v, dev):
             (g,) = torch.autograd.grad(out.sum(), x)
             assert out.isnan()[1].item() if reduction == "none" else out.isnan().item()
             assert g[1].isnan().all() and not g[[0, 2]].isnan().any(), (tail, reduction)
+
+
+@gpu
+@pytest.mark.parametrize("dt,v,k", [(F32, 300, 64), (BF16, 3000, 64), (BF16, 40000, 256), (F32, 9000, 1024), (BF16, 131080, 1000)])
+def test_the_order_of_the_slots_changes_no_bit(dt, v, k):
+    # neighbouring columns share vectors and threads; probabilities are multiples of 2^-24, so their sums
+    # are exact in any order
+    n = 6
+    g = torch.Generator().manual_seed(v + k)
+    s = 3 * torch.randn(n, v, generator=g)
+    idx = torch.stack([torch.arange(k) * step % v for step in (1, 2, 3, 5, 7, 1)])
+    idx[5] = v - 1 - torch.arange(k)
+    q = torch.randint(1, 2 ** 24 // k - 1, (n, k), generator=g).float() * 2.0 ** -24
+    live = torch.ones(n, k, dtype=torch.bool)
+    for i in range(n):                       # repeated columns (a step that wraps): one of them stays
+        seen = set()
+        for j in range(k):
+            c = int(idx[i, j])
+            live[i, j] = c not in seen
+            seen.add(c)
+    idx = torch.where(live, idx, -1)
+    sd, di, dq = to_dev(s.to(dt), idx, q)
+    want = None
+    for turn in range(4):
+        order = torch.randperm(k, generator=g)
+        order = torch.cat([torch.zeros(1, dtype=torch.int64), order[order != 0]]) if turn else torch.arange(k)
+        o = order.to(DEV)
+        runs = []
+        for _ in range(2):
+            x = sd.clone().requires_grad_(True)
+            rows = fm.kernels.kl_div_topk(x, di[:, o], dq[:, o], probs=True, tail="bucket", reduction="none")
+            (g1,) = torch.autograd.grad(rows, x, torch.ones(n, device=DEV))
+            y = sd.clone().requires_grad_(True)
+            total = fm.kernels.kl_div_topk(y, di[:, o], dq[:, o], probs=True, tail="bucket", reduction="sum")
+            (g2,) = torch.autograd.grad(total, y)
+            runs.append((rows.detach(), g1, total.detach(), g2))
+        want = want or runs[0]
+        for got in runs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
