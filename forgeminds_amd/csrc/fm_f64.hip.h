@@ -40,43 +40,47 @@ __device__ __forceinline__ double group_reduce64(double v) {
 }
 __device__ __forceinline__ double wave_sum64(double v) { return group_reduce64<64, Sum64>(v); }
 
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+  return __builtin_bit_cast(uint64_t, dpp64<CTRL>(__builtin_bit_cast(double, v)));
+}
+__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int l) {
+  return __builtin_bit_cast(uint64_t, readlane64(__builtin_bit_cast(double, v), l));
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+  v += dpp_u64<kDppXor1>(v);
+  v += dpp_u64<kDppXor2>(v);
+  v += dpp_u64<kDppHalfMirror>(v);
+  v += dpp_u64<kDppMirror>(v);
+  return (readlane_u64(v, 0) + readlane_u64(v, 16)) + (readlane_u64(v, 32) + readlane_u64(v, 48));
+}
 // inclusive prefix sum over the wave in lane order: four shifts inside the rows of sixteen lanes, then
 // the rows' totals
-__device__ __forceinline__ double wave_incl64(double v) {
+__device__ __forceinline__ uint64_t wave_incl_u64(uint64_t v) {
   const int lane = lane_id(), in_row = lane & 15;
-  double t = dpp64<0x111>(v);            // row_shr:1
-  v += in_row >= 1 ? t : 0.0;
-  t = dpp64<0x112>(v);
-  v += in_row >= 2 ? t : 0.0;
-  t = dpp64<0x114>(v);
-  v += in_row >= 4 ? t : 0.0;
-  t = dpp64<0x118>(v);
-  v += in_row >= 8 ? t : 0.0;
-  const double a = readlane64(v, 15), b = readlane64(v, 31), c = readlane64(v, 47);
-  v += lane >= 48 ? (a + b) + c : (lane >= 32 ? a + b : (lane >= 16 ? a : 0.0));
+  uint64_t t = dpp_u64<0x111>(v);            // row_shr:1
+  v += in_row >= 1 ? t : 0ull;
+  t = dpp_u64<0x112>(v);
+  v += in_row >= 2 ? t : 0ull;
+  t = dpp_u64<0x114>(v);
+  v += in_row >= 4 ? t : 0ull;
+  t = dpp_u64<0x118>(v);
+  v += in_row >= 8 ? t : 0ull;
+  const uint64_t a = readlane_u64(v, 15), b = readlane_u64(v, 31), c = readlane_u64(v, 47);
+  v += lane >= 48 ? (a + b) + c : (lane >= 32 ? a + b : (lane >= 16 ? a : 0ull));
   return v;
 }
-// integer sum over the workgroup
+// integer sum over the workgroup, the waves' by DPP
 template <int NW>
-__device__ __forceinline__ unsigned long long block_sum_int64(unsigned long long v, unsigned long long* smem) {
-  auto add = [](unsigned long long x, unsigned long long y) { return x + y; };
-  auto dpp = [](unsigned long long x, auto ctrl) {
-    return __builtin_bit_cast(unsigned long long, dpp64<decltype(ctrl)::value>(__builtin_bit_cast(double, x)));
-  };
-  v = add(v, dpp(v, std::integral_constant<int, kDppXor1>{}));
-  v = add(v, dpp(v, std::integral_constant<int, kDppXor2>{}));
-  v = add(v, dpp(v, std::integral_constant<int, kDppHalfMirror>{}));
-  v = add(v, dpp(v, std::integral_constant<int, kDppMirror>{}));
-  unsigned long long s = 0ull;
-#pragma unroll
-  for (int r = 0; r < 64; r += 16) s += __builtin_bit_cast(unsigned long long, readlane64(__builtin_bit_cast(double, v), r));
-  if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = s;
+__device__ __forceinline__ uint64_t block_sum_int64(uint64_t v, uint64_t* smem) {
+  v = wave_sum_u64(v);
+  if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = v;
   __syncthreads();
-  s = 0ull;
+  v = 0ull;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) s += smem[i];
+  for (int i = 0; i < NW; ++i) v += smem[i];
   __syncthreads();
-  return s;
+  return v;
 }
 
 // across the NW waves of a workgroup; the waves' results are combined by lanes rather than by every

@@ -7,23 +7,29 @@
 //   times the kept mass.
 //
 // Every filter keeps a prefix of the order, so what stays is described by one value and one index:
-// x > cut.x, or x == cut.x and column <= cut.col. The weights and all sums are held in 64 bits: the
-// result is an integer, and a border between two tokens that moves by 1e-8 of the mass (fp32 weights)
-// gives another token once in some ten thousand rows of a broad distribution.
+// x > cut.x, or x == cut.x and column <= cut.col. The weights are computed in 64 bits: the result is an
+// integer, and a border between two tokens that moves by 1e-8 of the mass (fp32 weights) gives another
+// token once in some ten thousand rows of a broad distribution. From there on they are integers: a weight
+// counts as the nearest multiple of 2^-fx (fx = 50 up to 8192 columns, 46 up to 2^17, 43 for 2^20), all sums
+// are exact, and a decision is a comparison of integers. So a row's result is the same whichever of the
+// ways below it takes, in whatever order its sums are formed: workgroup sizes go by the number of rows, and
+// a row alone is the row among many. What rounding remains is half a unit an element: v 2^-(fx + 1) of a mass
+// of at least 1 at worst, 9e-10 for 2^17 columns and 6e-8 for 2^20, the square root of that many units in
+// earnest (1e-12).
 //
 // One workgroup per row, which reads it once from memory and again from the caches:
 //   1  maximum of the row (NaN propagates)
 //   2  candidates: the elements from the maximum down to a bound at or below the cut, into a list in LDS.
 //      top-k: the waves' thread maxima vouch for k elements above the bound. min-p: its own bound. top-p
 //      alone (and a top-k whose list overflows): a histogram of the row's masses (or counts) over 2048 equal
-//      steps of the logit names the step that holds the cut; masses are 64-bit fixed point, so that the sum
-//      is the same in any order
+//      steps of the logit names the step that holds the cut
 //   3  the exact cut: histograms of the list narrow it to one step, whose elements are put in order. A step
 //      with more elements than that is searched by the bits of the value; among equal values the cut is a
 //      count, which the last sweep turns into a column
 //   4  token: masses of the segments in index order, the segment that holds u, the token in it -- from the
 //      list, or over the row again where the list is too long (flat rows)
-// Where nothing cuts, one sweep does: each segment's masses against its own maximum.
+// Where nothing cuts, one sweep does: each segment's weights against its own maximum, summed in 64 bits in an
+// order of the segment's own, brought to the row's maximum and rounded to the unit then.
 // Weights are computed for the candidates only, unless the mass of the whole row is asked for.
 //
 // What bounds it: the arithmetic of those weights, some 27 instructions an element with the histogram, on
@@ -120,6 +126,7 @@ __device__ __forceinline__ float uniform(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 __device__ __forceinline__ double uniform(double v) { return readlane64(v, 0); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) { return readlane_u64(v, 0); }
 
 // element e of a vector
 template <typename T>
@@ -148,26 +155,26 @@ struct SampleShared {
   static constexpr int kSegs = 1040;   // segments (v <= 2^20)
   struct {
     unsigned long long bins[kBins];
-    unsigned long long list[kList];       // (key << 32) | ~column: larger comes first
-    unsigned long long step[kStep];       // the candidates of one step or segment ...
-    unsigned long long mass[kStep];       // ... and their weights
+    uint64_t list[kList];       // (key << 32) | ~column: larger comes first
+    uint64_t step[kStep];       // the candidates of one step or segment ...
+    uint64_t mass[kStep];       // ... and their weights
   } h;
   u32x4 edges[2];
-  double seg[kSegs];
-  float segm[kSegs];
+  uint64_t seg[kSegs];
+  union {
+    float segm[kSegs];        // where nothing cuts: the segments' maxima
+    int ties[kSegs];          // else: their elements equal to the cut
+  };
   double red[THREADS / 64];
   float redf[1][THREADS / 64];
-  unsigned long long redu[THREADS / 64];
+  uint64_t redu[THREADS / 64];
   int redi[THREADS / 64];
   int count;
   int at;
-  int col;
   uint32_t klo, khi;
-  unsigned long long hits[4];
-  double hitw[4], lastw[4];
-  int lasts[4];
-  float x;
-  double weight;
+  int hits[4], lasts[4];
+  float hitx[4], lastx[4];
+  uint64_t before;
 };
 
 // exp((x - m) / T) = 2^((x - m) c), c = log2(e) / T, by the polynomial of exp2_64, written out for several elements at once:
@@ -228,49 +235,34 @@ __device__ __forceinline__ int thread_here() {
   return t;
 }
 
-// First of `n` non-negative entries (in LDS, in order) whose running sum reaches `target`
-// (strict: exceeds it); *before is the sum ahead of it. n when there is none. All threads call it.
-template <int THREADS, bool STRICT, typename F>
-__device__ __forceinline__ int find_running(F entry, int n, double target, SampleShared<THREADS>& sh, double* before) {
+// First of `n` entries (in LDS, in order) at which the running sum reaches `goal` (at least 1); *before is the
+// sum ahead of it. n when there is none. All threads call it.
+template <int THREADS, typename F>
+__device__ __forceinline__ int find_running(F entry, int n, uint64_t goal, SampleShared<THREADS>& sh, uint64_t* before) {
   constexpr int NW = THREADS / 64;
   const int tid = thread_here(), lane = tid & 63, wave = tid >> 6;
   const int per = (n + THREADS - 1) / THREADS;
-  auto there = [&](double run) { return STRICT ? run > target : run >= target; };
-  double mine = 0.0;
+  uint64_t mine = 0ull;
   for (int i = 0; i < per; ++i) {
     const int at = tid * per + i;
     if (at < n) mine += entry(at);
   }
-  const double incl = wave_incl64(mine);
-  if (lane == 63) sh.red[wave] = incl;
-  if (tid == 0) { sh.at = n; sh.weight = 0.0; }
+  uint64_t end = wave_incl_u64(mine);
+  if (lane == 63) sh.redu[wave] = end;
+  if (tid == 0) { sh.at = n; sh.before = 0ull; }
   __syncthreads();
-  double ahead = 0.0;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) if (i < wave) ahead += sh.red[i];
-  // the sum ahead of a lane is the very number that the lane before it compares
-  const double mine_end = ahead + incl;
-  double mine_start = __shfl_up(mine_end, 1, 64);
-  if (lane == 0) mine_start = ahead;
-  int at = n;
-  double run = mine_start;
-  if (there(mine_end) && (tid == 0 || !there(mine_start))) {
-    at = tid * per;
-    for (int i = 0; i < per; ++i) {
-      const double end = i == per - 1 ? mine_end : run + entry(at);
-      if (i == per - 1 || there(end)) break;
-      run = end;
-      ++at;
-    }
-    at = at < n ? at : n - 1;
-    // (rounding may let the sums of neighbouring lanes dip: the first one counts)
-    atomicMin(&sh.at, at);
+  for (int i = 0; i < NW; ++i) if (i < wave) end += sh.redu[i];
+  uint64_t run = end - mine;
+  if (run < goal && goal <= end) {        // one thread at most
+    int at = tid * per;
+    for (uint64_t w = entry(at); run + w < goal; w = entry(at)) { run += w; ++at; }
+    sh.at = at;
+    sh.before = run;
   }
   __syncthreads();
   const int found = uniform(sh.at);
-  if (at < n && at == found) sh.weight = run;
-  __syncthreads();
-  *before = uniform(sh.weight);
+  *before = uniform(sh.before);
   __syncthreads();
   return found;
 }
@@ -309,91 +301,67 @@ __device__ __forceinline__ void each_element(const RowView<T>& rv, F fn) {
 // for G vectors a lane.
 constexpr int seg_vecs(int G) { return 64 * G; }
 
-// The weights of this lane's vector of block `block` of the row (0 past its end) and their sum.
-template <typename T, typename F>
-__device__ __forceinline__ double block_weights(const RowView<T>& rv, int block, F weights_of, double* w) {
-  constexpr int EPV = Elem<T>::kVec;
-  const int c = block * 64 + (threadIdx.x & 63);
-  double mine = 0.0;
-#pragma unroll
-  for (int e = 0; e < EPV; ++e) w[e] = 0.0;
-  if (c < rv.nvec) {
-    float x[EPV];
-    Elem<T>::unpack(rv.load(c), x);
-    weights_of(x, rv.col0(c), w);
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) mine += w[e];
-  }
-  return mine;
-}
-
-// The first column whose running weight exceeds `target`, from the weights of the nseg segments:
-// weights_of(x, col0, w) gives those of a vector. Rounding may leave the target at the very end: then the
-// last column with a weight. Returns the column; *w is its weight, *seg its segment, *ahead the weight in
-// front of that.
+// The first column at which the running weight reaches `goal`, from the weights of the nseg segments:
+// weights_of(x, col0, w) gives those of a vector, as integers. (Where nothing cuts, a segment's rounded weight
+// may be a few units more than its elements' together: then its last column with a weight.) Returns the
+// column; *x is its logit, *seg its segment, *ahead the weight in front of that.
 template <typename T, int THREADS, int G, typename E, typename F>
-__device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, E entry, double target, F weights_of,
-                                    SampleShared<THREADS>& sh, double* w, int* seg, double* ahead) {
+__device__ __forceinline__ int pick(const RowView<T>& rv, int nseg, E entry, uint64_t goal, F weights_of,
+                                    SampleShared<THREADS>& sh, float* x_at, int* seg, uint64_t* ahead) {
   constexpr int EPV = Elem<T>::kVec;
   static_assert(G <= THREADS / 64, "a wave per block of the segment");
-  double before;
-  int s = find_running<THREADS, true>(entry, nseg, target, sh, &before);
-  const bool end = s == nseg;
-  if (end) {          // the last segment with a weight
-    if (threadIdx.x == 0) sh.at = 0;
-    __syncthreads();
-    for (int i = thread_here(); i < nseg; i += THREADS) if (entry(i) > 0.0) atomicMax(&sh.at, i);
-    __syncthreads();
-    s = uniform(sh.at);
-    __syncthreads();
-  }
+  uint64_t before;
+  int s = find_running<THREADS>(entry, nseg, goal, sh, &before);
+  s = s < nseg ? s : nseg - 1;
   *seg = s;
   *ahead = before;
   // its blocks, a wave each
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double wt[EPV], mine = 0.0, incl = 0.0;
+  const int c = (s * G + wave) * 64 + lane;
+  float x[EPV], kept[EPV];
+  uint64_t w[EPV], mine = 0ull, incl = 0ull;
+#pragma unroll
+  for (int e = 0; e < EPV; ++e) { x[e] = -INFINITY; w[e] = 0ull; }
   if (wave < G) {
-    mine = block_weights<T>(rv, s * G + wave, weights_of, wt);
-    incl = wave_incl64(mine);
-    if (lane == 63) sh.red[wave] = incl;
+    if (c < rv.nvec) {
+      Elem<T>::unpack(rv.load(c), x);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) kept[e] = x[e];
+      weights_of(kept, rv.col0(c), w);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) mine += w[e];
+    }
+    incl = wave_incl_u64(mine);
+    if (lane == 63) sh.redu[wave] = incl;
   }
-  if (threadIdx.x == 0) sh.col = -1;
   __syncthreads();
-  for (int g = 0; g < G; ++g) if (g < wave) before += sh.red[g];
-  int last = -1;
-  double last_w = 0.0;
+  for (int g = 0; g < G; ++g) if (g < wave) before += sh.redu[g];
   if (wave < G) {
-    double run = before + (incl - mine);
-    int hit = -1;
-    double hit_w = 0.0;
-    const int col0 = rv.col0((s * G + wave) * 64 + lane);
+    uint64_t run = before + (incl - mine);
+    int hit = -1, last = -1;
+    float hit_x = 0.f, last_x = 0.f;
 #pragma unroll
     for (int e = 0; e < EPV; ++e) {
-      run += wt[e];
-      if (wt[e] > 0.0) {
-        last = col0 + e;
-        last_w = wt[e];
-        if (!end && hit < 0 && run > target) { hit = col0 + e; hit_w = wt[e]; }
+      run += w[e];
+      if (w[e] != 0ull) {
+        last = rv.col0(c) + e;
+        last_x = x[e];
+        if (hit < 0 && run >= goal) { hit = last; hit_x = x[e]; }
       }
     }
+    // the first hit of the wave; of the waves' again the first
     const unsigned long long any = __ballot(hit >= 0), some = __ballot(last >= 0);
-    // the first hit of the wave; the waves' ones by column, the first one again
-    if (any != 0ull && lane == __builtin_ctzll(any)) sh.hits[wave] = (unsigned long long)(uint32_t)hit;
-    else if (any == 0ull && lane == 0) sh.hits[wave] = ~0ull;
-    const int top = some != 0ull ? 63 - __builtin_clzll(some) : 0;
-    last = __shfl(last, top, 64);
-    last_w = __shfl(last_w, top, 64);
-    if (any != 0ull && lane == __builtin_ctzll(any)) sh.hitw[wave] = hit_w;
-    if (lane == 0) { sh.lasts[wave] = last; sh.lastw[wave] = last_w; }
+    if (any != 0ull ? lane == __builtin_ctzll(any) : lane == 0) { sh.hits[wave] = hit; sh.hitx[wave] = hit_x; }
+    if (some != 0ull ? lane == 63 - __builtin_clzll(some) : lane == 0) { sh.lasts[wave] = last; sh.lastx[wave] = last_x; }
   }
   __syncthreads();
   int col = -1;
-  double cw = 0.0;
-  for (int g = G - 1; g >= 0; --g) if (sh.hits[g] != ~0ull) { col = (int)(uint32_t)sh.hits[g]; cw = sh.hitw[g]; }
+  float xc = 0.f;
+  for (int g = G - 1; g >= 0; --g) if (sh.hits[g] >= 0) { col = sh.hits[g]; xc = sh.hitx[g]; }
   if (col < 0)
-    for (int g = 0; g < G; ++g) if (sh.lasts[g] >= 0) { col = sh.lasts[g]; cw = sh.lastw[g]; }
+    for (int g = 0; g < G; ++g) if (sh.lasts[g] >= 0) { col = sh.lasts[g]; xc = sh.lastx[g]; }
   __syncthreads();
-  *w = cw;
+  *x_at = xc;
   return col;
 }
 
@@ -430,9 +398,8 @@ __device__ __forceinline__ void each_segment(const RowView<T>& rv, int nseg, F f
 // neighbours of a thread are added up before they go to the histogram, so that a row of few values does
 // not queue on few addresses.
 template <typename T, int THREADS, typename F>
-__device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo, uint32_t hi, unsigned long long ahead,
-                                               double goal, F amount, SampleShared<THREADS>& sh,
-                                               unsigned long long* above) {
+__device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo, uint32_t hi, uint64_t ahead,
+                                               uint64_t goal, F amount, SampleShared<THREADS>& sh, uint64_t* above) {
   while (lo < hi) {
     const int bits = 32 - __builtin_clz(hi - lo);
     const int shift = bits > 11 ? bits - 11 : 0;
@@ -440,34 +407,24 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
     for (int i = thread_here(); i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
     __syncthreads();
     int open = -1;
-    unsigned long long held = 0ull;
+    uint64_t held = 0ull;
     each_element<T, THREADS>(rv, [&](float x, int col) {
       const uint32_t key = key_of(x);
       if (key < lo || key > hi || col < 0 || col >= rv.v) return;
       const int b = (int)((hi - key) >> shift);
       if (b != open) {
-        if (open >= 0) atomicAdd(&sh.h.bins[open], held);
+        if (open >= 0) atomicAdd(&sh.h.bins[open], (unsigned long long)held);
         open = b;
         held = 0ull;
       }
       held += amount(x);
     });
-    if (open >= 0) atomicAdd(&sh.h.bins[open], held);
+    if (open >= 0) atomicAdd(&sh.h.bins[open], (unsigned long long)held);
     __syncthreads();
-    double before;
-    int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal - (double)ahead, sh, &before);
-    if (b == kBins) {       // rounding: everything stays, the lowest value is the cut
-      if (threadIdx.x == 0) sh.at = 0;
-      __syncthreads();
-      for (int i = thread_here(); i < kBins; i += THREADS) if (sh.h.bins[i] != 0ull) atomicMax(&sh.at, i);
-      __syncthreads();
-      b = uniform(sh.at);
-    }
-    // the amount ahead of that range, as an integer
-    unsigned long long mine = 0ull;
-    for (int i = thread_here(); i < b; i += THREADS) mine += sh.h.bins[i];
-    mine = block_sum_int64<THREADS / 64>(mine, sh.redu);
-    ahead += ((unsigned long long)(uint32_t)uniform((int)(mine >> 32)) << 32) | (uint32_t)uniform((int)(uint32_t)mine);
+    uint64_t before;
+    int b = find_running<THREADS>([&](int i) { return (uint64_t)sh.h.bins[i]; }, kBins, goal - ahead, sh, &before);
+    b = b < kBins ? b : kBins - 1;       // (some range reaches it)
+    ahead += before;
     const uint32_t top = hi - ((uint32_t)b << shift);
     const uint32_t span = (1u << shift) - 1u;
     lo = top - lo > span ? top - span : lo;
@@ -481,11 +438,11 @@ __device__ __forceinline__ uint32_t key_search(const RowView<T>& rv, uint32_t lo
 // Column of the c-th (1-based) element equal to x0 > -inf in index order; INT_MAX when there are no more
 // than c.
 template <typename T, int THREADS, int G>
-__device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x0, double c, SampleShared<THREADS>& sh) {
+__device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x0, int c, SampleShared<THREADS>& sh) {
   constexpr int EPV = Elem<T>::kVec;
-  auto equal = [&](float* x, int, double* w) __attribute__((always_inline)) {
+  auto equal = [&](float* x, int, uint64_t* w) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) w[e] = x[e] == x0 ? 1.0 : 0.0;
+    for (int e = 0; e < EPV; ++e) w[e] = x[e] == x0 ? 1ull : 0ull;
   };
   int count = 0;
   __syncthreads();
@@ -497,18 +454,19 @@ __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x
         for (int e = 0; e < EPV; ++e) count += x[e] == x0 ? 1 : 0;
       },
       [&](int s) {
-        const float all = wave_sum((float)count);
-        if ((threadIdx.x & 63) == 0) sh.seg[s] = (double)all;
+        const int all = wave_sum_i(count);
+        if ((threadIdx.x & 63) == 0) sh.ties[s] = all;
         count = 0;
       });
   __syncthreads();
-  double mine = 0.0;
-  for (int i = thread_here(); i < nseg; i += THREADS) mine += sh.seg[i];
-  const double all = block_reduce64<THREADS / 64, Sum64>(mine, sh.red);
-  if (c >= all) return 0x7fffffff;
-  double w, before;
+  uint64_t mine = 0ull;
+  for (int i = thread_here(); i < nseg; i += THREADS) mine += (uint64_t)sh.ties[i];
+  const uint64_t all = uniform(block_sum_int64<THREADS / 64>(mine, sh.redu));
+  if ((uint64_t)c >= all) return 0x7fffffff;
+  float x;
+  uint64_t before;
   int s;
-  return pick<T, THREADS, G>(rv, nseg, [&](int i) { return sh.seg[i]; }, c - 0.5, equal, sh, &w, &s, &before);
+  return pick<T, THREADS, G>(rv, nseg, [&](int i) { return (uint64_t)sh.ties[i]; }, (uint64_t)c, equal, sh, &x, &s, &before);
 }
 
 // Few entries, their amounts in sh.h.mass: fn(i, amount ahead of entry i, its own, all) for each of them, on
@@ -517,14 +475,14 @@ __device__ __forceinline__ int nth_equal(const RowView<T>& rv, int nseg, float x
 // search in it, or a sort ([1,128256] bf16 min-p: 12 us, 15 without; top-p 0.9: 39, 43 without). The amounts
 // are integers, the sums exact.
 template <int THREADS, typename K, typename F>
-__device__ __forceinline__ void each_of_few(const unsigned long long* from, int n, SampleShared<THREADS>& sh, K key, F fn) {
+__device__ __forceinline__ void each_of_few(const uint64_t* from, int n, SampleShared<THREADS>& sh, K key, F fn) {
   const int tid = thread_here(), part = tid & 7;
   for (int i0 = 0; i0 < n; i0 += THREADS / 8) {
     const int i = i0 + (tid >> 3);
     const auto mine = key(from[i < n ? i : n - 1]);
-    unsigned long long ahead = 0ull, all = 0ull;
+    uint64_t ahead = 0ull, all = 0ull;
     for (int o = part; o < n; o += 8) {
-      const unsigned long long w = sh.h.mass[o];
+      const uint64_t w = sh.h.mass[o];
       all += w;
       ahead += key(from[o]) > mine ? w : 0ull;
     }
@@ -548,7 +506,7 @@ __device__ __forceinline__ void sort_step(SampleShared<THREADS>& sh, int n) {
     for (int j = k / 2; j > 0; j /= 2) {
       for (int p = thread_here(); p < N / 2; p += THREADS) {
         const int i = 2 * p - (p & (j - 1)), o = i + j;
-        const unsigned long long a = sh.h.step[i], b = sh.h.step[o];
+        const uint64_t a = sh.h.step[i], b = sh.h.step[o];
         const bool up = (i & k) != 0;            // ascending half
         if ((a < b) != up) { sh.h.step[i] = b; sh.h.step[o] = a; }
       }
@@ -599,6 +557,14 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
   float m;
   uint32_t vouch = 0u;
   const bool whole = t_ok && T_ > 0.f && !use_k && !use_p && !use_m;
+  // 2^fx units of mass per 1: the sum of v weights of at most 1 stays at or below 2^63
+  const int vbits = a.v > 1 ? 32 - __builtin_clz((unsigned)a.v - 1u) : 0;
+  const int fx = 63 - vbits < 50 ? 63 - vbits : 50;
+  const double unit = __builtin_amdgcn_ldexp(1.0, fx);
+  // w * unit to the nearest integer (w <= 1 and unit <= 2^50: below 2^52), above the bits of 2^52
+  constexpr uint64_t kAbove = 0x4330000000000000ull;
+  auto fixed_above = [&](double w) { return __builtin_bit_cast(uint64_t, __builtin_fma(w, unit, 4503599627370496.0)); };
+  auto fixed = [&](double w) { return fixed_above(w) - kAbove; };
   if (whole) {
     // Nothing cuts: one sweep, each segment's weights against its own maximum, brought together below.
     const double c = kLog2ed / (double)T_;
@@ -635,14 +601,16 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         }
       }
       mine = wave_sum64(mine);
-      if ((tid & 63) == 0) { sh.seg[s] = mine; sh.segm[s] = top; }
+      if ((tid & 63) == 0) { sh.seg[s] = __builtin_bit_cast(uint64_t, mine); sh.segm[s] = top; }
     }
     __syncthreads();
     m = -INFINITY;
     for (int i = tid & 63; i < nseg; i += 64) m = __builtin_elementwise_maximum(m, sh.segm[i]);
     m = uniform(group_reduce<64, OpMaximum>(m));
     if (!(m < INFINITY && m > -INFINITY)) { no_row(); return; }
-    for (int i = tid; i < nseg; i += THREADS) sh.seg[i] *= exp2_64(((double)sh.segm[i] - (double)m) * c);
+    for (int i = tid; i < nseg; i += THREADS)
+      sh.seg[i] = (uint64_t)__builtin_rint(__builtin_bit_cast(double, sh.seg[i]) *
+                                           (exp2_64(((double)sh.segm[i] - (double)m) * c) * unit));
     __syncthreads();
   } else {
     // 1: the maximum; NaN propagates
@@ -709,7 +677,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       for (int e = 0; e < EPV; ++e) x[e] = x[e] >= from ? x[e] : -INFINITY;
     }
   };
-  double ties = 0.0;                // > 0: so many of the elements equal to cut.x stay, and cut.col is not known
+  int ties = 0;                     // > 0: so many of the elements equal to cut.x stay, and cut.col is not known
   if (!whole) {
     float x_min = -INFINITY;          // min-p: the least value with a weight of min_p
     if (use_m) {
@@ -718,16 +686,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       if ((double)x_min < xm) x_min = float_of_key(key_of(x_min) + 1u);      // the next float up
       if (x_min > m) x_min = m;
     }
-    // 2^fx units of mass per 1: the sum of v weights of at most 1 stays below 2^62
-    const int vbits = 62 - (32 - __builtin_clz((unsigned)a.v));
-    const int fx = vbits < 50 ? vbits : 50;
-    const double unit = __builtin_amdgcn_ldexp(1.0, fx);
-    // w * unit to the nearest integer (w <= 1 and unit <= 2^50: below 2^52)
-    auto fixed = [&](double w) {
-      return __builtin_bit_cast(unsigned long long, __builtin_fma(w, unit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-    };
-    auto value = [](unsigned long long e) { return float_of_key((uint32_t)(e >> 32)); };
-    auto column = [](unsigned long long e) { return (int)~(uint32_t)e; };
+    auto value = [](uint64_t e) { return float_of_key((uint32_t)(e >> 32)); };
+    auto column = [](uint64_t e) { return (int)~(uint32_t)e; };
 
     // steps of equal width from the maximum down
     float per = 0.f;
@@ -746,10 +706,10 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     bool listed = false;
     int n = 0, nb = 0;
     auto entry_of = [&](const u32x4& r, int c, int e) __attribute__((always_inline)) {
-      return ((unsigned long long)key_of(element<T>(r, e)) << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
+      return ((uint64_t)key_of(element<T>(r, e)) << 32) | (uint32_t)~(uint32_t)(rv.col0(c) + e);
     };
     // `entry` of the lanes `who` behind what the waves before this one put there; false past the end
-    auto put = [&](int& count, unsigned long long* to, int room, unsigned long long who, bool mine, unsigned long long entry) __attribute__((always_inline)) {
+    auto put = [&](int& count, uint64_t* to, int room, unsigned long long who, bool mine, uint64_t entry) __attribute__((always_inline)) {
       int base = 0;
       const int first = __builtin_ctzll(who);
       if ((threadIdx.x & 63) == first) base = atomicAdd(&count, (int)__builtin_popcountll(who));
@@ -829,18 +789,23 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     };
 
     // the amounts of entries, 0 for what the cut so far does not keep, into sh.h.mass
-    auto amounts = [&](const unsigned long long* from, int many, auto by_count) __attribute__((always_inline)) {
+    auto amounts = [&](const uint64_t* from, int many, auto by_count) __attribute__((always_inline)) {
       const Weight weight = base.fresh();
 #pragma unroll 1
       for (int i = tid; i < many; i += THREADS) {
-        const unsigned long long e = from[i];
+        const uint64_t e = from[i];
         sh.h.mass[i] = !kept(value(e), column(e)) ? 0ull : decltype(by_count)::value ? 1ull : fixed(weight(value(e)));
       }
       __syncthreads();
     };
 
     // 3: the exact cuts, first by count, then by the mass of what that leaves. The cut is the first element,
-    // in descending order, at which the running amount reaches the goal.
+    // in descending order, at which the running amount reaches the goal (the mass before it is below p times
+    // the whole: the first multiple of the unit that is not).
+    auto goal_of = [&](uint64_t mass) {
+      const uint64_t g = (uint64_t)__builtin_ceil((double)p * (double)mass);
+      return uniform(g > 1ull ? g : (uint64_t)1);
+    };
     if (use_k) {
       bound = vouch <= 0x007FFFFFu ? -INFINITY : float_of_key(vouch);      // that is key_of(-inf)
       const float range = m - bound;
@@ -861,21 +826,21 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       __syncthreads();
       // the amount by step
       const Weight weight = base.fresh();
-      double goal;
+      uint64_t goal = (uint64_t)(count ? k : 0);
       if (by_list) {
-        unsigned long long mine = 0ull;
+        uint64_t mine = 0ull;
 #pragma unroll 1
         for (int i = tid; i < n; i += THREADS) {
-          const unsigned long long e = sh.h.list[i];
+          const uint64_t e = sh.h.list[i];
           if (!kept(value(e), column(e))) continue;
-          const unsigned long long w = count ? 1ull : fixed(weight(value(e)));
+          const uint64_t w = count ? 1ull : fixed(weight(value(e)));
           const float y = step_of(value(e));
-          atomicAdd(&sh.h.bins[y < last_bin ? (int)y : kBins - 1], w);
+          atomicAdd(&sh.h.bins[y < last_bin ? (int)y : kBins - 1], (unsigned long long)w);
           mine += w;
         }
-        goal = (double)p * (double)block_sum_int64<NW>(mine, sh.redu);
+        if (!count) goal = goal_of(block_sum_int64<NW>(mine, sh.redu));
       } else {
-        double total = 0.0;
+        uint64_t total = 0ull;
         each([&](const u32x4& r, int c) {
           float x[EPV];
           Elem<T>::unpack(r, x);
@@ -889,21 +854,22 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
           } else {
             double w[EPV];
             weight.template eval<EPV>(x, w);
+            total -= EPV * kAbove;
 #pragma unroll
             for (int e = 0; e < EPV; ++e) {
-              total += w[e];
+              const uint64_t f = fixed_above(w[e]);
+              total += f;
               const float y = step_of(x[e]);
-              if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], fixed(w[e]));
+              if (y < last_bin) atomicAdd(&sh.h.bins[(int)y], (unsigned long long)(f - kAbove));
             }
           }
         });
-        goal = (double)p * block_reduce64<NW, Sum64>(total, sh.red) * unit;
+        if (!count) goal = goal_of(block_sum_int64<NW>(total, sh.redu));
       }
-      goal = count ? (double)k : uniform(goal);
       __syncthreads();
       // the step that holds the cut, its elements in sh.h.step
-      double ahead;
-      const int b = find_running<THREADS, false>([&](int i) { return (double)sh.h.bins[i]; }, kBins, goal, sh, &ahead);
+      uint64_t ahead;
+      const int b = find_running<THREADS>([&](int i) { return (uint64_t)sh.h.bins[i]; }, kBins, goal, sh, &ahead);
       if (by_list && b == kBins) return;         // everything stays
       if (!by_list && b < kBins) {
         // How many there are at least, from the mass and the largest weight of each step: rows whose list or
@@ -925,7 +891,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         __syncthreads();
 #pragma unroll 1
         for (int i = tid; i < n; i += THREADS) {
-          const unsigned long long e = sh.h.list[i];
+          const uint64_t e = sh.h.list[i];
           const float y = step_of(value(e));
           if ((y < last_bin ? (int)y : kBins - 1) == b && kept(value(e), column(e))) {
             const int at = atomicAdd(&sh.at, 1);
@@ -941,11 +907,10 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         amounts(sh.h.step, nb, by_count);
         if (tid == 0) sh.at = 0;
         __syncthreads();
-        const double left = goal - ahead;
-        each_of_few<THREADS>(sh.h.step, nb, sh, [](unsigned long long e) { return e; },
-            [&](int i, unsigned long long before, unsigned long long w, unsigned long long all) {
-              // the first whose running amount reaches the goal, or else the last
-              if (w > 0ull && (before == 0ull || (double)before < left) && ((double)(before + w) >= left || before + w == all)) sh.at = i;
+        const uint64_t left = goal - ahead;
+        each_of_few<THREADS>(sh.h.step, nb, sh, [](uint64_t e) { return e; },
+            [&](int i, uint64_t before, uint64_t w, uint64_t) {
+              if (before < left && left <= before + w) sh.at = i;      // one entry
             });
         __syncthreads();
         cut.x = uniform(value(sh.h.step[sh.at]));
@@ -955,9 +920,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       }
       if (b < kBins && nb <= kStep) {
         sort_step<THREADS>(sh, nb);
-        double unused;
-        int r = find_running<THREADS, false>(
-            [&](int i) { return count ? 1.0 : (double)fixed(weight(value(sh.h.step[i]))); }, nb, goal - ahead, sh, &unused);
+        uint64_t unused;
+        int r = find_running<THREADS>(
+            [&](int i) { return count ? (uint64_t)1 : fixed(weight(value(sh.h.step[i]))); }, nb, goal - ahead, sh, &unused);
         r = r < nb ? r : nb - 1;
         cut.x = uniform(value(sh.h.step[r]));
         cut.col = uniform(column(sh.h.step[r]));
@@ -965,19 +930,22 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       }
       // More elements than that: by the bits of the value, then by column among equal ones.
       uint32_t lo = 0u, hi = 0xFFFFFFFEu;
-      unsigned long long above = 0ull;
+      uint64_t above = 0ull;
       if (b < kBins) {
         lo = (uint32_t)uniform((int)sh.klo);
         hi = (uint32_t)uniform((int)sh.khi);
-        above = (unsigned long long)ahead;
+        above = ahead;
       }
       const uint32_t key = key_search<T, THREADS>(
-          rv, lo, hi, above, goal, [&](float x) { return count ? 1ull : fixed(weight(x)); }, sh, &above);
+          rv, lo, hi, above, goal, [&](float x) { return count ? (uint64_t)1 : fixed(weight(x)); }, sh, &above);
       const float x = float_of_key(key);
-      const double each_w = count ? 1.0 : (double)fixed(weight(x));
+      const uint64_t each_w = count ? (uint64_t)1 : fixed(weight(x));
       // the r-th of the equal ones stays iff above + (r - 1) * weight < goal
-      double need = each_w > 0.0 ? ceil((goal - (double)above) / each_w) : 1.0;
-      need = uniform(need >= 1.0 ? need : 1.0);
+      const uint64_t left = goal - above;
+      uint64_t r = each_w > 0ull ? (uint64_t)((double)left / (double)each_w) : 1ull;       // the quotient, or one off
+      if (r * each_w < left) ++r;
+      if (r > 1ull && (r - 1ull) * each_w >= left) --r;
+      const int need = uniform((int)(r > 1ull ? r : 1ull));
       if (!count || !use_p) {       // the last cut: the sweep below counts the equal ones by the way
         listed = false;
         if (x > cut.x) {
@@ -993,7 +961,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     if (use_k) settle(std::true_type{});
     if (use_p) settle(std::false_type{});
     if (x_min > cut.x) {       // every value equal to the bound stays
-      ties = 0.0;
+      ties = 0;
       cut.x = x_min;
       cut.col = 0x7fffffff;
     }
@@ -1002,11 +970,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
     if (listed && n <= kFew) {
       amounts(sh.h.list, n, std::false_type{});
       // larger: of a lower index
-      each_of_few<THREADS>(sh.h.list, n, sh, [](unsigned long long e) { return (uint32_t)e; },
-          [&](int i, unsigned long long ahead, unsigned long long w, unsigned long long all) {
-            const double target = u * (double)all;
-            if ((tid & 7) == 0 && (double)ahead <= target && target < (double)(ahead + w)) {
-              const unsigned long long e = sh.h.list[i];
+      each_of_few<THREADS>(sh.h.list, n, sh, [](uint64_t e) { return (uint32_t)e; },
+          [&](int i, uint64_t ahead, uint64_t w, uint64_t all) {
+            const uint64_t target = (uint64_t)(u * (double)all);
+            if ((tid & 7) == 0 && ahead <= target && target < ahead + w) {
+              const uint64_t e = sh.h.list[i];
               a.token[row] = column(e);
               if (a.logprob != nullptr)
                 a.logprob[row] = (float)(log2_64(base(value(e)) * unit / (double)all) * kLn2d);
@@ -1023,7 +991,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       for (int i = tid; i < kBins; i += THREADS) sh.h.bins[i] = 0ull;
       __syncthreads();
       const Weight weight = base.fresh();
-      unsigned long long me[PER], w[PER], mine = 0ull;
+      uint64_t me[PER], w[PER], mine = 0ull;
       int seg[PER];
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
@@ -1035,14 +1003,14 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
         if (!kept(value(me[j]), column(me[j]))) continue;
         w[j] = fixed(weight(value(me[j])));
         seg[j] = (int)(((uint32_t)column(me[j]) + (uint32_t)rv.lead) >> seg_bits);
-        atomicAdd(&sh.h.bins[seg[j]], w[j]);
+        atomicAdd(&sh.h.bins[seg[j]], (unsigned long long)w[j]);
         mine += w[j];
       }
       const double mass = uniform((double)block_sum_int64<NW>(mine, sh.redu));
-      const double target = u * mass;
-      double ahead;
-      const int s = find_running<THREADS, true>([&](int i) { return (double)sh.h.bins[i]; }, kBins, target, sh, &ahead);
-      if (tid == 0) { sh.at = 0; sh.col = -1; }
+      const uint64_t target = uniform((uint64_t)(u * mass));
+      uint64_t ahead;
+      const int s = find_running<THREADS>([&](int i) { return (uint64_t)sh.h.bins[i]; }, kBins, target + 1ull, sh, &ahead);
+      if (tid == 0) sh.at = 0;
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
@@ -1056,90 +1024,93 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const T* __restrict__ l
       const int ns = uniform(sh.at);
       for (int i = tid; i < ns; i += THREADS) {
         const int col = column(sh.h.step[i]);
-        unsigned long long before = 0ull;
+        uint64_t before = ahead;
         for (int o = 0; o < ns; ++o) before += column(sh.h.step[o]) < col ? sh.h.mass[o] : 0ull;
-        if (ahead + (double)before <= target && target < ahead + (double)(before + sh.h.mass[i])) {
-          sh.col = col;
-          sh.x = value(sh.h.step[i]);
+        if (before <= target && target < before + sh.h.mass[i]) {
+          a.token[row] = col;
+          if (a.logprob != nullptr)
+            a.logprob[row] = (float)(log2_64(weight(value(sh.h.step[i])) * unit / mass) * kLn2d);
         }
       }
-      __syncthreads();
-      if (sh.col >= 0) {
-        if (tid == 0) {
-          a.token[row] = sh.col;
-          if (a.logprob != nullptr) a.logprob[row] = (float)(log2_64(weight(sh.x) * unit / mass) * kLn2d);
-        }
-        return;
-      }
-      // rounding put the target between two segments: the sweep below decides
+      return;
     }
   }
 
   // 4 over the row: kept mass by segment, in index order (the weight of -inf is 0). Vectors without a kept
   // element cost their comparison only.
   const Weight weight = base.fresh();
-  auto kept_weights = [&](float* x, int col0, double* w) __attribute__((always_inline)) {
+  auto kept_doubles = [&](float* x, int col0, double* w) __attribute__((always_inline)) {
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < EPV; ++e) top = __builtin_elementwise_maximum(top, x[e]);
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) w[e] = 0.0;
-    if (__ballot(top >= cut.x) == 0ull) return;
+    if (__ballot(top >= cut.x) == 0ull) return false;
     mask(x, col0);
     weight.template eval<EPV>(x, w);
+    return true;
   };
-  auto equal = [&](float* x, int, double* w) __attribute__((always_inline)) {
+  auto kept_weights = [&](float* x, int col0, uint64_t* w) __attribute__((always_inline)) {
+    double wd[EPV];
+    if (!kept_doubles(x, col0, wd)) return;
 #pragma unroll
-    for (int e = 0; e < EPV; ++e) w[e] = x[e] == cut.x ? 1.0 : 0.0;
+    for (int e = 0; e < EPV; ++e) w[e] = fixed(wd[e]);
+  };
+  auto equal = [&](float* x, int, uint64_t* w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) w[e] = x[e] == cut.x ? 1ull : 0ull;
   };
   int at_seg;
-  double w, ahead;
+  float x_at;
+  uint64_t ahead;
   if (!whole) {
     __syncthreads();
-    double mine = 0.0;
+    uint64_t mine = 0ull;
     int equals = 0;
     each_segment<T, THREADS, G>(rv, nseg,
         [&](const u32x4& r, int c) {
           float x[EPV];
           Elem<T>::unpack(r, x);
-          if (ties > 0.0) {
+          if (ties > 0) {
 #pragma unroll
             for (int e = 0; e < EPV; ++e) equals += x[e] == cut.x ? 1 : 0;
           }
           double w[EPV];
-          kept_weights(x, rv.col0(c), w);
-          mine += total_of(w);
+          if (kept_doubles(x, rv.col0(c), w)) {
+            mine -= EPV * kAbove;
+#pragma unroll
+            for (int e = 0; e < EPV; ++e) mine += fixed_above(w[e]);
+          }
         },
         [&](int s) {
-          mine = wave_sum64(mine);
-          const float all_equals = ties > 0.0 ? wave_sum((float)equals) : 0.f;
-          if ((tid & 63) == 0) { sh.seg[s] = mine; sh.segm[s] = all_equals; }
-          mine = 0.0;
+          mine = wave_sum_u64(mine);
+          const int all_equals = ties > 0 ? wave_sum_i(equals) : 0;
+          if ((tid & 63) == 0) { sh.seg[s] = mine; sh.ties[s] = all_equals; }
+          mine = 0ull;
           equals = 0;
         });
     __syncthreads();
-    if (ties > 0.0) {
-      double mine = 0.0;
-      for (int i = tid; i < nseg; i += THREADS) mine += (double)sh.segm[i];
+    if (ties > 0) {
+      uint64_t mine = 0ull;
+      for (int i = tid; i < nseg; i += THREADS) mine += (uint64_t)sh.ties[i];
       int s_cut = nseg;
-      double before = 0.0;
+      uint64_t before = 0ull;
       cut.col = 0x7fffffff;
-      if (ties < uniform(block_reduce64<NW, Sum64>(mine, sh.red)))
-        cut.col = pick<T, THREADS, G>(rv, nseg, [&](int i) { return (double)sh.segm[i]; }, ties - 0.5, equal, sh, &w, &s_cut, &before);
-      const double each_w = weight(cut.x);
+      if ((uint64_t)ties < uniform(block_sum_int64<NW>(mine, sh.redu)))
+        cut.col = pick<T, THREADS, G>(rv, nseg, [&](int i) { return (uint64_t)sh.ties[i]; }, (uint64_t)ties, equal, sh, &x_at, &s_cut, &before);
+      const uint64_t each_w = fixed(weight(cut.x));
       __syncthreads();
       for (int i = tid; i < nseg; i += THREADS)
-        sh.seg[i] += each_w * (i < s_cut ? (double)sh.segm[i] : i == s_cut ? ties - before : 0.0);
+        sh.seg[i] += each_w * (i < s_cut ? (uint64_t)sh.ties[i] : i == s_cut ? (uint64_t)ties - before : (uint64_t)0);
       __syncthreads();
     }
   }
-  double mine = 0.0;
+  uint64_t mine = 0ull;
   for (int i = tid; i < nseg; i += THREADS) mine += sh.seg[i];
-  const double mass = block_reduce64<NW, Sum64>(mine, sh.red);
-  const int col = pick<T, THREADS, G>(rv, nseg, [&](int i) { return sh.seg[i]; }, u * mass, kept_weights, sh, &w, &at_seg, &ahead);
+  const double mass = uniform((double)block_sum_int64<NW>(mine, sh.redu));
+  const uint64_t goal = uniform((uint64_t)(u * mass)) + 1ull;
+  const int col = pick<T, THREADS, G>(rv, nseg, [&](int i) { return sh.seg[i]; }, goal, kept_weights, sh, &x_at, &at_seg, &ahead);
   if (tid == 0) {
     a.token[row] = col;
-    if (a.logprob != nullptr) a.logprob[row] = (float)(log2_64(w / mass) * kLn2d);
+    if (a.logprob != nullptr) a.logprob[row] = (float)(log2_64(weight(x_at) * unit / mass) * kLn2d);
   }
 }
 

@@ -4,7 +4,8 @@ uniform numbers, in one HIP launch.
 Nothing like it exists in the reference, whose kernel package stops at ``topk`` and ``softmax``
 (``forgemind/kernels/topk.py:273-297``, ``softmax.py:118-139``); the order of equal logits is that of
 its ``topk`` (``topk.py:13-16``). Random numbers are an input, so that a row's token depends on nothing
-but the row, its settings and its number: not on the batch, the launch or the device's generator.
+but the row, its settings and its number: not on the batch, the launch or the device's generator. (The
+kernel sums weights as integers, multiples of 2^-46 of the largest for rows of up to 2^17 columns.)
 """
 
 from __future__ import annotations
@@ -53,7 +54,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
 
     ``token`` (int64) is the first index, ascending, at which the running mass of what stays exceeds
     ``u`` times the whole; ``logprob`` (fp32) is the token's log-probability among what stays. Weights
-    and sums are held in 64 bits. A row without a distribution (it holds a NaN or ``+inf`` or nothing but
+    and sums are held in 64 bits, and a row gives the same bits whatever rows come with it. A row without a distribution (it holds a NaN or ``+inf`` or nothing but
     ``-inf``, or its temperature tensor holds a negative, infinite or NaN value) gets ``-1`` and NaN.
     Neither output is differentiable.
     """

@@ -77,7 +77,9 @@ int fm_kl_topk_bwd(const void* student, const void* idx, const void* teacher, co
  * NaN: off. Logits of -inf are never taken.
  * u: fp32 [n]. temperature, top_p, min_p: fp32 [n] or NULL for the number behind them for every row;
  * top_k: int32 [n] or NULL likewise. token: int64 [n]; logprob: fp32 [n] or NULL. logits may have any
- * alignment of their type. Weights and sums are held in 64 bits. v <= 2^20, n < 2^22 (FM_ERR_UNSUPPORTED
+ * alignment of their type. Weights are computed in 64 bits, rounded to multiples of 2^-fx (fx = 63 - log2 v
+ * rounded up, at most 50; where nothing cuts, the sums of 512 to 2048 columns are) and summed as integers: a
+ * row's token and logprob are the same bits whatever rows come with it. v <= 2^20, n < 2^22 (FM_ERR_UNSUPPORTED
  * past those). */
 int fm_sample(const void* logits, const float* u, const float* temperature, const int32_t* top_k,
               const float* top_p, const float* min_p, float temperature0, int top_k0, float top_p0,

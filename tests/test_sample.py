@@ -354,3 +354,31 @@ def test_sampled_listed_and_trained_on():
     assert abs(loss.item() - ref.mean().item()) <= 1e-5 * abs(ref.mean().item())
     bound = 2.0 ** -8 * grad.abs() / n + 300 * 2.0 ** -24 * size / n + 1e-38
     assert ((sd.grad.double().cpu() - grad / n).abs() <= bound).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt,v", [(F32, 32000), (BF16, 32000), (F16, 50257), (BF16, 9001)])
+def test_a_row_alone_is_the_row_among_many(dt, v):
+    """Token and log-probability are the same bits with more rows than compute units and with fewer,
+    where other workgroup sizes run. Half of the rows are one sequence of logits twice over, drawn at
+    u = 1/2: in exact arithmetic the border lies between the two, so any difference in the order of the
+    sums, or in how a weight is rounded, decides."""
+    n = 300
+    g = torch.Generator().manual_seed(v)
+    half = v // 2
+    x = torch.empty(n, v)
+    a = torch.randn(n, half, generator=g) * (0.05 + 3 * torch.rand(n, 1, generator=g))
+    x[:, :half], x[:, half:2 * half] = a, a
+    if v % 2:
+        x[:, -1] = -float("inf")
+    x[1::2], u = zipf(n // 2, v, v + 1)[0], torch.full((n,), 0.5)
+    u[1::2] = torch.rand(n // 2, generator=g)
+    x = x.to(dt)
+    xd, ud = x.to(DEV), u.to(DEV)
+    for kw in (dict(), dict(temperature=0.7), dict(min_p=1e-3), dict(min_p=1e-5), dict(min_p=0.2), dict(top_k=600),
+               dict(top_k=900), dict(top_k=3000), dict(top_k=5000, top_p=0.999), dict(top_p=0.5), dict(top_p=0.95),
+               dict(top_p=0.9999), dict(top_k=3000, min_p=1e-4), dict(top_p=0.99, min_p=1e-3)):
+        tok, lp = fm.kernels.sample_tokens(xd, ud, **kw)
+        for lo in range(0, n, 50):
+            t, l = fm.kernels.sample_tokens(xd[lo:lo + 50], ud[lo:lo + 50], **kw)
+            assert torch.equal(t, tok[lo:lo + 50]) and torch.equal(l, lp[lo:lo + 50]), (kw, lo)
