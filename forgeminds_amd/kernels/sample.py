@@ -20,8 +20,8 @@ from ._common import _note, fast_ok, tracing
 
 #: widest row of the kernel path; wider ones run the torch expression
 MAX_VOCAB = 1 << 20
-#: the kernel path takes fewer rows than this in one call
-MAX_ROWS = 1 << 22
+#: rows of one launch; more are drawn by several
+MAX_ROWS = (1 << 22) - 1
 
 
 def _setting(name: str, x, lead, like: torch.Tensor, dtype):
@@ -88,15 +88,19 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
         token, logprob = fb.sample_tokens(x2, u1, *(c.unsqueeze(-1) for c in cols))
         return token.view(lead), logprob.view(lead)
 
-    if logits.numel() == 0 or v > MAX_VOCAB or x2.shape[0] >= MAX_ROWS or tracing():
+    if logits.numel() == 0 or v > MAX_VOCAB or tracing():
         _note("sample_tokens shape")
-        return torch_path()
-    if logits.numel() >= 2 ** 31 * 4:
-        _note("sample_tokens numel")
         return torch_path()
     if not fast_ok(logits):
         return torch_path()
-    token, logprob = _hip.sample(x2.contiguous(), u1, *settings)
+    x2, n = x2.contiguous(), x2.shape[0]
+    if n <= MAX_ROWS:
+        token, logprob = _hip.sample(x2, u1, *settings)
+    else:
+        parts = [_hip.sample(x2[lo:lo + MAX_ROWS], u1[lo:lo + MAX_ROWS],
+                             *(s[lo:lo + MAX_ROWS] if torch.is_tensor(s) else s for s in settings))
+                 for lo in range(0, n, MAX_ROWS)]
+        token, logprob = (torch.cat(t) for t in zip(*parts))
     return token.view(lead), logprob.view(lead)
 
 

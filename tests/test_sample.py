@@ -382,3 +382,28 @@ def test_a_row_alone_is_the_row_among_many(dt, v):
         for lo in range(0, n, 50):
             t, l = fm.kernels.sample_tokens(xd[lo:lo + 50], ud[lo:lo + 50], **kw)
             assert torch.equal(t, tok[lo:lo + 50]) and torch.equal(l, lp[lo:lo + 50]), (kw, lo)
+
+
+@gpu
+def test_any_number_of_rows_and_elements_runs_on_the_kernel():
+    n, v = 2 ** 22 + 5, 3
+    fm.kernels.reset_stats()
+    x = torch.tensor([[0.0, 3.0, 1.0]], device=DEV).repeat(n, 1)
+    u = torch.rand(n, device=DEV)
+    temp = 0.5 + torch.rand(n, device=DEV)
+    tok, lp = fm.kernels.sample_tokens(x, u, temperature=temp, top_k=2)
+    assert tok.shape == (n,) and lp.shape == (n,)
+    for lo in (0, 2 ** 21, n - 7):
+        t, l = fm.kernels.sample_tokens(x[lo:lo + 7], u[lo:lo + 7], temperature=temp[lo:lo + 7], top_k=2)
+        assert torch.equal(t, tok[lo:lo + 7]) and torch.equal(l, lp[lo:lo + 7])
+    # 2^33 elements and more: 17 GB of logits
+    n, v = 67000, 128256
+    assert n * v > 2 ** 33
+    x, u = zipf(64, v, 33, BF16)
+    xd = x.to(DEV).repeat((n + 63) // 64, 1)[:n]
+    ud = u.to(DEV).repeat((n + 63) // 64)[:n]
+    tok, lp = fm.kernels.sample_tokens(xd, ud, top_k=50, top_p=0.9)
+    want = fm.kernels.sample_tokens(xd[:64], ud[:64], top_k=50, top_p=0.9)
+    rows = torch.arange(n, device=DEV) % 64
+    assert torch.equal(tok, want[0][rows]) and torch.equal(lp, want[1][rows])
+    assert fm.kernels.stats()["fallback"] == 0
