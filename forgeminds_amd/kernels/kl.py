@@ -422,7 +422,7 @@ def kl_div_topk(student: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor,
             or student.shape[-1] >= MAX_LIST_COLS or student.numel() // student.shape[-1] >= MAX_LIST_ROWS):
         _note("kl_div_topk shape")
         return fb.kl_div_topk(student, idx, teacher, teacher_lse, probs, tail, reduction, temperature)
-    if not _kernel_ok(student, teacher):
+    if not fast_ok(student, teacher):
         return fb.kl_div_topk(student, idx, teacher, teacher_lse, probs, tail, reduction, temperature)
     if not wants_grad(student):
         s2, i2, t2, lse_t = _list_rows(student, idx, teacher, teacher_lse, probs, tail)

@@ -715,3 +715,30 @@ def test_the_order_of_the_slots_changes_no_bit(dt, v, k):
         want = want or runs[0]
         for got in runs:
             assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+
+
+@gpu
+def test_students_past_two_to_the_33_elements_run_on_the_kernel():
+    # 17 GB of logits and as much gradient, rows that repeat every 64
+    n, v, k, m = 67000, 128256, 16, 64
+    assert n * v > 2 ** 33
+    g = torch.Generator().manual_seed(9)
+    s = (2 * torch.randn(m, v, generator=g)).to(BF16)
+    t, idx = (s.float() + 0.5 * torch.randn(m, v, generator=g)).topk(k)
+    idx[5::9] = -1
+    rows = torch.arange(n, device=DEV) % m
+    sd, idx, t = to_dev(s, idx, t)
+    big = sd.repeat((n + m - 1) // m, 1)[:n].requires_grad_(True)
+    live = (idx[rows, 0] >= 0).sum()
+    fm.kernels.reset_stats()
+    loss = fm.kernels.kl_div_topk(big, idx[rows], t[rows])
+    (grad,) = torch.autograd.grad(loss, big, torch.tensor(2.0 ** 17, device=DEV))
+    assert fm.kernels.stats()["fallback"] == 0
+    small = sd.clone().requires_grad_(True)
+    each = fm.kernels.kl_div_topk(small, idx, t, reduction="none")
+    (want,) = torch.autograd.grad(each, small, (2.0 ** 17 / live).expand(m))
+    total = each.detach().double()[rows].sum() / live
+    assert abs(loss.item() - total.item()) <= 2.0 ** -22 * total.item()
+    for at in (0, 5, 2 ** 31 // v, 2 ** 32 // v, 2 ** 33 // v - 1, 2 ** 33 // v, n - 1):
+        a, b = grad[at].float(), want[at % m].float()
+        assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 1e-30).all() and (at % m == 5) == (not b.any()), at
