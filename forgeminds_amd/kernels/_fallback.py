@@ -70,7 +70,10 @@ def kl_div_topk(student, idx, teacher, teacher_lse=None, probs: bool = False, ta
     Rows whose first slot is negative are skipped, other negative slots are empty, a repeated
     column counts once with the sum of its probabilities, a column past the row gives NaN.
     """
-    s = _wide(student)
+    live = idx[..., 0] >= 0
+    # a skipped row holds anything: nothing of it may meet a gradient of zero
+    idx = torch.where(live.unsqueeze(-1), idx, -1)
+    s = torch.where(live.unsqueeze(-1), _wide(student), 0.0)
     v = s.shape[-1]
     logp = torch.log_softmax(s / temperature, dim=-1)
     used = idx >= 0
@@ -96,7 +99,6 @@ def kl_div_topk(student, idx, teacher, teacher_lse=None, probs: bool = False, ta
         # rows without a bucket take a finite stand-in, so that no gradient meets an infinity
         out = torch.where(some.unsqueeze(-1), logp.masked_fill(listed, -float("inf")), logp)
         rows = rows + torch.where(some, left * (torch.log(torch.where(some, left, 1.0)) - torch.logsumexp(out, dim=-1)), 0.0)
-    live = used[..., 0]
     rows = torch.where(live, rows, 0.0)
     if reduction == "none":
         return rows.float() if rows.dtype != torch.float64 else rows

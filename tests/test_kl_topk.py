@@ -742,3 +742,27 @@ def test_students_past_two_to_the_33_elements_run_on_the_kernel():
     for at in (0, 5, 2 ** 31 // v, 2 ** 32 // v, 2 ** 33 // v - 1, 2 ** 33 // v, n - 1):
         a, b = grad[at].float(), want[at % m].float()
         assert ((a - b).abs() <= 2.0 ** -7 * b.abs() + 1e-30).all() and (at % m == 5) == (not b.any()), at
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("tail", ["renorm", "drop", "bucket"])
+def test_what_a_skipped_row_holds_does_not_matter(tail, dev):
+    # slot 0 is empty: NaN, infinities and columns past the row in what else the row holds change nothing
+    nan, inf = float("nan"), float("inf")
+    g = torch.Generator().manual_seed(3)
+    s = torch.randn(7, 12, generator=g)
+    idx = torch.randint(0, 12, (7, 3), generator=g)
+    idx[1:6, 0] = -1
+    t = torch.rand(7, 3, generator=g) * 0.3
+    lse = torch.full((7,), 4.0)
+    s[1], s[2], s[3, 5] = nan, -inf, inf
+    idx[4, 1] = 12
+    t[5, 1], t[5, 2], lse[5] = nan, inf, -inf
+    for probs in (False, True):
+        for reduction in ("none", "sum", "mean"):
+            x = s.to(dev).requires_grad_(True)
+            out = fm.kernels.kl_div_topk(x, idx.to(dev), t.to(dev), teacher_lse=lse.to(dev), probs=probs, tail=tail,
+                                         reduction=reduction)
+            (got,) = torch.autograd.grad(out.sum(), x)
+            assert torch.isfinite(out).all() and torch.isfinite(got).all() and (got[1:6] == 0).all(), (probs, reduction)
+            assert (got[[0, 6]] != 0).any(dim=-1).all()
