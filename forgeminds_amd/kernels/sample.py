@@ -34,8 +34,8 @@ def _setting(name: str, x, lead, like: torch.Tensor, dtype):
         raise ValueError(f"{name} is on {x.device}, the logits on {like.device}")
     if x.is_floating_point() != dtype.is_floating_point or x.dtype == torch.bool or x.is_complex():
         raise ValueError(f"{name} must be {'floating point' if dtype.is_floating_point else 'an integer'}, got {x.dtype}")
-    if dtype == torch.int32 and x.dtype != torch.int32:
-        x = x.clamp(-1, 2 ** 31 - 1)
+    if dtype == torch.int32 and x.dtype.itemsize >= 4 and x.dtype != torch.int32:
+        x = x.to(torch.int64).clamp(-1, 2 ** 31 - 1)
     return x.detach().to(dtype).contiguous().view(-1)
 
 

@@ -407,3 +407,24 @@ def test_any_number_of_rows_and_elements_runs_on_the_kernel():
     rows = torch.arange(n, device=DEV) % 64
     assert torch.equal(tok, want[0][rows]) and torch.equal(lp, want[1][rows])
     assert fm.kernels.stats()["fallback"] == 0
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("kind", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_top_k_of_every_integer_type(kind, dev):
+    x, u = zipf(5, 700, 12)
+    top_k = torch.tensor([0, 1, 7, 100, 127])
+    want = fm.kernels.sample_tokens(x.to(dev), u.to(dev), top_k=top_k.to(dev))
+    got = fm.kernels.sample_tokens(x.to(dev), u.to(dev), top_k=top_k.to(kind).to(dev))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for i in range(5):
+        check_row(x[i].numpy(), u[i].item(), got[0][i].item(), got[1][i].item(), top_k=int(top_k[i]))
+    if kind == torch.int64:       # past 32 bits: everything stays
+        high = torch.tensor([2 ** 32 + 5, 2 ** 40, 2 ** 31, 2 ** 63 - 1, 700], device=dev)
+        off = fm.kernels.sample_tokens(x.to(dev), u.to(dev))
+        for t in (high, high.to(torch.uint64)):
+            assert torch.equal(fm.kernels.sample_tokens(x.to(dev), u.to(dev), top_k=t)[0], off[0])
+    if kind != torch.uint8:       # negative: off, also below the least of 32 bits
+        low = torch.full((5,), torch.iinfo(kind).min, dtype=kind, device=dev)
+        off = fm.kernels.sample_tokens(x.to(dev), u.to(dev))
+        assert torch.equal(fm.kernels.sample_tokens(x.to(dev), u.to(dev), top_k=low)[0], off[0])
