@@ -65,9 +65,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
         raise ValueError(f"u must be floating point {tuple(lead)}, got {tuple(u.shape)} {u.dtype}")
     if u.device != logits.device:
         raise ValueError(f"u is on {u.device}, the logits on {logits.device}")
-    if not torch.is_tensor(temperature) and not 0 <= temperature < math.inf:
-        raise ValueError(f"temperature must be finite and not negative, got {temperature}")
-    if not torch.is_tensor(top_k) and (int(top_k) != top_k or top_k < 0):
+    if not torch.is_tensor(temperature) and not 0 <= temperature <= torch.finfo(torch.float32).max:
+        raise ValueError(f"temperature must be finite in 32 bits and not negative, got {temperature}")
+    if not torch.is_tensor(top_k) and (not 0 <= top_k < math.inf or int(top_k) != top_k):
         raise ValueError(f"top_k must be a non-negative integer, got {top_k}")
     for name, x in (("top_p", top_p), ("min_p", min_p)):
         if not torch.is_tensor(x) and not 0 <= x <= 1:

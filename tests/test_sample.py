@@ -428,3 +428,13 @@ def test_top_k_of_every_integer_type(kind, dev):
         low = torch.full((5,), torch.iinfo(kind).min, dtype=kind, device=dev)
         off = fm.kernels.sample_tokens(x.to(dev), u.to(dev))
         assert torch.equal(fm.kernels.sample_tokens(x.to(dev), u.to(dev), top_k=low)[0], off[0])
+
+
+def test_numbers_that_32_bits_do_not_hold_are_refused():
+    x, u = zipf(2, 20, 1)
+    for kw in [dict(temperature=1e39), dict(temperature=3.5e38), dict(top_k=float("inf")), dict(top_k=float("nan"))]:
+        with pytest.raises(ValueError):
+            fm.kernels.sample_tokens(x, u, **kw)
+    a = fm.kernels.sample_tokens(x, u, temperature=torch.finfo(F32).max, top_k=2 ** 70)
+    b = fm.kernels.sample_tokens(x * 0, u)
+    assert torch.equal(a[0], b[0])
