@@ -889,7 +889,7 @@ int check(const char* what, int64_t n, int64_t v, int k, int dtype, int index_bi
   FM_CHECK_ARG(index_bits == 32 || index_bits == 64, "%s: index_bits must be 32 or 64 (got %d)", what, index_bits);
   FM_CHECK_ARG(kind == FM_TEACHER_LOGITS || kind == FM_TEACHER_PROBS, "%s: bad teacher_kind %d", what, kind);
   FM_CHECK_ARG(tail == FM_TAIL_RENORM || tail == FM_TAIL_DROP || tail == FM_TAIL_BUCKET, "%s: bad tail %d", what, tail);
-  FM_CHECK_ARG(temperature > 0.0 && temperature <= 3.0e38, "%s: temperature must be positive and finite", what);
+  FM_CHECK_ARG(temperature > 0.0 && temperature < (double)INFINITY, "%s: temperature must be positive and finite", what);
   // (a launch has less than 2^32 threads, and a row up to 1024; offsets inside a row are 32 bits of bytes)
   if (n >= (1LL << 22) || v >= (1LL << 30) || k > kMaxList) {
     fm_host::set_error("%s: n must be below 2^22, v below 2^30 and k at most %d", what, kMaxList);

@@ -766,3 +766,17 @@ def test_what_a_skipped_row_holds_does_not_matter(tail, dev):
             (got,) = torch.autograd.grad(out.sum(), x)
             assert torch.isfinite(out).all() and torch.isfinite(got).all() and (got[1:6] == 0).all(), (probs, reduction)
             assert (got[[0, 6]] != 0).any(dim=-1).all()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+def test_temperatures_past_fp32(dev):
+    # any positive finite number: past 1e30 the student is even and the loss log v minus the list's entropy
+    s, idx, _t, _ = make(4, 500, 6, seed=2)
+    q = torch.softmax(torch.randn(4, 6, generator=torch.Generator().manual_seed(1)), -1)
+    want = math.log(500) + (q.double() * torch.log(q.double())).sum(-1)
+    for T in (1e32, 3.5e38, 1e200):
+        x = s.to(dev).requires_grad_(True)
+        rows = fm.kernels.kl_div_topk(x, idx.to(dev), q.to(dev), probs=True, tail="drop", reduction="none", temperature=T)
+        assert ((rows.detach().double().cpu() - want).abs() <= loss_tol(500, want) + (1 - q.double().sum(-1)).abs() * 7).all()
+        (g,) = torch.autograd.grad(rows.sum(), x)
+        assert (g.abs() <= 1.1 / T).all()
