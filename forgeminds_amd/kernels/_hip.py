@@ -476,9 +476,10 @@ def kl_topk_fwd(s2, idx2, teacher2, lse_t, probs: bool, tail: str, temperature: 
     dev = s2.device
     rows = torch.empty(n, device=dev, dtype=torch.float32)
     stats = torch.empty(n, 4, device=dev, dtype=torch.float32)
-    scal = torch.empty(2, device=dev, dtype=torch.float32) if reduction != "none" else None
+    # (tensors of their own: the loss goes to the caller, who may write to it, n_valid to the backward)
+    loss, n_valid = ((torch.empty((), device=dev, dtype=torch.float32), torch.empty((), device=dev, dtype=torch.float32))
+                     if reduction != "none" else (None, None))
     k, bits, tdt, kind, tl, temp = _list_args(idx2, teacher2, probs, tail, temperature)
-    loss, n_valid = (scal[0], scal[1]) if scal is not None else (None, None)
     with _guard(dev):
         _check(lib().fm_kl_topk_fwd(_ptr(s2), _ptr(idx2), _ptr(teacher2), _ptr(lse_t), _ptr(rows), _ptr(stats),
                                     _ptr(loss), _ptr(n_valid), n, v, k, dtype_code(s2.dtype), bits, tdt, kind, tl,
@@ -493,15 +494,16 @@ def kl_topk_loss_grad(s2, idx2, teacher2, lse_t, probs: bool, tail: str, tempera
     _dense(s2, idx2, teacher2, lse_t)
     n, v = s2.shape
     dev = s2.device
-    buf = torch.empty(n + 2, device=dev, dtype=torch.float32)
+    loss = torch.empty((), device=dev, dtype=torch.float32)
+    buf = torch.empty(n + 1, device=dev, dtype=torch.float32)      # n_valid, then the rows
     g = s2 if inplace else torch.empty_like(s2)
     k, bits, tdt, kind, tl, temp = _list_args(idx2, teacher2, probs, tail, temperature)
     with _guard(dev):
-        _check(lib().fm_kl_topk_loss_grad(_ptr(s2), _ptr(idx2), _ptr(teacher2), _ptr(lse_t), buf.data_ptr() + 8,
-                                          None, buf.data_ptr(), buf.data_ptr() + 4, _ptr(g), n, v, k,
+        _check(lib().fm_kl_topk_loss_grad(_ptr(s2), _ptr(idx2), _ptr(teacher2), _ptr(lse_t), buf.data_ptr() + 4,
+                                          None, _ptr(loss), buf.data_ptr(), _ptr(g), n, v, k,
                                           dtype_code(s2.dtype), bits, tdt, kind, tl, temp, REDUCE[reduction],
                                           _stream(s2)), "fm_kl_topk_loss_grad")
-    return buf[0], g, buf[2:]
+    return loss, g, buf[1:]
 
 
 def kl_topk_bwd(s2, idx2, teacher2, lse_t, stats, n_valid, grad_out, per_row: bool, probs: bool, tail: str,

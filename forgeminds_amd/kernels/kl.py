@@ -344,7 +344,8 @@ class _KLTopkFn(torch.autograd.Function):
             return loss
         loss, rows, stats, n_valid = _hip.kl_topk_fwd(s2.detach(), i2, t2, lse_t, probs, tail, temperature, reduction)
         ctx.save_for_backward(s2, i2, t2, lse_t, stats, n_valid if reduction == "mean" else None)
-        return rows.view(student.shape[:-1]) if reduction == "none" else loss
+        # (not as a view: autograd lets no one write to a view made in here)
+        return rows.view(student.shape[:-1]).detach() if reduction == "none" else loss
 
     @staticmethod
     @once_differentiable

@@ -780,3 +780,22 @@ def test_temperatures_past_fp32(dev):
         assert ((rows.detach().double().cpu() - want).abs() <= loss_tol(500, want) + (1 - q.double().sum(-1)).abs() * 7).all()
         (g,) = torch.autograd.grad(rows.sum(), x)
         assert (g.abs() <= 1.1 / T).all()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_the_loss_may_be_added_to_in_place(reduction, dt, dev):
+    s, idx, t, _ = make(6, 300, 4, dt, seed=3)
+    grads = []
+    for inplace in (False, True):
+        x = s.to(dev).view(2, 3, 300).requires_grad_(True)
+        loss = fm.kernels.kl_div_topk(x, idx.view(2, 3, 4).to(dev), t.view(2, 3, 4).to(dev), reduction=reduction)
+        aux = (x.float() ** 2).sum()
+        if inplace:
+            loss += aux
+            loss *= 3.0
+        else:
+            loss = (loss + aux) * 3.0
+        grads.append(torch.autograd.grad(loss.sum(), x)[0])
+    assert torch.equal(*grads)
