@@ -17,8 +17,9 @@
 //
 // Measured, lists of 64, loss and gradient from one launch: [8192,32000] bf16 204 us (5.1 TB/s, the rate of a
 // copy), [4096,128256] bf16 418 us (5.0), [1024,128256] fp32 with lists of 256 204 us (5.1); losses alone,
-// [4096,128256] bf16, 158 to 181 us (5.8 to 6.6 TB/s); loss and gradient in two launches, [1021,50257] fp16,
-// 24 and 43 us; [16,32000] bf16 14 us, where the steps of one row count.
+// [4096,128256] bf16, 157 to 185 us (5.7 to 6.7 TB/s); loss and gradient in two launches, [1021,50257] fp16,
+// 24 and 43 us, one loss a row at [8192,32000] bf16 102 and 183; [16,32000] bf16 14 us, where the steps of
+// one row count.
 #include "../../include/fm_hip_tokens.h"
 #include "fm_f64.hip.h"
 

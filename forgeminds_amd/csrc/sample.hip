@@ -33,11 +33,17 @@
 // Weights are computed for the candidates only, unless the mass of the whole row is asked for.
 //
 // What bounds it: the arithmetic of those weights, some 27 instructions an element with the histogram, on
-// the row's one compute unit; memory is far (256 rows of 128256 bf16 are 10 us of reading). Measured, bf16,
-// [1,128256]: unfiltered 28 us, min-p 12, top-k 50 25, top-p 0.9 39 (maximum 4, histogram 23, list 6, cut,
-// token and launch 6), 88 on a flat row, most of whose elements are kept. [256,128256]: 33, 24, 36, 54, 101.
-// [512,128256]: 55, 41, 48, 87, 171. [1024,32000]: 35, 25, 51, 54, 110. Splitting a row over workgroups
-// would divide the 23 us alone, for a second launch and partial histograms in memory: 10 us at best.
+// the row's one compute unit; memory is far (256 rows of 128256 bf16 are 10 us of reading), but in the
+// unfiltered sweep its 16 us ([512,50257] fp32) and the weights' 14 hardly overlap. Measured, bf16, us of the
+// kernel, rows of power laws with exponents from 1 to 2 (the slowest row decides: at exponent 1 the list
+// overflows and the kept weights are evaluated a second time):
+//                 unfiltered  min-p 0.02  top-k 50  top-p 0.9  top-p 0.9, flat rows
+//   [1,128256]            27          12        23         40                    99
+//   [256,128256]          34          24        33        105                   113
+//   [512,128256]          55          40        46        176                   188
+//   [1024,32000]          33          26        45        101                   106
+// Of the 40 us for one row the maximum takes 4, the histogram 23, the list 6. The first two would divide over
+// several workgroups a row (their partial results are integers and a maximum); that has not been tried.
 //
 // What keeps it small counts too: the code that a call runs through fits the instruction cache (64 KB for
 // two compute units). Putting the row's two partial vectors together in place, in every sweep, made each
@@ -1119,10 +1125,11 @@ void launch(const void* logits, const SampleArgs& a, int64_t n, hipStream_t st) 
   const int64_t nvec = a.v / Elem<T>::kVec + 2;
 #define GO(TH, G) FM_LAUNCH((sample_kernel<T, TH, G>), dim3((unsigned)n), dim3(TH), 0, st, static_cast<const T*>(logits), a)
   // Short rows: four waves, a block of 64 vectors a segment, so that each wave has segments to sweep
-  // ([2048,8000] bf16 top-p 0.9: 70 us with 512 threads, 56 with these). Rows for which there is a compute
-  // unit each: all of its waves ([1,128256] top-p 0.9: 51 us with 512 threads when it was 45 with these; a
-  // short list costs up to 6 us more). More rows: half-size workgroups, two rows a unit in different phases ([1024,32000]
-  // top-p 0.9: 99 us with the large ones, 66 with these).
+  // ([2048,8000] bf16 top-p 0.9: 84 us with 512 threads, 68 with these). Rows for which there is a compute
+  // unit each: all of its waves ([1,128256] top-p 0.95: 46 us with 512 threads, 40 with these; [256,128256]
+  // top-k 50 is slower by it, 30 and 33). More rows: half-size workgroups, two rows a unit in different phases
+  // ([1024,32000] top-p 0.9: 130 us with the large ones, 103 with these; where a quarter of 512 rows of min-p
+  // is flat it is the other way round, 79 and 88). The choice does not show in the results.
   if (nvec <= 1024) GO(256, 1);
   else if (n <= fm_host::num_cus()) GO(1024, 4);
   else GO(512, 4);

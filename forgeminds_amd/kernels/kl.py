@@ -310,7 +310,7 @@ def kl_div_logits_topk(student: torch.Tensor, teacher: torch.Tensor, k: int,
 # ------------------------------------------------------------------ from a teacher's list
 #: longest list a row may have on the kernel path
 MAX_LIST = 1024
-#: the kernel path takes fewer rows than this in one call, and fewer columns
+#: the kernel path takes fewer rows than this in one call, and fewer columns; more run the torch expression
 MAX_LIST_ROWS = 1 << 22
 MAX_LIST_COLS = 1 << 30
 _TAILS = ("renorm", "drop", "bucket")
@@ -395,6 +395,9 @@ def kl_div_topk(student: torch.Tensor, idx: torch.Tensor, teacher: torch.Tensor,
 
     Returns the fp32 loss (``"none"``: one per row). The teacher is a constant. ``temperature`` has
     no ``T**2`` factor. ``reuse`` / ``retain`` as in :func:`kl_div_logits`.
+
+    Traced calls (``torch.compile``) run the torch expression, with several fp32 tensors of the student's
+    shape, and so do lists longer than ``MAX_LIST``.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be mean|sum|none, got {reduction!r}")

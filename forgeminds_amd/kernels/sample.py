@@ -57,6 +57,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     and sums are held in 64 bits, and a row gives the same bits whatever rows come with it. A row without a distribution (it holds a NaN or ``+inf`` or nothing but
     ``-inf``, or its temperature tensor holds a negative, infinite or NaN value) gets ``-1`` and NaN.
     Neither output is differentiable.
+
+    Traced calls (``torch.compile``) and rows wider than ``MAX_VOCAB`` run the torch expression: a 64-bit
+    sort of every row.
     """
     if logits.dim() < 1 or logits.shape[-1] == 0 or not logits.is_floating_point():
         raise ValueError(f"sample_tokens needs floating-point logits [..., V], got {tuple(logits.shape)} {logits.dtype}")
