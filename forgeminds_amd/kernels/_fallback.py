@@ -74,8 +74,11 @@ def kl_div_topk(student, idx, teacher, teacher_lse=None, probs: bool = False, ta
     # a skipped row holds anything: nothing of it may meet a gradient of zero
     idx = torch.where(live.unsqueeze(-1), idx, -1)
     s = torch.where(live.unsqueeze(-1), _wide(student), 0.0)
+    if temperature < 1:       # the lowest fp32 value (a mask) divided by it leaves fp32
+        s = s.double()
+    z = s / temperature
     v = s.shape[-1]
-    logp = torch.log_softmax(s / temperature, dim=-1)
+    logp = torch.log_softmax(z, dim=-1)
     used = idx >= 0
     col = idx.long().clamp(0, v - 1)
     # the teacher's few values in the widest type at hand
@@ -97,12 +100,18 @@ def kl_div_topk(student, idx, teacher, teacher_lse=None, probs: bool = False, ta
         left = torch.where(listed.all(dim=-1) | (left == 0), 0.0, left)
         some = left != 0
         # rows without a bucket take a finite stand-in, so that no gradient meets an infinity
-        out = torch.where(some.unsqueeze(-1), logp.masked_fill(listed, -float("inf")), logp)
-        rows = rows + torch.where(some, left * (torch.log(torch.where(some, left, 1.0)) - torch.logsumexp(out, dim=-1)), 0.0)
+        out = torch.where(some.unsqueeze(-1), z.masked_fill(listed, -float("inf")), z)
+        # sums against maxima of their own: next to a mask's 3e38 the log of a sum has no digit left
+        top, top_out = (t.detach().amax(dim=-1, keepdim=True) for t in (z, out))
+        top_out = torch.where(torch.isinf(top_out), 0.0, top_out)
+        log_rest = ((top_out - top).squeeze(-1) + torch.logsumexp(out - top_out, dim=-1)
+                    - torch.logsumexp(z - top, dim=-1))
+        rows = rows + torch.where(some, left * (torch.log(torch.where(some, left, 1.0)) - log_rest), 0.0)
     rows = torch.where(live, rows, 0.0)
+    dtype = torch.promote_types(student.dtype, torch.float32)
     if reduction == "none":
-        return rows.float() if rows.dtype != torch.float64 else rows
-    total = rows.sum()
+        return rows.to(dtype)
+    total = rows.sum().to(dtype)
     if reduction == "mean":
         total = total / live.sum().clamp(min=1).to(total.dtype)
     return total

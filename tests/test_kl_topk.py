@@ -799,3 +799,31 @@ def test_the_loss_may_be_added_to_in_place(reduction, dt, dev):
             loss = (loss + aux) * 3.0
         grads.append(torch.autograd.grad(loss.sum(), x)[0])
     assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("T", [0.7, 1.0, 2.0])
+@pytest.mark.parametrize("dt", [F32, BF16, torch.float64])
+def test_bucket_over_the_lowest_values_on_the_torch_path(dt, T):
+    v, k, low = 300, 64, torch.finfo(BF16 if dt == BF16 else F32).min
+    g = torch.Generator().manual_seed(v)
+    s = torch.randn(7, v, generator=g)
+    idx = torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(7)])
+    q = torch.softmax(torch.randn(7, k, generator=g), -1) * 0.9
+    out = torch.ones(7, v, dtype=torch.bool).scatter_(1, idx, False)
+    s[0][out[0]] = low
+    s[1][out[1]] = low
+    s[1, ::2] = torch.where(out[1, ::2], -float("inf"), s[1, ::2])
+    s[2] = low
+    s[4][~out[4]] = low
+    s[5][~out[5]] = low
+    s[5][out[5]] = low / 2
+    s = s.to(dt)
+    loss, grad, size = low_reference(s, idx, q, T)
+    for reduction in ("none", "sum"):
+        x = s.clone().requires_grad_(True)
+        got = fm.kernels.kl_div_topk(x, idx, q, probs=True, tail="bucket", temperature=T, reduction=reduction)
+        assert got.dtype == (torch.float64 if dt == torch.float64 else F32)
+        tol = loss_tol(v, loss) + U * loss.abs()
+        assert agrees(got, loss, tol) if reduction == "none" else agrees(got, loss.sum(), tol.sum() + U * loss.sum().abs())
+        (gr,) = torch.autograd.grad(got.sum(), x)
+        check_grad(gr, grad, size, F32 if dt == torch.float64 else dt, v, what=reduction)
