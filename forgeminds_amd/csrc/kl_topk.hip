@@ -905,6 +905,7 @@ ListArgs list_args(const void* idx, const void* teacher, const float* lse, int k
   a.idx = idx; a.teacher = teacher; a.teacher_lse = lse; a.k = k; a.idx64 = index_bits == 64;
   a.teacher_dtype = teacher_dtype; a.probs = kind; a.tail = tail; a.inv_t = 1.0 / temperature;
   a.c = (float)(1.4426950408889634074 / temperature);
+  if (a.c == 0.f) a.c = 1.40129846e-45f;       // past 1e45: every finite logit counts the same, and -inf * c is -inf
   return a;
 }
 

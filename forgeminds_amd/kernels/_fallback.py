@@ -74,7 +74,7 @@ def kl_div_topk(student, idx, teacher, teacher_lse=None, probs: bool = False, ta
     # a skipped row holds anything: nothing of it may meet a gradient of zero
     idx = torch.where(live.unsqueeze(-1), idx, -1)
     s = torch.where(live.unsqueeze(-1), _wide(student), 0.0)
-    if temperature < 1:       # the lowest fp32 value (a mask) divided by it leaves fp32
+    if not 1 <= temperature <= 1e38:       # the lowest fp32 value (a mask) divided by it leaves fp32, or it does itself
         s = s.double()
     z = s / temperature
     v = s.shape[-1]

@@ -827,3 +827,22 @@ def test_bucket_over_the_lowest_values_on_the_torch_path(dt, T):
         assert agrees(got, loss, tol) if reduction == "none" else agrees(got, loss.sum(), tol.sum() + U * loss.sum().abs())
         (gr,) = torch.autograd.grad(got.sum(), x)
         check_grad(gr, grad, size, F32 if dt == torch.float64 else dt, v, what=reduction)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("T", [1e20, 2e38, 1e45, 1e200])
+def test_masked_logits_at_far_temperatures(T, dev):
+    # even over what the mask leaves: loss log 500 minus the list's entropy, -inf columns without gradient
+    n, v = 3, 1000
+    s = torch.randn(n, v, generator=torch.Generator().manual_seed(5))
+    s[:, 1::2] = -float("inf")
+    idx = torch.arange(0, 12, 2).repeat(n, 1)
+    q = torch.softmax(torch.randn(n, 6, generator=torch.Generator().manual_seed(6)), -1)
+    want = math.log(500) * q.double().sum(-1) + (q.double() * torch.log(q.double())).sum(-1)
+    for reduction in ("none", "sum"):
+        x = s.to(dev).requires_grad_(True)
+        got = fm.kernels.kl_div_topk(x, idx.to(dev), q.to(dev), probs=True, tail="drop", temperature=T, reduction=reduction)
+        ref = want if reduction == "none" else want.sum()
+        assert ((got.detach().double().cpu() - ref).abs() <= 3 * loss_tol(v, ref)).all()
+        (g,) = torch.autograd.grad(got.sum(), x)
+        assert not g.isnan().any() and (g[:, 1::2] == 0).all()
